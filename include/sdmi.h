@@ -279,6 +279,40 @@ int sdmi_attention_log2q(const void* q, int ldq, int64_t sq, const void* k, int 
                          int ldv, int64_t sv, void* o, int ldo, int64_t so, int batch, int heads, int nq, int nkv,
                          void* stream);
 
+/* ---- cross-attention to encoder states of another length.  The reference has its rectangular case only
+ *      (layers/SpatialTransformer.py:70-95: every sample its own 77 tokens, mask=None); sdmi_attention runs that one.
+ *      q, o: (batch, nq, heads * dim); k, v: (contexts, nkv, kv_heads * dim), h16 token-major views with row strides ld* and
+ *      element strides s* per sample / context.  Sample b reads context index[b] (int32; NULL: its own one, or the only one),
+ *      query head h the key head h * kv_heads / heads, key j only where j < lens[context] (int32 [contexts]; NULL: nkv) and,
+ *      with regions, where (query_regions[b * sqr + i] & key_regions[context * skr + j]) != 0: sets of up to 32 regions that a
+ *      position of the picture and a token of the prompt belong to.
+ *        o[b][i] = sum_j softmax_j(scale q.k) v over the keys that i sees; a row that sees none is 0.
+ *      Memory of keys at or past lens[context] is not read, and a key in no region may hold anything (NaN too); every other key
+ *      has to be finite.  lens outside [0, nkv] count as the nearer end; an index outside [0, contexts) sees nothing.
+ *      heads a multiple of kv_heads, dim a multiple of 8 up to 256, any nq >= 1 and nkv >= 0.  ws: scratch of
+ *      sdmi_cross_attention_ws_bytes for few rows over long states, whose keys are cut into pieces that a second launch joins
+ *      in a fixed order; with NULL or fewer bytes they are not cut.  Calls that may overlap in time need a workspace each. */
+int sdmi_cross_attention(const void* q, int ldq, int64_t sq, const void* k, int ldk, int64_t sk, const void* v, int ldv, int64_t sv,
+                         void* o, int ldo, int64_t so, int batch, int contexts, int heads, int kv_heads, int dim, int nq, int nkv,
+                         const int32_t* index, const int32_t* lens, const uint32_t* query_regions, int64_t sqr,
+                         const uint32_t* key_regions, int64_t skr, float scale, void* ws, int64_t ws_bytes, void* stream);
+int64_t sdmi_cross_attention_ws_bytes(int batch, int heads, int kv_heads, int dim, int nq, int nkv);
+
+/* ---- low-rank adapters of many requests beside one shared projection (no counterpart in the reference, whose Linears at
+ *      layers/SpatialTransformer.py:62-66 have one set of weights):
+ *        out[m] = x[m] w^T + t[m] b[id]^T (+ bias) (+ residual[m]),  t[m] = scale[id] x[m] a[id]^T,  id = ids[m / rows_per_id]
+ *      x [m][k], w [n][k], out / residual [m][n]: h16, as sdmi_gemm (out may be residual's memory).  lora_a h16
+ *      [adapters][groups * rank][k], lora_b h16 [adapters][n][rank], lora_scale fp32 [adapters], ids int32
+ *      [ceil(m / rows_per_id)]; an id outside [0, adapters) leaves its rows without an adapter.  groups > 1: w stacks that many
+ *      projections along n; group g is columns [g n / groups, (g + 1) n / groups) and rows [g rank, (g + 1) rank) of lora_a.
+ *      Adapters of smaller rank are padded with zeros (sdmi_pack_linear, sdmi_f32_to_h16_rows write both layouts).  n, k, rank
+ *      multiples of 8, rank up to 256; flags: SDMI_F_BIAS, SDMI_F_RESIDUAL; ws: scratch of sdmi_lora_gemm_ws_bytes, one per call
+ *      that may overlap in time. */
+int sdmi_lora_gemm(const void* x, int ldx, const void* w, int ldw, void* out, int ldo, int m, int n, int k, const float* bias,
+                   const void* residual, int ldr, const void* lora_a, const void* lora_b, const float* lora_scale, int adapters,
+                   int rank, int groups, const int32_t* ids, int rows_per_id, uint32_t flags, void* ws, int64_t ws_bytes, void* stream);
+int64_t sdmi_lora_gemm_ws_bytes(int m, int n, int k, int rank, int groups);
+
 /* ---- fused flash attention, ONE head of dim 512: the VAE mid block's attention (layers/SpatialTransformer.py:132-161,
  *      xformers.ops.memory_efficient_attention on (B, HW, 512)) without an N x N score buffer.  q/k/v/o are h16 token-major
  *      (B, n, >= 512) views with row strides ld* and per-batch element strides s*; o = softmax(q k^T * scale) v. */

@@ -570,6 +570,92 @@ def cross_attention_lnq(a, ln_mod, to_q_weight, k, v, heads, out=None):
     return o
 
 
+def _own_device(what, *tensors):
+    """The kernels run on the current device's current stream: every tensor has to live there."""
+    cur = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.device.index != cur):
+            raise L.SdmiError("%s: a tensor is on %s, the current device is cuda:%d" % (what, t.device, cur))
+
+
+def _int32(t, shape, what):
+    if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous()):
+        raise L.SdmiError("%s: expected contiguous int32 %s, got %s %s" % (what, shape, t.dtype, tuple(t.shape)))
+    return 0 if t is None else t.data_ptr()
+
+
+def cross_attention(q, k, v, heads, kv_heads=None, dim=64, scale=None, index=None, lens=None, query_regions=None, key_regions=None, out=None):
+    """softmax(scale q k^T) v per head over encoder states of another length (sdmi_cross_attention).  q: (b, nq) tokens of
+    heads * dim channels; k, v: (contexts, nkv) tokens of kv_heads * dim; all column views of token buffers.  index (b,): the
+    context each sample reads (default: its own, or the only one); lens (contexts,): keys of each context that exist;
+    query_regions (b, nq) and key_regions (contexts, nkv): sets of regions as 32-bit words, a query sees the keys its set
+    meets.  All int32 device tensors, read by the kernel (a captured graph sees later contents).  scale: default dim ** -0.5.
+    A row that sees no key is 0."""
+    kv_heads = heads if kv_heads is None else kv_heads
+    n, nkv = k.n, k.hw
+    o = out if out is not None else new_act(q.n, q.h, q.w, heads * dim, q.device)
+    if (q.c, k.c, v.c) != (heads * dim, kv_heads * dim, kv_heads * dim) or (v.n, v.hw) != (n, nkv) or (o.n, o.hw, o.c) != (q.n, q.hw, heads * dim):
+        raise L.SdmiError("cross_attention: q (%d,%d,%d) / k (%d,%d,%d) / v (%d,%d,%d) / out (%d,%d,%d) do not match %d heads on %d key heads of %d" %
+                          (q.n, q.hw, q.c, n, nkv, k.c, v.n, v.hw, v.c, o.n, o.hw, o.c, heads, kv_heads, dim))
+    _own_device("cross_attention", q.buf, k.buf, v.buf, o.buf, index, lens, query_regions, key_regions)
+    ip, lp = _int32(index, (q.n,), "cross_attention: index"), _int32(lens, (n,), "cross_attention: lens")
+    qr, kr = _int32(query_regions, (q.n, q.hw), "cross_attention: query_regions"), _int32(key_regions, (n, nkv), "cross_attention: key_regions")
+    need = L.load().sdmi_cross_attention_ws_bytes(q.n, heads, kv_heads, dim, q.hw, nkv)
+    ws = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None     # the call's own: two graphs never share it
+    o.rstats = o.normed = None
+    o.stats.pop(o.off, None)
+    L.call("sdmi_cross_attention", q.ptr, q.ld, q.hw * q.ld, k.ptr, k.ld, nkv * k.ld, v.ptr, v.ld, nkv * v.ld, o.ptr, o.ld, o.hw * o.ld, q.n, n, heads,
+           kv_heads, dim, q.hw, nkv, ip, lp, qr, q.hw, kr, nkv, dim ** -0.5 if scale is None else float(scale), _ptr(ws), need, _stream())
+    return o
+
+
+class LoraPack(object):
+    """Adapters of one projection in the layout of sdmi_lora_gemm: a h16 (adapters, groups * rank, k), b h16 (adapters, n, rank),
+    scale fp32 (adapters,)."""
+    __slots__ = ("a", "b", "scale", "adapters", "rank", "groups")
+
+    def __init__(self, a, b, scale):
+        h = act_dtype()
+        if a.dim() != 3 or b.dim() != 3 or a.dtype != h or b.dtype != h or not a.is_contiguous() or not b.is_contiguous() or a.shape[0] != b.shape[0] or \
+                b.shape[2] == 0 or a.shape[1] % b.shape[2]:
+            raise L.SdmiError("LoraPack: a (adapters, groups * rank, k) and b (adapters, n, rank) are contiguous %s, got %s %s and %s %s" %
+                              (h, a.dtype, tuple(a.shape), b.dtype, tuple(b.shape)))
+        if scale.dtype != torch.float32 or tuple(scale.shape) != (a.shape[0],) or not scale.is_contiguous():
+            raise L.SdmiError("LoraPack: scale is contiguous fp32 (%d,), got %s %s" % (a.shape[0], scale.dtype, tuple(scale.shape)))
+        self.a, self.b, self.scale = a, b, scale
+        self.adapters, self.rank, self.groups = a.shape[0], b.shape[2], a.shape[1] // b.shape[2]
+
+
+def lora_gemm(a, wp, n_out, lora, ids, bias=None, residual=None, out=None):
+    """Token GEMM with a low-rank adapter per request (sdmi_lora_gemm): rows = n*hw of `a`, W packed [n_out][a.c], lora: LoraPack.
+    ids: int32 device tensor whose length divides the rows: entry i is the adapter of rows [i * rows / len(ids), ...), anything
+    outside [0, adapters) for none; read by the kernel (a captured graph sees later contents)."""
+    m = a.n * a.hw
+    res = out if out is not None else new_act(a.n, a.h, a.w, n_out, a.device)
+    if (res.n * res.hw, res.c) != (m, n_out):
+        raise L.SdmiError("lora_gemm: `out` holds %d rows x %d channels, the product has %d x %d" % (res.n * res.hw, res.c, m, n_out))
+    if tuple(wp.shape) != (n_out, a.c) or wp.stride(1) != 1 or lora.a.shape[2] != a.c or lora.b.shape[1] != n_out:
+        raise L.SdmiError("lora_gemm: weight %s, adapters a %s / b %s for %d -> %d channels" %
+                          (tuple(wp.shape), tuple(lora.a.shape), tuple(lora.b.shape), a.c, n_out))
+    if residual is not None and (residual.n * residual.hw, residual.c) != (m, n_out):
+        raise L.SdmiError("lora_gemm: residual holds %d rows x %d channels, the product has %d x %d" % (residual.n * residual.hw, residual.c, m, n_out))
+    if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (n_out,) or not bias.is_contiguous()):
+        raise L.SdmiError("lora_gemm: bias is contiguous fp32 (%d,), got %s %s" % (n_out, bias.dtype, tuple(bias.shape)))
+    ip = _int32(ids, (ids.numel(),), "lora_gemm: ids")
+    if ids.numel() == 0 or m % ids.numel():
+        raise L.SdmiError("lora_gemm: %d ids do not divide %d rows" % (ids.numel(), m))
+    _own_device("lora_gemm", a.buf, wp, lora.a, lora.b, lora.scale, ids, bias, None if residual is None else residual.buf, res.buf)
+    ws = torch.empty((m * lora.groups * lora.rank,), dtype=act_dtype(), device=a.device)      # the call's own: two graphs never share it
+    res.rstats = res.normed = None
+    res.stats.pop(res.off, None)
+    L.call("sdmi_lora_gemm", a.ptr, a.ld, wp.data_ptr(), wp.stride(0), res.ptr, res.ld, m, n_out, a.c, _ptr(bias), residual.ptr if residual is not None else 0,
+           residual.ld if residual is not None else 0, lora.a.data_ptr(), lora.b.data_ptr(), lora.scale.data_ptr(), lora.adapters, lora.rank, lora.groups,
+           ip, m // ids.numel(), (L.F_BIAS if bias is not None else 0) | (L.F_RESIDUAL if residual is not None else 0), ws.data_ptr(), 2 * ws.numel(),
+           _stream())
+    _audit("lora_gemm %dx%dx%d" % (m, n_out, a.c), res)
+    return res
+
+
 def linear_small_m(x, wp, bias, silu_in=False):
     """fp32 (M<=64, K) x bf16 [N][K] -> fp32 (M, N)."""
     x = x.contiguous()

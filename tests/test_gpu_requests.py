@@ -1,0 +1,369 @@
+"""GPU: cross-attention to encoder states of another length (sdmi_cross_attention) and adapters of many requests beside a shared
+projection (sdmi_lora_gemm) against their definitions in 64 bits, element by element.
+
+Tolerances, u = half a step of the 16-bit type (finfo.eps / 2), e = 2^-24 the same of fp32:
+  attention  p is rounded to 16 bits (u p; below the type's smallest normal number half its smallest step, tiny * eps / 2), o once more
+             (u |o|).  A score is off by at most (dim + 4) e sum |q||k| scale (fp32 sums of exact products, the scaling) and the base-2
+             exponential by 4 e |score| (its argument's rounding) + 8 e, so every p is off by a factor of 1 +- r, r the sum of these; sums
+             of up to nkv terms add (nkv + 64) e each, and an error of p goes into numerator and denominator.  With a = sum p |v| / sum p:
+             tol = u (a + |o|) + (2 r + 2 (nkv + 64) e) (a + |o|) + nkv tiny eps / 2 max |v|.
+  adapters   t is rounded to 16 bits (u |t|), out once (u |out|), the fp32 sums are off by (terms) e of the sums of absolute values:
+             tol = u |out| + sum_r |b| (u |t| + tiny eps / 2 + 2 (k + 4) e scale sum |x||a|) + (k + rank + 8) e (sum |x||w| + sum |t||b| + |bias| + |residual|)."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from stable_diffusion_amd import engine as E, _lib as L
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+H16 = E.act_dtype() if torch.cuda.is_available() else torch.float16
+U, TINY, E32 = torch.finfo(H16).eps / 2, torch.finfo(H16).tiny * torch.finfo(H16).eps / 2, 2.0 ** -24
+
+
+def _h(rs, *shape, std=1.0):
+    return torch.from_numpy((rs.standard_normal(shape) * std).astype(np.float32)).to(H16)
+
+
+def _i32(v):
+    return torch.tensor(v, dtype=torch.int64).to(torch.int32).to(DEV)
+
+
+# ------------------------------------------------------------------------------------------------------------ attention
+def _attention_oracle(q, k, v, heads, kvh, dim, scale, index, lens, qr, kr):
+    """(o, tolerance) in 64 bits on the CPU, sample by sample and head by head; q (b, nq, heads * dim), k / v (contexts, nkv, kvh * dim)."""
+    b, nq, nkv, n = q.shape[0], q.shape[1], k.shape[1], k.shape[0]
+    o, tol = torch.zeros(b, nq, heads * dim, dtype=torch.float64), torch.zeros(b, nq, heads * dim, dtype=torch.float64)
+    for i in range(b):
+        c = index[i] if index is not None else (0 if n == 1 else i)
+        if not 0 <= c < n:
+            continue
+        ln = min(max(lens[c], 0), nkv) if lens is not None else nkv
+        seen = torch.ones(nq, ln, dtype=torch.bool)
+        keys = torch.arange(ln)
+        if qr is not None:
+            seen = (qr[i][:, None] & kr[c][None, :ln]) != 0
+            keys = torch.nonzero(kr[c][:ln] != 0).flatten()       # a key in no region may hold anything
+            seen = seen[:, keys]
+        if keys.numel() == 0:
+            continue
+        for h in range(heads):
+            g = h * kvh // heads
+            qd, kd, vd = q[i, :, h * dim:(h + 1) * dim].double(), k[c, keys, g * dim:(g + 1) * dim].double(), v[c, keys, g * dim:(g + 1) * dim].double()
+            s = scale * (qd @ kd.t())
+            r = (dim + 4) * E32 * scale * (qd.abs() @ kd.abs().t()) + 4 * E32 * (s.abs() + s.abs().amax(1, keepdim=True)) + 8 * E32
+            r = r.masked_fill(~seen, 0.0).amax(1, keepdim=True) if keys.numel() else 0.0
+            p = torch.exp(s - s.masked_fill(~seen, -math.inf).amax(1, keepdim=True).clamp_min(-1e30)).masked_fill(~seen, 0.0)
+            l = p.sum(1, keepdim=True)
+            l = torch.where(l == 0, torch.ones_like(l), l)
+            oo, aa = p @ vd / l, p @ vd.abs() / l
+            o[i, :, h * dim:(h + 1) * dim] = oo
+            t = U * (aa + oo.abs()) + (2 * r + 2 * (ln + 64) * E32) * (aa + oo.abs()) + ln * TINY * float(vd.abs().max())
+            tol[i, :, h * dim:(h + 1) * dim] = torch.where(seen.any(1, keepdim=True), t, torch.zeros_like(t))
+    return o, tol
+
+
+def _close(got, want, tol, what):
+    got = got.double().cpu()
+    assert torch.isfinite(got).all(), what
+    bad = (got - want).abs() > tol
+    print("%s: max error / tolerance %.3f" % (what, float(((got - want).abs() / tol.clamp_min(1e-300)).max())), flush=True)
+    assert not bad.any(), (what, int(bad.sum()), float((got - want).abs().max()), torch.nonzero(bad)[:4].tolist())
+
+
+def _attention_case(seed, batch, contexts, heads, kvh, dim, nq, nkv, index=None, lens=None, regions=0, nan=True, std=1.5):
+    rs = np.random.RandomState(seed)
+    q, k, v = _h(rs, batch, nq, heads * dim, std=std), _h(rs, contexts, nkv, kvh * dim), _h(rs, contexts, nkv, kvh * dim)
+    qr = kr = None
+    if regions:
+        bits = lambda *s: torch.from_numpy(((1 << rs.randint(0, regions, s).astype(np.int64)) * rs.randint(0, 4, s).clip(0, 1)).astype(np.uint32).view(np.int32))
+        qr, kr = bits(batch, nq), bits(contexts, nkv)
+    # what lies past a context's end, or in no region, is anything
+    kd, vd = k.clone(), v.clone()
+    if nan:
+        for c in range(contexts):
+            dead = torch.zeros(nkv, dtype=torch.bool)
+            if lens is not None:
+                dead[min(max(lens[c], 0), nkv):] = True
+            if kr is not None:
+                dead |= kr[c] == 0
+            kd[c][dead], vd[c][dead] = float("nan"), float("inf")
+    return q, k, v, kd, vd, qr, kr
+
+
+def _run_attention(q, kd, vd, heads, kvh, dim, index, lens, qr, kr, scale=None, out=None):
+    """k and v as neighbouring column ranges of one wider buffer, q as the middle of another."""
+    b, nq, n, nkv = q.shape[0], q.shape[1], kd.shape[0], kd.shape[1]
+    w = kvh * dim
+    kv = torch.full((n, nkv, 2 * w + 16), float("nan"), dtype=H16)
+    kv[..., 8:8 + w], kv[..., 8 + w:8 + 2 * w] = kd, vd
+    qb = torch.full((b, nq, heads * dim + 24), float("nan"), dtype=H16)
+    qb[..., 16:16 + heads * dim] = q
+    kva, qa = E.Act(kv.to(DEV), n, 1, nkv, 2 * w + 16), E.Act(qb.to(DEV), b, 1, nq, heads * dim + 24)
+    o = E.cross_attention(qa.cols(16, heads * dim), kva.cols(8, w), kva.cols(8 + w, w), heads, kv_heads=kvh, dim=dim, scale=scale,
+                          index=None if index is None else _i32(index), lens=None if lens is None else _i32(lens),
+                          query_regions=None if qr is None else qr.to(DEV), key_regions=None if kr is None else kr.to(DEV), out=out)
+    return o.buf if out is None else o
+
+
+ATT = [  # batch, contexts, heads, kv heads, dim, nq, nkv, index, lens, regions
+    (1, 1, 1, 1, 64, 1, 1, None, None, 0),
+    (2, 2, 2, 2, 64, 130, 77, None, [77, 1], 0),
+    (3, 1, 2, 2, 64, 65, 64, None, [63], 0),
+    (3, 2, 2, 1, 64, 129, 65, [1, 0, 1], [65, 0], 0),
+    (2, 2, 5, 5, 64, 200, 231, None, [200, 129], 0),
+    (4, 3, 4, 2, 40, 33, 100, [2, 2, 0, 1], [100, 64, 65], 0),
+    (2, 2, 3, 3, 8, 70, 9, None, None, 0),
+    (1, 1, 2, 2, 32, 300, 128, None, None, 0),
+    (2, 2, 2, 2, 72, 97, 127, None, [127, 128], 0),
+    (2, 2, 8, 8, 80, 101, 133, None, [133, -5], 0),
+    (2, 2, 2, 2, 96, 131, 190, None, [1000, 3], 0),
+    (2, 2, 4, 1, 128, 66, 257, None, None, 0),
+    (2, 2, 2, 2, 160, 140, 130, None, [130, 66], 0),
+    (2, 2, 2, 2, 200, 140, 70, None, None, 0),
+    (2, 2, 2, 1, 256, 150, 193, None, [150, 193], 0),
+    # few rows: one wave tile for four waves; long keys in pieces
+    (2, 2, 4, 4, 64, 1, 5, None, [5, 0], 0),
+    (3, 3, 8, 2, 64, 1, 1025, None, [1025, 1, 128], 0),
+    (2, 2, 16, 2, 128, 1, 2000, None, [1999, 130], 0),
+    (2, 2, 2, 2, 256, 7, 700, None, [700, 0], 0),
+    (1, 1, 2, 2, 160, 40, 1111, None, None, 0),
+    (2, 3, 2, 2, 32, 64, 4099, [2, 0], [4099, 7, 4001], 0),
+    (1, 1, 2, 2, 64, 144, 3001, None, None, 0),
+    (1, 1, 1, 1, 96, 129, 1500, None, [1409], 0),
+    # regions
+    (2, 2, 2, 2, 64, 150, 154, None, None, 3),
+    (2, 1, 4, 2, 64, 9, 600, None, [599], 32),
+    (2, 2, 2, 2, 80, 131, 90, [1, 1], [0, 90], 32),
+    (1, 1, 2, 2, 256, 3, 900, None, None, 2),
+    (2, 2, 2, 1, 160, 70, 65, None, None, 4),
+    (2, 2, 2, 2, 96, 140, 2100, None, [2100, 1], 2),
+    (1, 1, 2, 2, 128, 140, 300, None, None, 32),
+    (1, 1, 2, 2, 32, 140, 300, None, None, 32),
+]
+
+
+@pytest.mark.parametrize("case", range(len(ATT)))
+def test_attention(case):
+    batch, contexts, heads, kvh, dim, nq, nkv, index, lens, regions = ATT[case]
+    q, k, v, kd, vd, qr, kr = _attention_case(case, batch, contexts, heads, kvh, dim, nq, nkv, index, lens, regions)
+    got = _run_attention(q, kd, vd, heads, kvh, dim, index, lens, qr, kr)
+    want, tol = _attention_oracle(q, k, v, heads, kvh, dim, dim ** -0.5, index, lens, qr, kr)
+    _close(got, want, tol, "attention %s" % (ATT[case],))
+
+
+@pytest.mark.parametrize("nq,nkv", [(200, 100), (1, 2000)])
+def test_attention_large_scores_and_other_scale(nq, nkv):
+    """Scores of some hundreds (one key takes it all) and a scale of the caller's."""
+    q, k, v, kd, vd, _, _ = _attention_case(77, 2, 2, 2, 2, 64, nq, nkv, std=60.0)
+    got = _run_attention(q, kd, vd, 2, 2, 64, None, None, None, None, scale=0.3)
+    want, tol = _attention_oracle(q, k, v, 2, 2, 64, float(np.float32(0.3)), None, None, None, None)
+    _close(got, want, tol, "attention, scores of hundreds")
+
+
+@pytest.mark.parametrize("nq", [3, 200])
+def test_attention_no_keys_gives_zeros(nq):
+    q = _h(np.random.RandomState(1), 2, nq, 128)
+    qa, kv = E.Act(q.to(DEV), 2, 1, nq, 128), E.Act(torch.empty((2, 0, 128), dtype=H16, device=DEV), 2, 1, 0, 128)
+    assert not E.cross_attention(qa, kv, kv, 2).buf.any()
+    kv = E.Act(torch.full((2, 90, 128), float("nan"), dtype=H16, device=DEV), 2, 1, 90, 128)
+    assert not E.cross_attention(qa, kv, kv, 2, index=_i32([-1, 2])).buf.any()          # no such context
+    assert not E.cross_attention(qa, kv, kv, 2, lens=_i32([0, -3])).buf.any()
+    sets = dict(query_regions=_i32([[1] * nq] * 2), key_regions=_i32([[0] * 90] * 2))
+    assert not E.cross_attention(qa, kv, kv, 2, **sets).buf.any()
+
+
+@pytest.mark.parametrize("nq,nkv", [(37, 77), (130, 77), (5, 1500)])
+def test_attention_writes_its_own_columns_only(nq, nkv):
+    q, k, v, kd, vd, _, _ = _attention_case(5, 2, 2, 2, 2, 40, nq, nkv, lens=[nkv, 3])
+    buf = torch.full((2, nq, 96), 7.0, dtype=H16, device=DEV)
+    out = E.Act(buf, 2, 1, nq, 96).cols(8, 80)
+    _run_attention(q, kd, vd, 2, 2, 40, None, [nkv, 3], None, None, out=out)
+    want, tol = _attention_oracle(q, k, v, 2, 2, 40, 40 ** -0.5, None, [nkv, 3], None, None)
+    _close(buf[..., 8:88], want, tol, "attention into a view")
+    assert bool((buf[..., :8] == 7.0).all()) and bool((buf[..., 88:] == 7.0).all())
+
+
+def test_attention_offsets_past_32_bits():
+    """Rows 128 KB apart (the last one 5 GB behind the first) and contexts further still."""
+    nkv, ld = 40000, 1 << 16
+    rs = np.random.RandomState(3)
+    base = torch.empty((nkv, ld), dtype=H16, device=DEV)
+    k, v, q = _h(rs, 1, nkv, 64), _h(rs, 1, nkv, 64), _h(rs, 2, 1, 64)
+    base[:, :64], base[:, 64:128] = k[0].to(DEV), v[0].to(DEV)
+    qd, o = q.to(DEV), torch.empty((2, 1, 64), dtype=H16, device=DEV)
+    ws = torch.empty((L.load().sdmi_cross_attention_ws_bytes(2, 1, 1, 64, 1, nkv),), dtype=torch.uint8, device=DEV)
+    # two contexts: rows 0.. and rows 20000.. of the same memory
+    L.call("sdmi_cross_attention", qd.data_ptr(), 64, 64, base.data_ptr(), ld, 20000 * ld, base.data_ptr() + 128, ld, 20000 * ld, o.data_ptr(), 64, 64, 2, 2, 1, 1, 64, 1,
+           20000, 0, 0, 0, 0, 0, 0, 0.125, ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream)
+    want, tol = _attention_oracle(q, k.view(2, 20000, 64), v.view(2, 20000, 64), 1, 1, 64, 0.125, None, None, None, None)
+    _close(o, want, tol, "attention over 5 GB of rows")
+
+
+def test_attention_without_workspace_is_not_cut():
+    q, k, v, kd, vd, _, _ = _attention_case(8, 2, 2, 2, 2, 64, 1, 3000)
+    qa, ka, va, o = (t.to(DEV) for t in (q, kd, vd, torch.empty_like(q)))
+    assert L.load().sdmi_cross_attention_ws_bytes(2, 2, 2, 64, 1, 3000) > 0
+    L.call("sdmi_cross_attention", qa.data_ptr(), 128, 128, ka.data_ptr(), 128, 128 * 3000, va.data_ptr(), 128, 128 * 3000, o.data_ptr(), 128, 128, 2, 2, 2, 2, 64, 1, 3000,
+           0, 0, 0, 0, 0, 0, 0.125, 0, 0, torch.cuda.current_stream().cuda_stream)
+    want, tol = _attention_oracle(q, k, v, 2, 2, 64, 0.125, None, None, None, None)
+    _close(o, want, tol, "attention without a workspace")
+
+
+# ------------------------------------------------------------------------------------------------------------ adapters
+def _lora_oracle(x, w, a, b, scale, ids, per, groups, bias, residual):
+    x, w, a, b = x.double(), w.double(), a.double(), b.double()
+    m, n, r = x.shape[0], w.shape[0], b.shape[2]
+    out, mag = x @ w.t(), x.abs() @ w.abs().t()
+    extra = torch.zeros_like(out)
+    for i in range(m):
+        j = ids[i // per]
+        if not 0 <= j < a.shape[0]:
+            continue
+        sc = float(scale[j])
+        t, ta = sc * (a[j] @ x[i]), sc * (a[j].abs() @ x[i].abs())
+        for g in range(groups):
+            c = slice(g * n // groups, (g + 1) * n // groups)
+            tg, tag = t[g * r:(g + 1) * r], ta[g * r:(g + 1) * r]
+            out[i, c] += b[j, c] @ tg
+            mag[i, c] += b[j, c].abs() @ tg.abs()
+            extra[i, c] = b[j, c].abs() @ (U * tg.abs() + TINY + 2 * (x.shape[1] + 4) * E32 * tag)
+    if bias is not None:
+        out, mag = out + bias.double(), mag + bias.double().abs()
+    if residual is not None:
+        out, mag = out + residual.double(), mag + residual.double().abs()
+    return out, U * out.abs() + TINY + extra + (x.shape[1] + r + 8) * E32 * mag
+
+
+def _lora_case(seed, m, k, n, groups, rank, adapters, bias, residual):
+    rs = np.random.RandomState(seed)
+    x, w, a, b = _h(rs, m, k), _h(rs, n, k, std=k ** -0.5), _h(rs, adapters, groups * rank, k, std=k ** -0.5), _h(rs, adapters, n, rank, std=rank ** -0.5)
+    scale = torch.from_numpy((rs.rand(adapters) * 2 - 0.5).astype(np.float32))
+    return x, w, a, b, scale, torch.from_numpy(rs.randn(n).astype(np.float32)) if bias else None, _h(rs, m, n) if residual else None
+
+
+def _run_lora(x, w, a, b, scale, ids, bias, residual, out=None):
+    m, k, n = x.shape[0], x.shape[1], w.shape[0]
+    xb = torch.full((1, m, k + 16), float("nan"), dtype=H16)
+    xb[0, :, 8:8 + k] = x
+    res = None if residual is None else E.Act(residual.to(DEV).view(1, m, n), 1, 1, m, n)
+    y = E.lora_gemm(E.Act(xb.to(DEV), 1, 1, m, k + 16).cols(8, k), w.to(DEV), n, E.LoraPack(a.to(DEV), b.to(DEV), scale.to(DEV)), _i32(ids),
+                    bias=None if bias is None else bias.to(DEV), residual=res, out=out)
+    return y.buf.view(m, -1) if out is None else y
+
+
+LORA = [  # rows per id, ids, k, n, groups, rank, adapters, bias, residual
+    (1, [0], 8, 8, 1, 8, 1, False, False),
+    (1, [2], 1024, 1024, 1, 16, 4, True, True),
+    (1, [1, 0, -1, 3, 1], 72, 40, 1, 8, 3, True, False),
+    (7, [1, 0, 2], 320, 320, 1, 16, 3, True, True),
+    (64, [0, 1], 64, 128, 1, 32, 2, False, False),
+    (100, [1, 1, 0], 136, 104, 1, 24, 2, True, False),
+    (130, [0], 640, 120, 3, 8, 1, False, False),
+    (77, [3, -1, 0, 1], 192, 984, 3, 16, 4, True, True),
+    (33, [1, 0], 200, 72, 3, 40, 2, False, True),
+    (1, list(range(64)), 128, 256, 1, 32, 64, True, False),
+    (1, [(i * 7) % 5 - 1 for i in range(205)], 256, 192, 1, 128, 4, True, True),
+    (1, [(i * i) % 97 for i in range(150)], 88, 72, 1, 8, 97, False, False),
+    (3, [(i * 5) % 9 for i in range(50)], 104, 176, 2, 16, 9, False, True),
+    (300, [-1, 5], 96, 64, 1, 16, 5, True, False),
+    (1, [2 ** 31 - 1, -2 ** 31, 0, 1], 64, 64, 1, 256, 1, False, False),
+    (900, [1, 0], 64, 64, 1, 64, 2, True, True),
+    (2304, [0, 1], 64, 1920, 3, 8, 2, False, False),
+    (1, [0] * 17, 5120, 16, 1, 8, 1, True, False),
+]
+
+
+@pytest.mark.parametrize("case", range(len(LORA)))
+def test_lora(case):
+    per, ids, k, n, groups, rank, adapters, bias, residual = LORA[case]
+    x, w, a, b, scale, bi, res = _lora_case(case, per * len(ids), k, n, groups, rank, adapters, bias, residual)
+    got = _run_lora(x, w, a, b, scale, ids, bi, res)
+    want, tol = _lora_oracle(x, w, a, b, scale, ids, per, groups, bi, res)
+    _close(got, want, tol, "lora %s" % ((per, len(ids)) + LORA[case][2:],))
+
+
+def test_lora_last_id_covers_fewer_rows():
+    x, w, a, b, scale, _, _ = _lora_case(4, 150, 64, 72, 1, 16, 3, False, False)
+    ids = [2, 0, 1]                                         # 64 + 64 + 22 rows
+    xd, wd, ad, bd, sd, idd = x.to(DEV), w.to(DEV), a.to(DEV), b.to(DEV), scale.to(DEV), _i32(ids)
+    out = torch.full((152, 80), 5.0, dtype=H16, device=DEV)
+    ws = torch.empty((150 * 16,), dtype=H16, device=DEV)
+    L.call("sdmi_lora_gemm", xd.data_ptr(), 64, wd.data_ptr(), 64, out.data_ptr(), 80, 150, 72, 64, 0, 0, 0, ad.data_ptr(), bd.data_ptr(), sd.data_ptr(), 3, 16, 1,
+           idd.data_ptr(), 64, 0, ws.data_ptr(), 2 * ws.numel(), torch.cuda.current_stream().cuda_stream)
+    want, tol = _lora_oracle(x, w, a, b, scale, ids, 64, 1, None, None)
+    _close(out[:150, :72], want, tol, "lora, ragged last request")
+    assert bool((out[150:] == 5.0).all()) and bool((out[:, 72:] == 5.0).all())
+
+
+def test_lora_residual_in_place():
+    x, w, a, b, scale, bi, res = _lora_case(6, 200, 128, 136, 1, 8, 2, True, True)
+    want, tol = _lora_oracle(x, w, a, b, scale, [1, 0], 100, 1, bi, res)
+    stream = E.Act(res.to(DEV).view(1, 200, 136), 1, 1, 200, 136)
+    E.lora_gemm(E.Act(x.to(DEV).view(1, 200, 128), 1, 1, 200, 128), w.to(DEV), 136, E.LoraPack(a.to(DEV), b.to(DEV), scale.to(DEV)), _i32([1, 0]), bias=bi.to(DEV),
+                residual=stream, out=stream)
+    _close(stream.buf[0], want, tol, "lora, residual in place")
+
+
+# ------------------------------------------------------------------------------------------------------------ streams and graphs
+def _both(seed, nq, nkv):
+    """A projection with adapters whose result attends to encoder states, as a block of the UNet does; returns a function that runs it."""
+    rs = np.random.RandomState(seed)
+    x, w, a, b, scale, _, _ = _lora_case(seed, 2 * nq, 128, 128, 1, 16, 3, False, False)
+    kv = _h(rs, 2, nkv, 256).to(DEV)
+    lens, index, ids = _i32([nkv, nkv // 2]), _i32([0, 1]), _i32([0, 1])
+    xa, wd, pack = E.Act(x.to(DEV).view(2, nq, 128), 2, 1, nq, 128), w.to(DEV), E.LoraPack(a.to(DEV), b.to(DEV), scale.to(DEV))
+    kva = E.Act(kv, 2, 1, nkv, 256)
+
+    def run():
+        q = E.lora_gemm(xa, wd, 128, pack, ids)
+        return E.cross_attention(q, kva.cols(0, 128), kva.cols(128, 128), 2, index=index, lens=lens).buf
+    return run, lens, index, ids
+
+
+@pytest.mark.parametrize("nq,nkv", [(1, 2000), (144, 77)])
+def test_two_streams_at_once_give_the_bits_of_one(nq, nkv):
+    runs = [_both(s, nq, nkv)[0] for s in (1, 2)]
+    alone = [r().clone() for r in runs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    outs = [[], []]
+    for _ in range(10):
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                outs[i].append(runs[i]())
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        assert all(torch.equal(o, alone[i]) for o in outs[i])
+
+
+@pytest.mark.parametrize("nq,nkv", [(1, 2000), (144, 77)])
+def test_graphs_replayed_together_see_new_lengths_and_ids(nq, nkv):
+    """Two captured graphs replayed on two streams at once; lengths, contexts and adapters change between the replays."""
+    made = [_both(s, nq, nkv) for s in (3, 4)]
+    graphs, outs = [], []
+    for run, _, _, _ in made:
+        run()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(run())
+        graphs.append(g)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for step in range(4):
+        want = []
+        for run, lens, index, ids in made:
+            lens.copy_(_i32([nkv - step, 1 + 17 * step]))
+            index.copy_(_i32([step % 2, 1]))
+            ids.copy_(_i32([step - 1, 2]))
+            want.append(run().clone())                  # eager work between the replays
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+                g.replay()
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            assert torch.equal(o, w), step

@@ -1,0 +1,46 @@
+"""CPU: sdmi_cross_attention and sdmi_lora_gemm refuse bad arguments with an error code and a message, before any launch (the
+pointers here are never followed), and their workspace sizes."""
+import pytest
+
+from stable_diffusion_amd import _lib as L
+
+P = 0x10000000     # an aligned address that is never followed
+
+ATT = dict(q=P, ldq=128, sq=128, k=P, ldk=128, sk=1280, v=P, ldv=128, sv=1280, o=P, ldo=128, so=128, batch=2, contexts=2, heads=2, kv_heads=2, dim=64, nq=1, nkv=10,
+           index=None, lens=None, qr=None, sqr=0, kr=None, skr=0, scale=0.125, ws=None, ws_bytes=0, stream=None)
+LORA = dict(x=P, ldx=64, w=P, ldw=64, out=P, ldo=64, m=4, n=64, k=64, bias=None, residual=None, ldr=0, a=P, b=P, scale=P, adapters=2, rank=8, groups=1, ids=P, rows=1,
+            flags=0, ws=P, ws_bytes=1 << 20, stream=None)
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(q=None), "null"), (dict(k=None), "null"), (dict(o=None), "null"), (dict(batch=0), "shape"), (dict(heads=3), "shape"), (dict(kv_heads=0), "shape"),
+    (dict(dim=60), "shape"), (dict(dim=264, kv_heads=1, heads=1, ldq=264, ldk=264, ldv=264, ldo=264), "shape"), (dict(dim=0), "shape"), (dict(nq=0), "shape"),
+    (dict(nkv=-1), "shape"), (dict(contexts=0), "contexts"), (dict(contexts=3), "index"), (dict(ldq=120), "stride"), (dict(ldq=132), "multiples"), (dict(ldk=64), "stride"),
+    (dict(ldo=66), "multiples"), (dict(ldk=1 << 22), "too large"), (dict(sk=1284), "alignment"), (dict(q=P + 8), "alignment"), (dict(o=P + 4), "alignment"),
+    (dict(qr=P), "together"), (dict(kr=P), "together"), (dict(index=P + 2), "alignment"), (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"),
+    (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
+])
+def test_attention_refuses(change, word):
+    with pytest.raises(L.SdmiError, match=word):
+        L.call("sdmi_cross_attention", *{**ATT, **change}.values())
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(x=None), "null"), (dict(ids=None), "null"), (dict(ws=None), "null"), (dict(b=None), "null"), (dict(m=0), "shape"), (dict(n=60), "shape"), (dict(k=60), "shape"),
+    (dict(rank=12), "shape"), (dict(rank=0), "shape"), (dict(rank=264), "shape"), (dict(groups=0), "shape"), (dict(groups=3), "shape"), (dict(adapters=0), "adapters"),
+    (dict(rows=0), "rows per id"), (dict(flags=8), "flags"), (dict(flags=1), "bias"), (dict(flags=4), "residual"), (dict(flags=4, residual=P, ldr=32), "residual"),
+    (dict(ldx=32), "strides"), (dict(ldw=68), "strides"), (dict(ldo=60), "strides"), (dict(ldx=1 << 22), "too large"), (dict(x=P + 8), "alignment"),
+    (dict(flags=4, residual=P + 8, ldr=64), "alignment"), (dict(ids=P + 2), "alignment"), (dict(ws_bytes=8), "workspace"),
+])
+def test_lora_refuses(change, word):
+    with pytest.raises(L.SdmiError, match=word):
+        L.call("sdmi_lora_gemm", *{**LORA, **change}.values())
+
+
+def test_workspace_sizes():
+    lib = L.load()
+    assert lib.sdmi_cross_attention_ws_bytes(2, 5, 5, 64, 9216, 77) == 0            # one pass
+    assert lib.sdmi_cross_attention_ws_bytes(1, 2, 2, 64, 1, 5000) > 0              # keys in pieces
+    assert lib.sdmi_cross_attention_ws_bytes(1, 2, 2, 60, 1, 5000) == 0             # refused shapes need nothing
+    assert lib.sdmi_lora_gemm_ws_bytes(100, 96, 64, 16, 3) >= 100 * 48 * 2
+    assert lib.sdmi_lora_gemm_ws_bytes(100, 96, 64, 12, 3) == 0
