@@ -198,8 +198,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void lora_gemm_kernel(const LoraPa
   {                                                                                                 \
     constexpr int INFLIGHT = (GROUPS) * (PA + PB);                                                  \
     static_assert(INFLIGHT >= 0 && INFLIGHT < 64, "vmcnt is a 6-bit counter");                      \
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(INFLIGHT) : "memory");                      \
-    __builtin_amdgcn_s_barrier();                                                                   \
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(INFLIGHT) : "memory");          \
   }
   f32x4 acc[MT][NT];
 #pragma unroll

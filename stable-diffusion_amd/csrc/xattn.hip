@@ -33,109 +33,120 @@ struct XattnParams {
 
 constexpr float XA_LOWEST = -1e30f;  // start of the running maximum: below every scaled score, and finite, so that m - m is 0
 
-// LDS row strides in elements.  K: fragment reads are 16 B at the same column of 8 consecutive rows: (DP + 8) / 2 dwords is
-// 4 mod 8, which spreads them over the banks.  V: a transposed read takes 4 rows x 64 B: stride 16 or 48 dwords mod 64.
-template <int DP> constexpr int xa_kstr() { return DP + 8; }
-template <int DP> constexpr int xa_vstr() { return (DP / 2) % 64 == 16 || (DP / 2) % 64 == 48 ? DP : DP + 32; }
+// LDS images of a tile are linear in 16-byte pieces (a wave's DMA writes 1 KB in lane order), DP / 8 pieces to a row; the piece
+// that lies at position c of row r is c ^ xa_kx(r) (K) or c ^ xa_vx(r) (V), applied on the source side.  K fragments: 8
+// consecutive rows at one logical piece have to fall on 8 different quarters of the 64 banks; V: a transposed read takes 4
+// rows x 64 B, which have to fall on 4 different quarters.  Rows of 64, 192 or 320 B step through the quarters by themselves.
+template <int DP> __device__ __forceinline__ int xa_kx(int row) {
+  return DP == 64 ? (row >> 1) & 7 : DP % 128 == 0 ? row & 7 : (row >> 2) & 3;
+}
+template <int DP> __device__ __forceinline__ int xa_vx(int row) {
+  return DP == 64 ? ((row >> 1) & 1) << 2 : DP % 128 == 0 ? (row & 3) << 2 : 0;
+}
+
+constexpr float XA_RAISE = 8.0f;  // the running maximum is raised once a score passes it by 2^8 (p <= 256 keeps its precision in 16 bits)
 
 enum { XA_FULL = 0, XA_TAIL = 1, XA_REGIONS = 2 };
 
-// One wave's share of a key tile: KS blocks of 32 keys against its 32 rows.
-template <int DP, int KS, int MODE>
-__device__ __forceinline__ void xa_step(const u16* sK, const u16* sV, const unsigned* sR, const hx8 (&qf)[DP / 16], f32x16 (&oacc)[DP / 32],
-                                        float& m, float& l, float c, int key0, int klim, unsigned qset, int lane) {
-  constexpr int KSTR = xa_kstr<DP>(), VSTR = xa_vstr<DP>();
+// One wave's share of a key tile: KS blocks of 32 keys (from row kr0 of the tile) against its QT x 32 rows.
+template <int DP, int QT, int KS, int MODE>
+__device__ __forceinline__ void xa_step(const u16* sK, const u16* sV, const unsigned* sR, const hx8 (&qf)[QT][DP / 16], f32x16 (&oacc)[QT][DP / 32],
+                                        float (&m)[QT], float (&l)[QT], float c, int kr0, int key0, int klim, const unsigned (&qset)[QT], int lane) {
   const int r = lane & 31, hh = lane >> 5, dblk = (lane >> 4) & 1, tq = (lane & 15) >> 2, tp = lane & 3;
-  f32x16 s[KS];
 #pragma unroll
-  for (int b = 0; b < KS; ++b)
+  for (int b = 0; b < KS; ++b) {
+    f32x16 s[QT];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
+    for (int x = 0; x < QT; ++x)
 #pragma unroll
-  for (int ks = 0; ks < DP / 16; ++ks)
+      for (int i = 0; i < 16; ++i) s[x][i] = 0.f;
+    const int krow = kr0 + 32 * b + r;
 #pragma unroll
-    for (int b = 0; b < KS; ++b) s[b] = MFMA32(*(const hx8*)&sK[(32 * b + r) * KSTR + 16 * ks + 8 * hh], qf[ks], s[b], 0, 0, 0);
-  if constexpr (MODE == XA_TAIL) {
+    for (int ks = 0; ks < DP / 16; ++ks) {
+      const hx8 kf = *(const hx8*)&sK[krow * DP + (((2 * ks + hh) ^ xa_kx<DP>(krow)) << 3)];
 #pragma unroll
-    for (int b = 0; b < KS; ++b)
+      for (int x = 0; x < QT; ++x) s[x] = MFMA32(kf, qf[x][ks], s[x], 0, 0, 0);
+    }
+    if constexpr (MODE == XA_TAIL) {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        if (key0 + 32 * b + 8 * (i >> 2) + 4 * hh + (i & 3) >= klim) s[b][i] = -__builtin_inff();
-  }
-  if constexpr (MODE == XA_REGIONS) {  // keys past the end carry the empty set
+        if (key0 + 32 * b + 8 * (i >> 2) + 4 * hh + (i & 3) >= klim) {
 #pragma unroll
-    for (int b = 0; b < KS; ++b)
+          for (int x = 0; x < QT; ++x) s[x][i] = -__builtin_inff();
+        }
+    }
+    if constexpr (MODE == XA_REGIONS) {  // keys past the end carry the empty set
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const u32x4 kr = *(const u32x4*)&sR[32 * b + 8 * g + 4 * hh];
+        const u32x4 kr = *(const u32x4*)&sR[kr0 + 32 * b + 8 * g + 4 * hh];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (!(kr[e] & qset)) s[b][4 * g + e] = -__builtin_inff();
+#pragma unroll
+          for (int x = 0; x < QT; ++x)
+            if (!(kr[e] & qset[x])) s[x][4 * g + e] = -__builtin_inff();
       }
-  }
-  float mx = s[0][0];
-#pragma unroll
-  for (int b = 0; b < KS; ++b)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[b][i]);
-  mx = fmaxf(mx, __shfl_xor(mx, 32));
-  const float mnew = fmaxf(m, mx * c);
-  // no lane's maximum moved (the usual case after a few tiles): nothing to rescale
-  if (__builtin_amdgcn_ballot_w64(mnew > m) != 0) {
-    const float alpha = __builtin_amdgcn_exp2f(m - mnew);
-    l *= alpha;
-#pragma unroll
-    for (int dt = 0; dt < DP / 32; ++dt)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) oacc[dt][i] *= alpha;
-    m = mnew;
-  }
-  float rs = 0.f;
-#pragma unroll
-  for (int b = 0; b < KS; ++b)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], c, -m));
-      s[b][i] = e;
-      rs += e;
     }
-  l += rs;
+    hx8 pb[QT][2];
 #pragma unroll
-  for (int b = 0; b < KS; ++b)
+    for (int x = 0; x < QT; ++x) {
+      float mx = s[x][0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[x][i]);
+      mx *= c;
+      if (__builtin_amdgcn_ballot_w64(mx > m[x] + XA_RAISE) != 0) {
+        const float mnew = fmaxf(m[x], fmaxf(mx, __shfl_xor(mx, 32)));
+        const float alpha = __builtin_amdgcn_exp2f(m[x] - mnew);
+        l[x] *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) oacc[x][dt][i] *= alpha;
+        m[x] = mnew;
+      }
+      float rs = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[x][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][i], c, -m[x]));
+        rs += s[x][i];
+      }
+      l[x] += rs;
+#pragma unroll
+      for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) pb[x][s2][j] = (h16)s[x][8 * s2 + j];
+    }
 #pragma unroll
     for (int s2 = 0; s2 < 2; ++s2) {
-      hx8 pb;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) pb[j] = (h16)s[b][8 * s2 + j];
+      const int vrow = kr0 + 32 * b + 16 * s2 + 4 * hh + tq;  // and vrow + 8, whose swizzle is the same
 #pragma unroll
       for (int dt = 0; dt < DP / 32; ++dt) {
-        const u16* vp = sV + (32 * b + 16 * s2 + 4 * hh + tq) * VSTR + 32 * dt + 16 * dblk + 4 * tp;
+        const u16* vp = sV + vrow * DP + (((4 * dt + 2 * dblk + (tp >> 1)) ^ xa_vx<DP>(vrow)) << 3) + 4 * (tp & 1);
         union { struct { short4_t a, b; } h; hx8 v; } u;
         u.h.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((short4_t __attribute__((address_space(3)))*)vp);
-        u.h.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((short4_t __attribute__((address_space(3)))*)(vp + 8 * VSTR));
-        oacc[dt] = MFMA32(u.v, pb, oacc[dt], 0, 0, 0);
+        u.h.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((short4_t __attribute__((address_space(3)))*)(vp + 8 * DP));
+#pragma unroll
+        for (int x = 0; x < QT; ++x) oacc[x][dt] = MFMA32(u.v, pb[x][s2], oacc[x][dt], 0, 0, 0);
       }
     }
+  }
 }
 
-template <int DP, int WK> constexpr int xa_tile_keys() { return WK == 1 ? 64 : 128; }
-template <int DP, int WK> constexpr int xa_bufs() { return xa_tile_keys<DP, WK>() * (xa_kstr<DP>() + xa_vstr<DP>()) * 2 * 2 <= 80 * 1024 ? 2 : 1; }
-template <int DP, int WK> constexpr int xa_lds_bytes() {
-  constexpr int stage = xa_bufs<DP, WK>() * xa_tile_keys<DP, WK>() * ((xa_kstr<DP>() + xa_vstr<DP>()) * 2 + 4);
-  constexpr int merge = WK == 1 ? 0 : 4 * 32 * DP * 4 + 4 * 32 * 8;
-  return stage > merge ? stage : merge;
-}
-
-// Block: 4 waves.  WK = 1: each wave owns 32 of the block's 128 rows and sweeps all keys.  WK = 4: the block has 32 rows, each
-// wave sweeps a quarter of every key tile (few rows, long states: one query, decoding), the waves' (m, l, O) merge in the LDS.
-template <int DP, int WK, bool REG>
-__global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void xattn_kernel(const XattnParams p) {
-  constexpr int KT = xa_tile_keys<DP, WK>(), KS = KT / 32 / WK, KSTR = xa_kstr<DP>(), VSTR = xa_vstr<DP>(), NB = xa_bufs<DP, WK>();
-  constexpr int CH = DP / 8, PT = KT * CH / 256;  // 16-byte pieces of a row; pieces of K (and of V) a thread stages per tile
-  constexpr int BUF = KT * (KSTR + VSTR);         // elements per buffer
+// Block: 4 waves = WR row groups of QT x 32 rows by WK shares of every tile of KT keys; the shares' (m, l, O) merge in the LDS.
+template <int DP, int QT, int WK, int KT, bool REG>
+struct XaShape {
+  static constexpr int WR = 4 / WK, KS = KT / 32 / WK, ROWS = WR * QT * 32, BUF = 2 * KT * DP;  // BUF: elements of K and V of a tile
+  static constexpr int merge = WK == 1 ? 0 : 4 * QT * 32 * (DP * 4 + 8);
+  static constexpr int stage = 2 * (BUF * 2 + (REG ? KT * 4 : 0));
+  static constexpr int bytes = stage > merge ? stage : merge;
+};
+template <int DP, int QT, int WK, int KT, bool REG>
+__global__ __launch_bounds__(256, DP * QT <= 64 ? 3 : DP * QT <= 128 ? 2 : 1) void xattn_kernel(const XattnParams p) {
+  typedef XaShape<DP, QT, WK, KT, REG> S;
+  constexpr int CH = DP / 8, PT = KT * CH / 256;  // 16-byte pieces of a row; pieces of K (and of V) a thread moves per tile
+  static_assert(KT * CH % 256 == 0 && S::KS >= 1, "tile / wave grid mismatch");
   extern __shared__ __attribute__((aligned(16))) u16 smem[];
-  unsigned* const sreg = (unsigned*)(smem + NB * BUF);
-  const int t = threadIdx.x, lane = t & 63, wv = t >> 6, r = lane & 31, hh = lane >> 5;
+  unsigned* const sreg = (unsigned*)(smem + 2 * S::BUF);
+  const int t = threadIdx.x, lane = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6), wr = wv / WK, wk = wv % WK, r = lane & 31, hh = lane >> 5;
   int bid = xcd_remap(blockIdx.x, gridDim.x);
   const int rt = bid % p.rtiles;
   bid /= p.rtiles;
@@ -148,162 +159,159 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void xattn_k
   const int ntiles = (len + KT - 1) / KT;
   const int t0 = (int)((long long)ntiles * sp / p.splits), t1 = (int)((long long)ntiles * (sp + 1) / p.splits);
   const int cz = ctx_ok ? ctx : 0;
-  const char* kb = (const char*)(p.k + (long long)cz * p.sk + (long long)hk * p.dim);
-  const char* vb = (const char*)(p.v + (long long)cz * p.sv + (long long)hk * p.dim);
+  const u16* kb = p.k + (long long)cz * p.sk + (long long)hk * p.dim;
+  const u16* vb = p.v + (long long)cz * p.sv + (long long)hk * p.dim;
   const unsigned* krp = REG ? p.kreg + (long long)cz * p.skr : nullptr;
 
-  // ---- this wave's rows: row rho of the kv head is query rho / group, head rho % group of the group
-  const int rho = (rt * (WK == 1 ? 4 : 1) + (WK == 1 ? wv : 0)) * 32 + r;
-  const bool row_ok = rho < p.rows;
-  const int qi = (row_ok ? rho : p.rows - 1) / p.group, head = hk * p.group + (row_ok ? rho : p.rows - 1) % p.group;
-  const u16* Q = p.q + (long long)bz * p.sq + (long long)qi * p.ldq + head * p.dim;
-  hx8 qf[DP / 16];
-#pragma unroll
-  for (int ks = 0; ks < DP / 16; ++ks) {
-    const int d = 16 * ks + 8 * hh;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) qf[ks][e] = (h16)0.f;
-    if (d < p.dim) qf[ks] = *(const hx8*)(Q + d);
-  }
-  const unsigned qset = REG ? (row_ok ? p.qreg[(long long)bz * p.sqr + qi] : 0u) : 0u;
-
-  // ---- staging through registers: the next tile's loads are in flight under this tile's products.  A key past the end (or
-  // in no region) is staged as zeros whatever memory holds there: p = 0 must not meet a NaN in the second product.
+  // ---- staging by LDS-DMA, two buffers.  A key past the end reads as zeros (it lies past the descriptor's records, so memory is
+  // not touched), a piece past the head's width too; so does V of a key in no region: p = 0 must not meet a NaN.
   unsigned koff[PT], voff[PT];
-  int srow[PT];
-  bool cok[PT];
 #pragma unroll
   for (int i = 0; i < PT; ++i) {
-    const int piece = t + 256 * i, row = piece / CH, ch = piece % CH;
-    srow[i] = row;
-    cok[i] = ch * 8 < p.dim;
-    koff[i] = 2u * ((unsigned)row * p.ldk + ch * 8);
-    voff[i] = 2u * ((unsigned)row * p.ldv + ch * 8);
+    const int piece = t + 256 * i, row = piece / CH, ch = piece % CH, ck = ch ^ xa_kx<DP>(row), cv = ch ^ xa_vx<DP>(row);
+    koff[i] = ck * 8 < p.dim ? 2u * ((unsigned)row * p.ldk + ck * 8) : DMA_OOB;
+    voff[i] = cv * 8 < p.dim ? 2u * ((unsigned)row * p.ldv + cv * 8) : DMA_OOB;
   }
-  u32x4 kreg_[PT], vreg_[PT];
-  unsigned rreg = 0;
-  auto load = [&](int tile) {
-    const int key0 = tile * KT;
-    const char* kt = kb + (long long)key0 * p.ldk * 2;
-    const char* vt = vb + (long long)key0 * p.ldv * 2;
-#pragma unroll
-    for (int i = 0; i < PT; ++i) {
-      kreg_[i] = vreg_[i] = u32x4{0u, 0u, 0u, 0u};
-      if (key0 + srow[i] < len && cok[i]) {
-        kreg_[i] = *(const u32x4*)(kt + koff[i]);
-        vreg_[i] = *(const u32x4*)(vt + voff[i]);
-        if (REG && krp[key0 + srow[i]] == 0) kreg_[i] = vreg_[i] = u32x4{0u, 0u, 0u, 0u};
-      }
-    }
-    if (REG && t < KT) rreg = key0 + t < len ? krp[key0 + t] : 0u;
-  };
-  auto store = [&](int buf) {
-    u16* sK = smem + buf * BUF;
-    u16* sV = sK + KT * KSTR;
-#pragma unroll
-    for (int i = 0; i < PT; ++i) {
-      const int piece = t + 256 * i, row = piece / CH, ch = piece % CH;
-      *(u32x4*)&sK[row * KSTR + ch * 8] = kreg_[i];
-      *(u32x4*)&sV[row * VSTR + ch * 8] = vreg_[i];
-    }
-    if (REG && t < KT) sreg[buf * KT + t] = rreg;
-  };
-
-  f32x16 oacc[DP / 32];
-#pragma unroll
-  for (int dt = 0; dt < DP / 32; ++dt)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) oacc[dt][i] = 0.f;
-  float m = XA_LOWEST, l = 0.f;
-  if (t0 < t1) {
-    load(t0);
-    store(0);
-  }
-  __syncthreads();
-  for (int tile = t0; tile < t1; ++tile) {
-    const int cur = NB == 2 ? (tile - t0) & 1 : 0;
-    if (tile + 1 < t1) load(tile + 1);
-    const u16* sK = smem + cur * BUF + (WK == 1 ? 0 : wv * 32 * KSTR);
-    const u16* sV = smem + cur * BUF + KT * KSTR + (WK == 1 ? 0 : wv * 32 * VSTR);
-    const int key0 = tile * KT + (WK == 1 ? 0 : wv * 32);
+  const unsigned lds0 = lds_addr_of(smem) + wv * 1024;
+  auto stage = [&](int tile, int buf) {
+    const int key0 = tile * KT, left = min(len - key0, KT);
+    const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void*)(kb + (long long)key0 * p.ldk), 0, (unsigned)left * p.ldk * 2u, 0x00020000);
+    const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void*)(vb + (long long)key0 * p.ldv), 0, (unsigned)left * p.ldv * 2u, 0x00020000);
+    const unsigned dst = lds0 + buf * (S::BUF * 2);
     if constexpr (REG) {
-      xa_step<DP, KS, XA_REGIONS>(sK, sV, sreg + cur * KT + (WK == 1 ? 0 : wv * 32), qf, oacc, m, l, p.c, key0, len, qset, lane);
+      unsigned word[PT];
+#pragma unroll
+      for (int i = 0; i < PT; ++i) {
+        const int row = (t + 256 * i) / CH;
+        word[i] = row < left ? krp[key0 + row] : 0u;
+      }
+      if (t < KT) sreg[buf * KT + t] = t < left ? krp[key0 + t] : 0u;
+#pragma unroll
+      for (int i = 0; i < PT; ++i) dma_buf16(rk, koff[i], 0, dst + i * 4096);
+#pragma unroll
+      for (int i = 0; i < PT; ++i) dma_buf16(rv, word[i] ? voff[i] : DMA_OOB, 0, dst + KT * DP * 2 + i * 4096);
     } else {
-      if (tile * KT + KT <= len) xa_step<DP, KS, XA_FULL>(sK, sV, nullptr, qf, oacc, m, l, p.c, key0, len, 0u, lane);
-      else xa_step<DP, KS, XA_TAIL>(sK, sV, nullptr, qf, oacc, m, l, p.c, key0, len, 0u, lane);
+#pragma unroll
+      for (int i = 0; i < PT; ++i) dma_buf16(rk, koff[i], 0, dst + i * 4096);
+#pragma unroll
+      for (int i = 0; i < PT; ++i) dma_buf16(rv, voff[i], 0, dst + KT * DP * 2 + i * 4096);
     }
-    if (tile + 1 < t1) {
-      if constexpr (NB == 1) __syncthreads();
-      store(NB == 2 ? cur ^ 1 : 0);
-      __syncthreads();
-    }
-  }
-  l += __shfl_xor(l, 32);
-  const long long prow = ((long long)bz * p.kvh + hk) * p.rows + rho;
-  u16* O = p.o + (long long)bz * p.so + (long long)qi * p.ldo + head * p.dim;
+  };
+#define XA_LANDED() \
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory")
+  if (t0 < t1) stage(t0, 0);
 
-  if constexpr (WK == 1) {
-    if (!row_ok) return;
-    const float inv = l > 0.f ? 1.0f / l : 0.f;
-    if (p.splits > 1) {
-      if (hh == 0) p.pml[prow * p.splits + sp] = make_float2(m, l);
-      float* po = p.po + (prow * p.splits + sp) * p.dim;
+  // ---- this wave's rows: row rho of the kv head is query rho / group, head rho % group of the group
+  int qi[QT], head[QT], rho[QT];
+  hx8 qf[QT][DP / 16];
+  unsigned qset[QT];
+#pragma unroll
+  for (int x = 0; x < QT; ++x) {
+    rho[x] = rt * S::ROWS + (wr * QT + x) * 32 + r;
+    const int rc = min(rho[x], p.rows - 1);
+    qi[x] = rc / p.group;
+    head[x] = hk * p.group + rc % p.group;
+    const u16* Q = p.q + (long long)bz * p.sq + (long long)qi[x] * p.ldq + head[x] * p.dim;
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) {
+      const int d = 16 * ks + 8 * hh;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) qf[x][ks][e] = (h16)0.f;
+      if (d < p.dim) qf[x][ks] = *(const hx8*)(Q + d);
+    }
+    qset[x] = REG ? p.qreg[(long long)bz * p.sqr + qi[x]] : 0u;
+  }
+  f32x16 oacc[QT][DP / 32];
+  float m[QT], l[QT];
+#pragma unroll
+  for (int x = 0; x < QT; ++x) {
+    m[x] = XA_LOWEST;
+    l[x] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) oacc[x][dt][i] = 0.f;
+  }
+  const int kr0 = wk * (KT / WK), tfull = min(t1, len / KT);  // tiles below tfull are whole
+  XA_LANDED();
+  for (int tile = t0; tile < (REG ? t1 : tfull); ++tile) {
+    const int cur = (tile - t0) & 1;
+    if (tile + 1 < t1) stage(tile + 1, cur ^ 1);
+    const u16* sK = smem + cur * S::BUF;
+    xa_step<DP, QT, S::KS, REG ? XA_REGIONS : XA_FULL>(sK, sK + KT * DP, sreg + cur * KT, qf, oacc, m, l, p.c, kr0, 0, 0, qset, lane);
+    XA_LANDED();
+  }
+  if (!REG && t0 < t1 && tfull < t1) {  // the one partial tile: all sets of waves are past it, its data has landed
+    const u16* sK = smem + ((t1 - 1 - t0) & 1) * S::BUF;
+    xa_step<DP, QT, S::KS, XA_TAIL>(sK, sK + KT * DP, sreg, qf, oacc, m, l, p.c, kr0, (t1 - 1) * KT + kr0, len, qset, lane);
+  }
+#undef XA_LANDED
+#pragma unroll
+  for (int x = 0; x < QT; ++x) l[x] += __shfl_xor(l[x], 32);
+
+  if constexpr (WK > 1) {
+    // merge: m and l of the rows, then each share's O scaled to the common maximum; share wk of a row group finishes the groups
+    // g = wk, wk + WK, ... of every 32 columns, summing in the order of the shares
+    float* const mo = (float*)smem;                         // [wave][x][dt][16][64]
+    float2* const mml = (float2*)(mo + 4 * QT * 32 * DP);   // [wave][x][32]
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < QT; ++x)
+      if (hh == 0) mml[(wv * QT + x) * 32 + r] = make_float2(m[x], l[x]);
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < QT; ++x) {
+      float mall = XA_LOWEST, lall = 0.f;
+#pragma unroll
+      for (int w = 0; w < WK; ++w) mall = fmaxf(mall, mml[((wr * WK + w) * QT + x) * 32 + r].x);
+#pragma unroll
+      for (int w = 0; w < WK; ++w) {
+        const float2 v = mml[((wr * WK + w) * QT + x) * 32 + r];
+        lall += v.y * __builtin_amdgcn_exp2f(v.x - mall);
+      }
+      const float alpha = __builtin_amdgcn_exp2f(m[x] - mall);
+#pragma unroll
+      for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mo[(((wv * QT + x) * (DP / 32) + dt) * 16 + i) * 64 + lane] = oacc[x][dt][i] * alpha;
+      m[x] = mall;
+      l[x] = lall;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < QT; ++x)
 #pragma unroll
       for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const int d = 32 * dt + 8 * g + 4 * hh;
-          if (d < p.dim) *(f32x4*)(po + d) = f32x4{oacc[dt][4 * g], oacc[dt][4 * g + 1], oacc[dt][4 * g + 2], oacc[dt][4 * g + 3]};
+          if (g % WK != wk) continue;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float y = 0.f;
+#pragma unroll
+            for (int w = 0; w < WK; ++w) y += mo[((((wr * WK + w) * QT + x) * (DP / 32) + dt) * 16 + 4 * g + e) * 64 + lane];
+            oacc[x][dt][4 * g + e] = y;
+          }
         }
-      return;
-    }
+  }
+#pragma unroll
+  for (int x = 0; x < QT; ++x) {
+    if (rho[x] >= p.rows) continue;
+    const float inv = l[x] > 0.f ? 1.0f / l[x] : 0.f;
+    const long long prow = ((long long)bz * p.kvh + hk) * p.rows + rho[x];
+    float* po = p.po + (prow * p.splits + sp) * p.dim;
+    u16* O = p.o + (long long)bz * p.so + (long long)qi[x] * p.ldo + head[x] * p.dim;
+    if (p.splits > 1 && wk == 0 && hh == 0) p.pml[prow * p.splits + sp] = make_float2(m[x], l[x]);
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const int d = 32 * dt + 8 * g + 4 * hh;
-        if (d < p.dim)
-          *(uint2*)(O + d) = make_uint2(pack2h(oacc[dt][4 * g] * inv, oacc[dt][4 * g + 1] * inv), pack2h(oacc[dt][4 * g + 2] * inv, oacc[dt][4 * g + 3] * inv));
-      }
-  } else {
-    // merge the four waves: m and l of the 32 rows, then each wave's O scaled to the common maximum, summed in wave order
-    float* const mo = (float*)smem;                    // [wave][dt][16][64]
-    float2* const mml = (float2*)(mo + 4 * 32 * DP);   // [wave][32]
-    __syncthreads();
-    if (hh == 0) mml[wv * 32 + r] = make_float2(m, l);
-    __syncthreads();
-    float2 w4[4];
-#pragma unroll
-    for (int w = 0; w < 4; ++w) w4[w] = mml[w * 32 + r];
-    const float mall = fmaxf(fmaxf(w4[0].x, w4[1].x), fmaxf(w4[2].x, w4[3].x));
-    float lall = 0.f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) lall += w4[w].y * __builtin_amdgcn_exp2f(w4[w].x - mall);
-    const float alpha = __builtin_amdgcn_exp2f(m - mall);
-#pragma unroll
-    for (int dt = 0; dt < DP / 32; ++dt)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) mo[((wv * (DP / 32) + dt) * 16 + i) * 64 + lane] = oacc[dt][i] * alpha;
-    __syncthreads();
-    if (!row_ok) return;
-    const float inv = lall > 0.f ? 1.0f / lall : 0.f;
-    if (p.splits > 1 && wv == 0 && hh == 0) p.pml[prow * p.splits + sp] = make_float2(mall, lall);
-    float* po = p.po + (prow * p.splits + sp) * p.dim;
-#pragma unroll
-    for (int x = 0; x < DP / 32; ++x) {  // wave w finishes the groups g = w of every 32 columns
-      const int d = 32 * x + 8 * wv + 4 * hh;
-      float y[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        y[e] = 0.f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) y[e] += mo[((w * (DP / 32) + x) * 16 + 4 * wv + e) * 64 + lane];
-      }
-      if (d < p.dim) {
-        if (p.splits > 1) *(f32x4*)(po + d) = f32x4{y[0], y[1], y[2], y[3]};
+        if (g % WK != wk || d >= p.dim) continue;
+        const f32x4 y = {oacc[x][dt][4 * g], oacc[x][dt][4 * g + 1], oacc[x][dt][4 * g + 2], oacc[x][dt][4 * g + 3]};
+        if (p.splits > 1) *(f32x4*)(po + d) = y;
         else *(uint2*)(O + d) = make_uint2(pack2h(y[0] * inv, y[1] * inv), pack2h(y[2] * inv, y[3] * inv));
       }
-    }
   }
 }
 
@@ -323,23 +331,30 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(const XattnParams p, lo
   const float* po = p.po + row * p.splits * p.dim;
   for (int d0 = 0; d0 < p.dim; d0 += 128) {  // every lane takes part: the weights come from all of them
     const int d = d0 + 2 * lane;
+    const float* pd = po + (d < p.dim ? d : 0);
     float y0 = 0.f, y1 = 0.f;
-    for (int s = 0; s < p.splits; ++s) {
-      const float as = __shfl(a, s);
-      const float2 v = d < p.dim ? *(const float2*)(po + (long long)s * p.dim + d) : make_float2(0.f, 0.f);
-      y0 += as * v.x;
-      y1 += as * v.y;
+    for (int s0 = 0; s0 < p.splits; s0 += 8) {  // eight splits' loads in flight: one memory latency for all of them
+      float2 v[8];
+#pragma unroll
+      for (int s = 0; s < 8; ++s) v[s] = *(const float2*)(pd + (long long)min(s0 + s, p.splits - 1) * p.dim);
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+        const float as = s0 + s < p.splits ? __shfl(a, s0 + s) : 0.f;
+        y0 += as * v[s].x;
+        y1 += as * v[s].y;
+      }
     }
     if (d < p.dim) *(uint32_t*)(O + d) = pack2h(y0 * inv, y1 * inv);
   }
 }
 
 // ------------------------------------------------------------------------------------------------------------ host
-struct XattnPlan { int wk, rtiles, splits; };
-static XattnPlan xattn_plan(int batch, int kvh, int rows, int nkv) {
+struct XattnPlan { int kind, rtiles, splits; };  // kind 0: 128 rows a block, 1: 128 rows in 64-row waves by two key shares, 2: few rows
+static XattnPlan xattn_plan(int batch, int kvh, int dim, int rows, int nkv) {
   XattnPlan pl;
-  pl.wk = rows <= 64 ? 4 : 1;
-  pl.rtiles = (rows + (pl.wk == 4 ? 31 : 127)) / (pl.wk == 4 ? 32 : 128);
+  pl.kind = rows <= 64 ? 2 : (dim <= 64 && nkv >= 512) ? 1 : 0;
+  const int per = pl.kind == 2 ? (dim <= 128 ? 32 : 64) : 128;
+  pl.rtiles = (rows + per - 1) / per;
   const long long blocks = (long long)batch * kvh * pl.rtiles;
   // few rows over long states: cut the keys until the chip is full (512 blocks: two per CU), at least 256 keys to a piece
   long long s = 512 / (blocks > 0 ? blocks : 1);
@@ -349,9 +364,9 @@ static XattnPlan xattn_plan(int batch, int kvh, int rows, int nkv) {
   return pl;
 }
 
-template <int DP, int WK, bool REG>
+template <int DP, int QT, int WK, int KT, bool REG>
 static int xattn_launch2(const XattnParams& p, int blocks, hipStream_t st) {
-  constexpr int bytes = xa_lds_bytes<DP, WK>();
+  constexpr int bytes = XaShape<DP, QT, WK, KT, REG>::bytes;
   static_assert(bytes <= 160 * 1024, "LDS of a CU");
   if constexpr (bytes > 64 * 1024) {
     static std::atomic<unsigned long long> done{0};
@@ -359,7 +374,7 @@ static int xattn_launch2(const XattnParams& p, int blocks, hipStream_t st) {
     (void)hipGetDevice(&dev);
     const unsigned long long bit = 1ull << (dev & 63);
     if (!(done.load(std::memory_order_relaxed) & bit)) {
-      const hipError_t e = hipFuncSetAttribute((const void*)xattn_kernel<DP, WK, REG>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+      const hipError_t e = hipFuncSetAttribute((const void*)xattn_kernel<DP, QT, WK, KT, REG>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
       if (e != hipSuccess) {
         sdmi_set_error("cross_attention: %d bytes of LDS refused: %s", bytes, hipGetErrorString(e));
         return SDMI_ELAUNCH;
@@ -367,14 +382,20 @@ static int xattn_launch2(const XattnParams& p, int blocks, hipStream_t st) {
       done.fetch_or(bit, std::memory_order_relaxed);
     }
   }
-  hipLaunchKernelGGL((xattn_kernel<DP, WK, REG>), dim3(blocks), dim3(256), bytes, st, p);
-  sdmi_note_kernel("xattn_kernel<%d, %d, %s>%s", DP, WK, REG ? "true" : "false", p.splits > 1 ? " + xattn_join_kernel" : "");
+  hipLaunchKernelGGL((xattn_kernel<DP, QT, WK, KT, REG>), dim3(blocks), dim3(256), bytes, st, p);
+  sdmi_note_kernel("xattn_kernel<%d, %d, %d, %d, %s>%s", DP, QT, WK, KT, REG ? "true" : "false", p.splits > 1 ? " + xattn_join_kernel" : "");
   return sdmi_check_launch("cross_attention");
 }
+template <int DP, int QT, int WK, int KT>
+static int xattn_launch1(const XattnParams& p, int blocks, hipStream_t st) {
+  return p.qreg ? xattn_launch2<DP, QT, WK, KT, true>(p, blocks, st) : xattn_launch2<DP, QT, WK, KT, false>(p, blocks, st);
+}
 template <int DP>
-static int xattn_launch(const XattnParams& p, int wk, int blocks, hipStream_t st) {
-  if (wk == 4) return p.qreg ? xattn_launch2<DP, 4, true>(p, blocks, st) : xattn_launch2<DP, 4, false>(p, blocks, st);
-  return p.qreg ? xattn_launch2<DP, 1, true>(p, blocks, st) : xattn_launch2<DP, 1, false>(p, blocks, st);
+static int xattn_launch(const XattnParams& p, int kind, int blocks, hipStream_t st) {
+  if constexpr (DP <= 64)
+    if (kind == 1) return xattn_launch1<DP, 2, 2, 128>(p, blocks, st);
+  if (kind == 2) return xattn_launch1<DP, 1, DP <= 128 ? 4 : 2, DP <= 128 ? 128 : 64>(p, blocks, st);
+  return xattn_launch1<DP, 1, 1, 64>(p, blocks, st);
 }
 
 static bool xattn_shape_ok(int batch, int heads, int kv_heads, int dim, int nq, int nkv) {
@@ -384,7 +405,7 @@ static bool xattn_shape_ok(int batch, int heads, int kv_heads, int dim, int nq, 
 
 extern "C" int64_t sdmi_cross_attention_ws_bytes(int batch, int heads, int kv_heads, int dim, int nq, int nkv) {
   if (!xattn_shape_ok(batch, heads, kv_heads, dim, nq, nkv)) return 0;
-  const XattnPlan pl = xattn_plan(batch, kv_heads, nq * (heads / kv_heads), nkv);
+  const XattnPlan pl = xattn_plan(batch, kv_heads, dim, nq * (heads / kv_heads), nkv);
   return pl.splits == 1 ? 0 : (int64_t)batch * heads * nq * pl.splits * ((int64_t)dim * 4 + 8);
 }
 
@@ -413,7 +434,7 @@ extern "C" int sdmi_cross_attention(const void* q, int ldq, int64_t sq, const vo
   p.rows = nq * p.group;
   p.index = index; p.lens = lens; p.qreg = query_regions; p.kreg = key_regions; p.sqr = sqr; p.skr = skr;
   p.c = scale * 1.44269504088896340736f;
-  XattnPlan pl = xattn_plan(batch, kv_heads, p.rows, nkv);
+  XattnPlan pl = xattn_plan(batch, kv_heads, dim, p.rows, nkv);
   const int64_t prows = (int64_t)batch * heads * nq;
   if (pl.splits > 1 && (!ws || ws_bytes < prows * pl.splits * ((int64_t)dim * 4 + 8))) pl.splits = 1;  // as with split-K: no room, no split
   SDMI_REQUIRE(pl.splits == 1 || ((uintptr_t)ws & 15) == 0, "cross_attention: workspace alignment");
@@ -424,12 +445,12 @@ extern "C" int sdmi_cross_attention(const void* q, int ldq, int64_t sq, const vo
   SDMI_REQUIRE(blocks < (1ll << 31) && (prows + 3) / 4 < (1ll << 31), "cross_attention: grid too large");
   hipStream_t st = (hipStream_t)stream;
   int rc;
-  if (dim <= 32) rc = xattn_launch<32>(p, pl.wk, (int)blocks, st);
-  else if (dim <= 64) rc = xattn_launch<64>(p, pl.wk, (int)blocks, st);
-  else if (dim <= 96) rc = xattn_launch<96>(p, pl.wk, (int)blocks, st);
-  else if (dim <= 128) rc = xattn_launch<128>(p, pl.wk, (int)blocks, st);
-  else if (dim <= 160) rc = xattn_launch<160>(p, pl.wk, (int)blocks, st);
-  else rc = xattn_launch<256>(p, pl.wk, (int)blocks, st);
+  if (dim <= 32) rc = xattn_launch<32>(p, pl.kind, (int)blocks, st);
+  else if (dim <= 64) rc = xattn_launch<64>(p, pl.kind, (int)blocks, st);
+  else if (dim <= 96) rc = xattn_launch<96>(p, pl.kind, (int)blocks, st);
+  else if (dim <= 128) rc = xattn_launch<128>(p, pl.kind, (int)blocks, st);
+  else if (dim <= 160) rc = xattn_launch<160>(p, pl.kind, (int)blocks, st);
+  else rc = xattn_launch<256>(p, pl.kind, (int)blocks, st);
   if (rc != SDMI_OK || pl.splits == 1) return rc;
   hipLaunchKernelGGL(xattn_join_kernel, dim3((unsigned)((prows + 3) / 4)), dim3(256), 0, st, p, (long long)prows);
   return sdmi_check_launch("cross_attention (join)");
