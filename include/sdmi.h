@@ -305,9 +305,10 @@ int64_t sdmi_cross_attention_ws_bytes(int batch, int heads, int kv_heads, int di
  *      [adapters][groups * rank][k], lora_b h16 [adapters][n][rank], lora_scale fp32 [adapters], ids int32
  *      [ceil(m / rows_per_id)]; an id outside [0, adapters) leaves its rows without an adapter.  groups > 1: w stacks that many
  *      projections along n; group g is columns [g n / groups, (g + 1) n / groups) and rows [g rank, (g + 1) rank) of lora_a.
- *      Adapters of smaller rank are padded with zeros (sdmi_pack_linear, sdmi_f32_to_h16_rows write both layouts).  n, k, rank
- *      multiples of 8, rank up to 256; flags: SDMI_F_BIAS, SDMI_F_RESIDUAL; ws: scratch of sdmi_lora_gemm_ws_bytes, one per call
- *      that may overlap in time. */
+ *      Adapters of smaller rank are padded with zeros (sdmi_pack_linear, sdmi_f32_to_h16_rows write both layouts).  k, rank
+ *      and n / groups multiples of 8, rank up to 256, up to 64 groups; flags: SDMI_F_BIAS, SDMI_F_RESIDUAL; ws: scratch of
+ *      sdmi_lora_gemm_ws_bytes (0: may be NULL), one per call that may overlap in time.  All pointers but lora_scale and ids are
+ *      16-byte aligned. */
 int sdmi_lora_gemm(const void* x, int ldx, const void* w, int ldw, void* out, int ldo, int m, int n, int k, const float* bias,
                    const void* residual, int ldr, const void* lora_a, const void* lora_b, const float* lora_scale, int adapters,
                    int rank, int groups, const int32_t* ids, int rows_per_id, uint32_t flags, void* ws, int64_t ws_bytes, void* stream);

@@ -6,12 +6,15 @@
 // ids outside [0, adapters) mean "no adapter" for their rows.  `groups` low-rank pairs stand side by side along N: the fused
 // q|k|v projection (layers/SpatialTransformer.py:62-64) has one pair for each of its three parts.
 //
-// Two launches: t first (reads x once more: 2 m k bytes, and each adapter's a once per row tile), then the product, in which
-// the adapters are more K: behind the K-tiles of (x, w) come tiles whose 16-byte pieces are (t, b) of the (adapter, group)
-// pairs that occur in the block's rows and columns, zeros where a row belongs to another adapter.  They pass through the same
-// LDS ring and the same MFMAs, so one fp32 accumulator holds the sum and the result is rounded once.  t is rounded to 16 bits
-// between the launches, as the matrix cores take it: half a step of t, weighted like the other products' factors.
+// Two launches: t first (lora_shrink_kernel: reads x once more, 2 m k bytes, and each adapter's a once per 16 rows), then the
+// product.  t is rounded to 16 bits between them, as the matrix cores take it: half a step of t, weighted like the other
+// products' factors; every sum is fp32 and the result is rounded once.
+//   - many rows (lora_gemm_kernel): the adapters are more K.  Behind the K-tiles of (x, w) come tiles whose 16-byte pieces are
+//     (t, b); they pass through the same LDS ring and the same MFMAs into the same accumulators.
+//   - up to 64 rows (lora_rows_kernel; one token of each request): the product is a stream over w, the adapters' b rows are read
+//     once per request beside it.  With few rows and ranks it computes t as well: one launch.
 #include "common.h"
+#include <atomic>
 
 __device__ __attribute__((aligned(16))) unsigned g_lora_zero16[4] = {0u, 0u, 0u, 0u};
 
@@ -26,8 +29,8 @@ struct LoraParams {
   const float* scale;
   const int* ids;
   int adapters, rank, groups, rpi;
-  u16* t;   // [M][groups * rank]
-  int ldt;
+  u16* t;  // [M][groups * rank]
+  int ldt, tiles_n, per, tpg;  // per = N / groups; request-aligned tiles: tpg column tiles to a group
 };
 
 __device__ __forceinline__ int lora_id(const LoraParams& p, int row) {
@@ -36,66 +39,176 @@ __device__ __forceinline__ int lora_id(const LoraParams& p, int row) {
 }
 
 // ------------------------------------------------------------------------------------------------------------ t = scale x a^T
-// Block: 16 rows x up to 64 columns of t, K cut over the four waves (32 of it a step), joined in wave order through the LDS.
-// Operands come straight from memory in fragment layout (8 consecutive k of one row per lane).  Rows of several adapters: one
-// sweep for each, every row keeping its own.
-constexpr int SHR_NT = 4;  // 16-column tiles a block computes
-__global__ __launch_bounds__(256) void lora_shrink_kernel(const LoraParams p) {
-  __shared__ float red[3][SHR_NT * 4][64];
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, l15 = lane & 15, lq = lane >> 4;
-  const int row = blockIdx.x * 16 + l15, rowc = min(row, p.M - 1), n0 = blockIdx.y * (SHR_NT * 16), NR = p.groups * p.rank;
+// Block: RW x 16 rows by 16 NT columns of t, K cut over KW waves (32 of it a step), joined in wave order through the LDS; a wave
+// works for ONE adapter: blockIdx.z is the z-th distinct one among its 16 rows, every row keeps its own adapter's result, waves
+// beyond the last one have nothing to do.  Operands come straight from memory in fragment layout (8 consecutive k of one row
+// per lane); UN steps' loads are issued before the first product waits for one.
+template <int NT, int RW, int KW>
+__global__ __launch_bounds__(64 * RW * KW, 1) void lora_shrink_kernel(const LoraParams p) {
+  constexpr int UN = NT == 4 ? 5 : 10;
+  __shared__ float red[RW][KW > 1 ? KW - 1 : 1][KW > 1 ? NT * 4 : 1][64];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, rw = wv / KW, kw = wv % KW, l15 = lane & 15, lq = lane >> 4;
+  const int row = (blockIdx.x * RW + rw) * 16 + l15, rowc = min(row, p.M - 1), n0 = blockIdx.y * (NT * 16), NR = p.ldt;
   const int mine = row < p.M ? lora_id(p, row) : -1;
-  const u16* xr = p.x + (long long)rowc * p.ldx;
-  unsigned long long todo = __builtin_amdgcn_ballot_w64(mine >= 0);  // the same in every wave
-  while (todo) {
-    const int id = __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo));
+  unsigned long long todo = __builtin_amdgcn_ballot_w64(mine >= 0);  // the same in every wave of a row tile
+  int id = 0;
+  for (int z = blockIdx.z; todo; --z) {
+    id = __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo));
+    if (z == 0) break;
     todo &= ~__builtin_amdgcn_ballot_w64(mine == id);
-    const u16* ab = p.la + (long long)id * NR * p.K;
-    f32x4 acc[SHR_NT];
+  }
+  f32x4 acc[NT];
 #pragma unroll
-    for (int j = 0; j < SHR_NT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const u16* ar[SHR_NT];
+  for (int j = 0; j < NT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (todo) {
+    const u16* const zp = (const u16*)g_lora_zero16;
+    const u16* xr = p.x + (long long)rowc * p.ldx + 8 * lq;
+    const u16* ar[NT];
 #pragma unroll
-    for (int j = 0; j < SHR_NT; ++j) ar[j] = ab + (long long)min(n0 + 16 * j + l15, NR - 1) * p.K;
-#pragma unroll 4
-    for (int kb = wv * 32; kb < p.K; kb += 128) {
-      const int k = kb + 8 * lq;
-      hx8 xf, af[SHR_NT];
+    for (int j = 0; j < NT; ++j) ar[j] = p.la + ((long long)id * NR + min(n0 + 16 * j + l15, NR - 1)) * p.K;
+    for (int kb = kw * 32; kb < p.K; kb += 32 * KW * UN) {
+      hx8 xf[UN], af[UN][NT];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) xf[e] = (h16)0.f;
+      for (int u = 0; u < UN; ++u) {
+        const int k = kb + 32 * KW * u;
+        const bool in = k + 8 * lq < p.K;  // K is a multiple of 8; past it x reads as zeros, and a as its first columns
+        xf[u] = *(const hx8*)(in ? xr + k : zp);
 #pragma unroll
-      for (int j = 0; j < SHR_NT; ++j) af[j] = xf;
-      if (k < p.K) {
-        xf = *(const hx8*)(xr + k);
-#pragma unroll
-        for (int j = 0; j < SHR_NT; ++j) af[j] = *(const hx8*)(ar[j] + k);
+        for (int j = 0; j < NT; ++j) af[u][j] = *(const hx8*)(ar[j] + (in ? k + 8 * lq : 0));
       }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int j = 0; j < SHR_NT; ++j) acc[j] = MFMA16(af[j], xf, acc[j], 0, 0, 0);
+      for (int u = 0; u < UN; ++u)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[j] = MFMA16(af[u][j], xf[u], acc[j], 0, 0, 0);
     }
-    if (wv > 0) {
+  }
+  if constexpr (KW > 1) {
+    if (kw > 0) {
 #pragma unroll
-      for (int j = 0; j < SHR_NT; ++j)
+      for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) red[wv - 1][4 * j + i][lane] = acc[j][i];
-    }
-    __syncthreads();
-    if (wv == 0 && mine == id) {
-      const float sc = p.scale[id];
-#pragma unroll
-      for (int j = 0; j < SHR_NT; ++j) {
-        float y[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = (((acc[j][i] + red[0][4 * j + i][lane]) + red[1][4 * j + i][lane]) + red[2][4 * j + i][lane]) * sc;
-        const int n = n0 + 16 * j + 4 * lq;
-        if (n < NR) *(uint2*)(p.t + (long long)row * p.ldt + n) = make_uint2(pack2h(y[0], y[1]), pack2h(y[2], y[3]));
-      }
+        for (int i = 0; i < 4; ++i) red[rw][kw - 1][4 * j + i][lane] = acc[j][i];
     }
     __syncthreads();
   }
+  if (kw == 0 && todo && mine == id) {
+    const float sc = p.scale[id];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      float y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        y[i] = acc[j][i];
+        if constexpr (KW > 1) {
+#pragma unroll
+          for (int w = 0; w < KW - 1; ++w) y[i] += red[rw][w][4 * j + i][lane];
+        }
+        y[i] *= sc;
+      }
+      const int n = n0 + 16 * j + 4 * lq;
+      if (n < NR) *(uint2*)(p.t + (long long)row * p.ldt + n) = make_uint2(pack2h(y[0], y[1]), pack2h(y[2], y[3]));
+    }
+  }
 }
 
-// ------------------------------------------------------------------------------------------------------------ the product
+// ------------------------------------------------------------------------------------------------------------ up to 64 rows
+// Block: 16 columns x all M <= 16 MT rows, K cut over 8 waves (32 of it a step), fragments straight from memory: w is read once by
+// the whole grid, x by every block (L2).  The adapters: thread (m, n) takes the dot product of t[m] and b[id][n], rank long, from
+// memory too.  FUSE: the block computes t of its rows itself (m * groups * rank <= 64 dot products of length K, one wave each
+// in turn) instead of reading what an earlier launch left.
+template <int MT, bool FUSE>
+__global__ __launch_bounds__(512, 1) void lora_rows_kernel(const LoraParams p) {
+  constexpr int UN = MT == 4 ? 4 : 8;
+  __shared__ float red[8][MT * 4][64];
+  __shared__ float st[FUSE ? 64 : 1];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, l15 = lane & 15, lq = lane >> 4, n0 = blockIdx.x * 16;
+  const u16* const zp = (const u16*)g_lora_zero16;
+  if constexpr (FUSE) {
+    // only the groups that this block's columns lie in
+    const int g0 = n0 / p.per, g1 = min(n0 + 15, p.N - 1) / p.per, ng = (g1 - g0 + 1) * p.rank;
+    for (int d = wv; d < p.M * ng; d += 8) {
+      const int m = d / ng, r = g0 * p.rank + (d - m * ng), id = lora_id(p, m);
+      if (id < 0) continue;
+      const u16 *xr = p.x + (long long)m * p.ldx, *ar = p.la + ((long long)id * p.ldt + r) * p.K;
+      float s = 0.f;
+      for (int k = 8 * lane; k < p.K; k += 512) {
+        float xv[8], av[8];
+        unpack8(*(const uint4*)(xr + k), xv);
+        unpack8(*(const uint4*)(ar + k), av);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s = __builtin_fmaf(xv[e], av[e], s);
+      }
+      s = wave_sum(s);
+      if (lane == 0) st[m * p.ldt + r] = (float)f2h16(s * p.scale[id]);  // rounded as the stored t is
+    }
+  }
+  f32x4 acc[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  {
+    const u16* wrow = p.w + (long long)min(n0 + l15, p.N - 1) * p.ldw;
+    const u16* xr[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) xr[i] = p.x + (long long)min(16 * i + l15, p.M - 1) * p.ldx + 8 * lq;
+    for (int kb = wv * 32; kb < p.K; kb += 256 * UN) {
+      hx8 wf[UN], xf[UN][MT];
+#pragma unroll
+      for (int u = 0; u < UN; ++u) {
+        const int k = kb + 256 * u;
+        const bool in = k + 8 * lq < p.K;
+        wf[u] = *(const hx8*)(wrow + (in ? k + 8 * lq : 0));
+#pragma unroll
+        for (int i = 0; i < MT; ++i) xf[u][i] = *(const hx8*)(in ? xr[i] + k : zp);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int u = 0; u < UN; ++u)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[i] = MFMA16(wf[u], xf[u][i], acc[i], 0, 0, 0);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) red[wv][4 * i + e][lane] = acc[i][e];  // row 16 i + l15, column 4 lq + e
+  __syncthreads();
+  // thread -> (row, column): 16 neighbouring threads share a row and read 16 consecutive b rows
+  const int c = threadIdx.x & 15, n = n0 + c;
+  if (n >= p.N) return;
+  const int g = n / p.per;
+#pragma unroll
+  for (int m0 = 0; m0 < MT * 16; m0 += 32) {
+    const int m = m0 + (threadIdx.x >> 4);
+    if (m >= p.M || m >= MT * 16) continue;
+    float y = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) y += red[w][4 * (m >> 4) + (c & 3)][(c >> 2) * 16 + (m & 15)];
+    const int id = lora_id(p, m);
+    if (id >= 0) {
+      const u16* br = p.lb + ((long long)id * p.N + n) * p.rank;
+      const u16* tr = p.t + (long long)m * p.ldt + g * p.rank;
+#pragma unroll 4
+      for (int r = 0; r < p.rank; r += 8) {
+        float bv[8], tv[8];
+        unpack8(*(const uint4*)(br + r), bv);
+        if constexpr (FUSE) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) tv[e] = st[m * p.ldt + g * p.rank + r + e];
+        } else {
+          unpack8(*(const uint4*)(tr + r), tv);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y = __builtin_fmaf(tv[e], bv[e], y);
+      }
+    }
+    if (p.bias) y += p.bias[n];
+    if (p.residual) y += h2f(p.residual[(long long)m * p.ldr + n]);
+    p.out[(long long)m * p.ldo + n] = f2h(y);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------ many rows
 constexpr int LBK = 64;
 __device__ __forceinline__ int lora_off(int row, int chunk) { return row * LBK + ((chunk ^ ((row >> 1) & 7)) << 3); }
 // 64 lanes x 16 B from 64 addresses to 1 KB of LDS at byte address `lds`; waited for by the loop's own s_waitcnt
@@ -103,43 +216,29 @@ __device__ __forceinline__ void lora_dma16(const void* src, unsigned lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory", "m0");
 }
 
-template <int BM, int BN, int WM, int WN, int NSTAGE>
-__global__ __launch_bounds__(64 * WM * WN, 2) void lora_gemm_kernel(const LoraParams p) {
+// MIXED = false: a tile lies inside one request and one group (the grid is laid out by them), so its adapter is one scalar and the
+// adapter's K-tiles are strided like the others.  MIXED = true (requests of fewer rows than a tile): tiles of consecutive rows; the
+// first wave lists the distinct adapters of the block's rows, and the adapters' K-tiles are gathered piece by piece.
+template <int BM, int BN, int WM, int WN, int NSTAGE, bool MIXED>
+__global__ __launch_bounds__(64 * WM * WN, (WM * WN == 4 && NSTAGE * (BM + BN) * LBK * 2 <= 80 * 1024) || WM * WN == 8 ? 2 : 1) void lora_gemm_kernel(const LoraParams p) {
   constexpr int NTH = 64 * WM * WN, RP = NTH / 8, TM = BM / WM, TN = BN / WN, MT = TM / 16, NT = TN / 16, PA = BM / RP, PB = BN / RP;
   constexpr int STAGE = (BM + BN) * LBK;
-  static_assert(BM % RP == 0 && BN % RP == 0 && RP % 16 == 0 && BM <= 128, "tile / wave grid mismatch");
-  extern __shared__ __attribute__((aligned(16))) u16 smem[];  // the ring, then rowid[BM], the list of adapters [BM] and its length
+  static_assert(BM % RP == 0 && BN % RP == 0 && RP % 16 == 0 && NT % 2 == 0, "tile / wave grid mismatch");
+  extern __shared__ __attribute__((aligned(16))) u16 smem[];  // the ring; MIXED: then rowid[BM], the list of adapters [BM] and its length
   int* const rowid = (int*)(smem + NSTAGE * STAGE);
   int* const list = rowid + BM;
-  const int t = threadIdx.x, lane = t & 63, wv = t >> 6, wr = wv / WN, wc = wv % WN, l15 = lane & 15, lq = lane >> 4;
-  const int tiles_n = (p.N + BN - 1) / BN, tiles_m = (p.M + BM - 1) / BM;
-  const int bid = xcd_remap(blockIdx.x, tiles_m * tiles_n);
-  const int brow = bid / tiles_n * BM, bcol = bid % tiles_n * BN;
-
-  const int r0 = t >> 3, lchunk = (t & 7) ^ ((r0 >> 1) & 7), wave_row0 = __builtin_amdgcn_readfirstlane(wv) * 8;
-  const __amdgpu_buffer_rsrc_t rsrcA = __builtin_amdgcn_make_buffer_rsrc((void*)(p.x + (long long)brow * p.ldx), 0, DMA_OOB, 0x00020000);
-  const __amdgpu_buffer_rsrc_t rsrcB = __builtin_amdgcn_make_buffer_rsrc((void*)(p.w + (long long)bcol * p.ldw), 0, DMA_OOB, 0x00020000);
-  unsigned a_voff[PA], b_voff[PB];
-#pragma unroll
-  for (int i = 0; i < PA; ++i) a_voff[i] = brow + r0 + RP * i < p.M ? (unsigned)(((r0 + RP * i) * p.ldx + lchunk * 8) * 2) : DMA_OOB;
-#pragma unroll
-  for (int i = 0; i < PB; ++i) b_voff[i] = bcol + r0 + RP * i < p.N ? (unsigned)(((r0 + RP * i) * p.ldw + lchunk * 8) * 2) : DMA_OOB;
-  const unsigned lds0 = lds_addr_of(smem);
-
-  // ---- the adapters of this block's rows.  One request covers them all (the usual case for images): a scalar load.  Else the
-  // first wave lists the distinct ones, in the order of their first rows.
-  const int last = min(brow + BM, p.M) - 1;
-  const bool one = brow / p.rpi == last / p.rpi;
-  int id0 = -1, nids;
-  if (one) {
-    id0 = lora_id(p, brow);
-    nids = id0 >= 0 ? 1 : 0;
-  } else {
-    if (t < BM) rowid[t] = brow + t <= last ? lora_id(p, brow + t) : -1;
+  const int t = threadIdx.x, lane = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6), wr = wv / WN, wc = wv % WN, l15 = lane & 15, lq = lane >> 4;
+  const int bid = xcd_remap(blockIdx.x, gridDim.x);
+  const int mt = __builtin_amdgcn_readfirstlane(bid / p.tiles_n), nt = bid - mt * p.tiles_n;
+  const int per = p.per;
+  int brow, rend, bcol, cend, g_lo, ng = 1, nids, id0 = -1;
+  if constexpr (MIXED) {
+    brow = mt * BM; rend = min(brow + BM, p.M); bcol = nt * BN; cend = min(bcol + BN, p.N);
+    g_lo = bcol / per; ng = (cend - 1) / per - g_lo + 1;
+    if (t < BM) rowid[t] = brow + t < rend ? lora_id(p, brow + t) : -1;
     __syncthreads();
     if (wv == 0) {
-      int n = 0;
-      int v[(BM + 63) / 64];
+      int n = 0, v[(BM + 63) / 64];
 #pragma unroll
       for (int h = 0; h < (BM + 63) / 64; ++h) v[h] = 64 * h + lane < BM ? rowid[64 * h + lane] : -1;
 #pragma unroll
@@ -158,38 +257,65 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void lora_gemm_kernel(const LoraPa
       if (lane == 0) list[BM] = n;
     }
     __syncthreads();
-    nids = list[BM];
+    nids = __builtin_amdgcn_readfirstlane(list[BM]);
+  } else {
+    const int tm = (p.rpi + BM - 1) / BM;
+    const int req = __builtin_amdgcn_readfirstlane(mt / tm);
+    brow = req * p.rpi + (mt - req * tm) * BM;
+    rend = min(min(brow + BM, (req + 1) * p.rpi), p.M);
+    if (brow >= rend) return;  // the last request may be shorter
+    g_lo = __builtin_amdgcn_readfirstlane(nt / p.tpg);
+    bcol = g_lo * per + (nt - g_lo * p.tpg) * BN;
+    cend = min(bcol + BN, (g_lo + 1) * per);
+    id0 = __builtin_amdgcn_readfirstlane(p.ids[req]);
+    id0 = id0 < p.adapters ? id0 : -1;
+    nids = id0 >= 0 ? 1 : 0;
   }
-  const int per = p.N / p.groups;
-  const int g_lo = bcol / per, ng = (min(bcol + BN, p.N) - 1) / per - g_lo + 1;
-  const int r8 = p.rank >> 3, nslots = nids * ng;
-  const int ntot = p.nk + (nslots * r8 + 7) / 8;
-  const u16* const zp = (const u16*)g_lora_zero16;
 
-  // K-tile KT into ring slot SLOT; always PA + PB DMA instructions per wave, so that the counted waits below hold
+  const int r0 = t >> 3, lchunk = (t & 7) ^ ((r0 >> 1) & 7);
+  const u16* const xa = p.x + (long long)brow * p.ldx;
+  const u16* const wb = p.w + (long long)bcol * p.ldw;
+  // MIXED = false: the adapter's panels, t of these rows and b of these columns
+  const u16* const ta = p.t + (long long)brow * p.ldt + g_lo * p.rank;
+  const u16* const lb = p.lb + ((long long)(id0 < 0 ? 0 : id0) * p.N + bcol) * p.rank;
+  const unsigned lds0 = lds_addr_of(smem) + wv * 1024;
+  const int nslots = nids * ng, r8 = p.rank >> 3, rk = nids ? p.rank : 0;
+  const int ntot = p.nk + (nslots * r8 + 7) / 8;
+
+  // K-tile KT into ring slot SLOT; always PA + PB DMA instructions per wave (past the last tile: zeros), so that the counted waits
+  // below hold
   auto stage = [&](int kt, int slot) {
-    const unsigned la = lds0 + (slot * STAGE + wave_row0 * LBK) * 2;
-    if (kt < p.nk || kt >= ntot) {
-      const bool in = kt * LBK + lchunk * 8 < p.K;
-      const int soff = kt * (LBK * 2);
+    const unsigned la = lds0 + slot * (STAGE * 2);
+    if (!MIXED || kt < p.nk || kt >= ntot) {
+      const bool ext = !MIXED && kt >= p.nk;
+      const int k0 = (ext ? kt - p.nk : kt) * LBK, klim = ext ? rk : p.K;
+      const int lda = ext ? p.ldt : p.ldx, ldb = ext ? p.rank : p.ldw;
+      const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc((void*)(ext ? ta : xa), 0, DMA_OOB, 0x00020000);
+      const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc((void*)(ext ? lb : wb), 0, DMA_OOB, 0x00020000);
+      const unsigned v = 2u * (k0 + lchunk * 8);
+      const bool in = k0 + lchunk * 8 < klim;
 #pragma unroll
-      for (int i = 0; i < PA; ++i) dma_buf16(rsrcA, in ? a_voff[i] : DMA_OOB, soff, la + i * (RP * LBK * 2));
+      for (int i = 0; i < PA; ++i)
+        dma_buf16(ra, in & (brow + r0 + RP * i < rend) ? v + 2u * (unsigned)((r0 + RP * i) * lda) : DMA_OOB, 0, la + i * (RP * LBK * 2));
 #pragma unroll
-      for (int i = 0; i < PB; ++i) dma_buf16(rsrcB, in ? b_voff[i] : DMA_OOB, soff, la + (BM * LBK + i * RP * LBK) * 2);
+      for (int i = 0; i < PB; ++i)
+        dma_buf16(rb, in & (bcol + r0 + RP * i < cend) ? v + 2u * (unsigned)((r0 + RP * i) * ldb) : DMA_OOB, 0, la + (BM * LBK + i * RP * LBK) * 2);
     } else {
+      const u16* const zp = (const u16*)g_lora_zero16;
       const int piece = (kt - p.nk) * 8 + lchunk, s = piece / r8, rc = piece - s * r8;
       const bool ok = s < nslots;
-      const int g = g_lo + s % ng, id = ok ? (one ? id0 : list[s / ng]) : 0;
+      const int si = s / ng, g = g_lo + s - si * ng, id = ok ? list[si] : 0;
+      const int c_lo = g * per, c_hi = c_lo + per;
 #pragma unroll
       for (int i = 0; i < PA; ++i) {
         const int r = r0 + RP * i;
-        const bool okr = ok && brow + r < p.M && (one || rowid[r] == id);
+        const bool okr = ok && brow + r < rend && rowid[r] == id;
         lora_dma16(okr ? p.t + (long long)(brow + r) * p.ldt + g * p.rank + rc * 8 : zp, la + i * (RP * LBK * 2));
       }
 #pragma unroll
       for (int i = 0; i < PB; ++i) {
         const int n = bcol + r0 + RP * i;
-        const bool okn = ok && n < p.N && n / per == g;
+        const bool okn = ok && n < cend && n >= c_lo && n < c_hi;
         lora_dma16(okn ? p.lb + ((long long)id * p.N + n) * p.rank + rc * 8 : zp, la + (BM * LBK + i * RP * LBK) * 2);
       }
     }
@@ -219,12 +345,15 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void lora_gemm_kernel(const LoraPa
 #pragma unroll
       for (int j = 0; j < NT; ++j) acc[i][j] = MFMA16(wf[j], af[i], acc[i][j], 0, 0, 0);
   };
-#pragma unroll
+  // one copy of the staging code for the prologue and one for the loop: a cold block first has to fetch its instructions (with the
+  // prologue unrolled the 18432 x 640 x 1920 product took 80 instead of 69 us)
+#pragma unroll 1
   for (int s = 0; s < NSTAGE; ++s) stage(s, s);
   hx8 af0[MT], wf0[NT], af1[MT], wf1[NT];
   LORA_WAIT(NSTAGE - 1);
   frags(af0, wf0, 0, 0);
   int slot = 0;
+#pragma unroll 1
   for (int kt = 0; kt < ntot; ++kt) {
     const int nslot = slot + 1 == NSTAGE ? 0 : slot + 1;
     frags(af1, wf1, slot, 1);
@@ -237,68 +366,131 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void lora_gemm_kernel(const LoraPa
   }
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // the trailing DMAs land before the LDS goes to another block
 #undef LORA_WAIT
+  // lanes l and l ^ 16 hold neighbouring 4-column pieces of a row: one exchange per pair of 16-column tiles leaves each with 8
+  // columns of one of them, 16-byte residual loads and stores
+  auto swz = [](float v) { return __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, v), 0x401F)); };
 #pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int m = brow + wr * TM + i * 16 + l15;
-    if (m >= p.M) continue;
+  for (int j = 0; j < NT; j += 2) {
+    const int n = bcol + wc * TN + (j + (lq & 1)) * 16 + (lq >> 1) * 8;
+    const bool okn = n < cend;
+    f32x4 b0 = {0.f, 0.f, 0.f, 0.f}, b1 = b0;
+    if (p.bias && okn) {
+      b0 = *(const f32x4*)(p.bias + n);
+      b1 = *(const f32x4*)(p.bias + n + 4);
+    }
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const int n = bcol + wc * TN + j * 16 + 4 * lq;
-      if (n >= p.N) continue;
-      float y[4];
+    for (int i = 0; i < MT; ++i) {
+      float y[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = acc[i][j][e] + (p.bias ? p.bias[n + e] : 0.f);
-      if (p.residual) {
-        const uint2 rr = *(const uint2*)(p.residual + (long long)m * p.ldr + n);
-        float r4[4];
-        unpack2(rr.x, r4[0], r4[1]);
-        unpack2(rr.y, r4[2], r4[3]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] += r4[e];
+      for (int e = 0; e < 4; ++e) {
+        const float keep = (lq & 1) ? acc[i][j + 1][e] : acc[i][j][e], give = (lq & 1) ? acc[i][j][e] : acc[i][j + 1][e];
+        const float got = swz(give);
+        y[e] = ((lq & 1) ? got : keep) + b0[e];
+        y[4 + e] = ((lq & 1) ? keep : got) + b1[e];
       }
-      *(uint2*)(p.out + (long long)m * p.ldo + n) = make_uint2(pack2h(y[0], y[1]), pack2h(y[2], y[3]));
+      const int m = brow + wr * TM + i * 16 + l15;
+      if (m < rend && okn) {
+        if (p.residual) {
+          float r[8];
+          unpack8(*(const uint4*)(p.residual + (long long)m * p.ldr + n), r);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] += r[e];
+        }
+        *(uint4*)(p.out + (long long)m * p.ldo + n) = pack8(y);
+      }
     }
   }
 }
 
 // ------------------------------------------------------------------------------------------------------------ host
 static bool lora_shape_ok(int m, int n, int k, int rank, int groups) {
-  return m > 0 && n > 0 && k > 0 && groups > 0 && n % groups == 0 && n % 8 == 0 && k % 8 == 0 && rank > 0 && rank % 8 == 0 && rank <= 256 && groups <= 64;
+  // a group's columns are whole 8-column pieces: the kernels' tiles start at its first
+  return m > 0 && n > 0 && k > 0 && groups > 0 && groups <= 64 && n % groups == 0 && (n / groups) % 8 == 0 && k % 8 == 0 && rank > 0 && rank % 8 == 0 && rank <= 256;
 }
+static bool lora_fused(int m, int rank, int groups) { return m <= 16 && m * groups * rank <= 64; }
 
 extern "C" int64_t sdmi_lora_gemm_ws_bytes(int m, int n, int k, int rank, int groups) {
-  return lora_shape_ok(m, n, k, rank, groups) ? (int64_t)m * groups * rank * 2 : 0;
+  return lora_shape_ok(m, n, k, rank, groups) && !lora_fused(m, rank, groups) ? (int64_t)m * groups * rank * 2 : 0;
 }
 
+template <int NT>
+static void lora_shrink_launch(const LoraParams& p, hipStream_t st) {
+  const int z = min(p.rpi >= 16 ? (p.rpi % 16 == 0 ? 1 : 2) : min((15 + p.rpi - 1) / p.rpi + 1, 16), p.adapters);  // requests that 16 rows can touch
+  const int tiles = (p.M + 15) / 16, ny = (p.ldt + 16 * NT - 1) / (16 * NT);
+  // enough row tiles for the chip: a wave sweeps all of K; else eight waves share it
+  if (tiles >= 1024) hipLaunchKernelGGL((lora_shrink_kernel<NT, 4, 1>), dim3((tiles + 3) / 4, ny, z), dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((lora_shrink_kernel<NT, 1, 8>), dim3(tiles, ny, z), dim3(512), 0, st, p);
+}
+
+template <int BM, int BN, int WM, int WN, int NSTAGE, bool MIXED>
+static int lora_launch2(LoraParams p, hipStream_t st) {
+  constexpr int bytes = NSTAGE * (BM + BN) * LBK * 2 + (MIXED ? (2 * BM + 1) * 4 : 0);
+  static_assert(bytes <= 160 * 1024, "LDS of a CU");
+  if constexpr (bytes > 64 * 1024) {
+    static std::atomic<unsigned long long> done{0};
+    int dev = 0;
+    (void)hipGetDevice(&dev);
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (!(done.load(std::memory_order_relaxed) & bit)) {
+      const hipError_t e = hipFuncSetAttribute((const void*)lora_gemm_kernel<BM, BN, WM, WN, NSTAGE, MIXED>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+      if (e != hipSuccess) {
+        sdmi_set_error("lora_gemm: %d bytes of LDS refused: %s", bytes, hipGetErrorString(e));
+        return SDMI_ELAUNCH;
+      }
+      done.fetch_or(bit, std::memory_order_relaxed);
+    }
+  }
+  long long tiles_m;
+  if (MIXED) {
+    p.tiles_n = (p.N + BN - 1) / BN;
+    tiles_m = (p.M + BM - 1) / BM;
+  } else {
+    p.tpg = (p.per + BN - 1) / BN;
+    p.tiles_n = p.groups * p.tpg;
+    tiles_m = (long long)((p.M + p.rpi - 1) / p.rpi) * ((p.rpi + BM - 1) / BM);
+  }
+  SDMI_REQUIRE(tiles_m * p.tiles_n < (1ll << 31), "lora_gemm: grid too large");
+  hipLaunchKernelGGL((lora_gemm_kernel<BM, BN, WM, WN, NSTAGE, MIXED>), dim3((unsigned)(tiles_m * p.tiles_n)), dim3(64 * WM * WN), bytes, st, p);
+  sdmi_note_kernel("lora_shrink_kernel + lora_gemm_kernel<%d, %d, %s>", BM, BN, MIXED ? "true" : "false");
+  return sdmi_check_launch("lora_gemm");
+}
 template <int BM, int BN, int WM, int WN, int NSTAGE>
 static int lora_launch(const LoraParams& p, hipStream_t st) {
-  constexpr int bytes = NSTAGE * (BM + BN) * LBK * 2 + (2 * BM + 1) * 4;
-  static_assert(bytes <= 64 * 1024, "LDS without an attribute");
-  const long long blocks = (long long)((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
-  SDMI_REQUIRE(blocks < (1ll << 31), "lora_gemm: grid too large");
-  hipLaunchKernelGGL((lora_gemm_kernel<BM, BN, WM, WN, NSTAGE>), dim3((unsigned)blocks), dim3(64 * WM * WN), bytes, st, p);
-  sdmi_note_kernel("lora_shrink_kernel + lora_gemm_kernel<%d, %d>", BM, BN);
-  return sdmi_check_launch("lora_gemm");
+  // a tile inside one request: when padding every request to whole tiles costs at most a quarter of the rows
+  const bool aligned = 4ll * ((p.rpi + BM - 1) / BM) * BM <= 5ll * p.rpi;
+  return aligned ? lora_launch2<BM, BN, WM, WN, NSTAGE, false>(p, st) : lora_launch2<BM, BN, WM, WN, NSTAGE, true>(p, st);
+}
+template <bool FUSE>
+static int lora_rows_launch(const LoraParams& p, hipStream_t st) {
+  const dim3 grid((p.N + 15) / 16), block(512);
+  if (p.M <= 16) hipLaunchKernelGGL((lora_rows_kernel<1, FUSE>), grid, block, 0, st, p);
+  else if constexpr (!FUSE) {
+    if (p.M <= 32) hipLaunchKernelGGL((lora_rows_kernel<2, FUSE>), grid, block, 0, st, p);
+    else hipLaunchKernelGGL((lora_rows_kernel<4, FUSE>), grid, block, 0, st, p);
+  }
+  sdmi_note_kernel(FUSE ? "lora_rows_kernel" : "lora_shrink_kernel + lora_rows_kernel");
+  return sdmi_check_launch("lora_gemm (few rows)");
 }
 
 extern "C" int sdmi_lora_gemm(const void* x, int ldx, const void* w, int ldw, void* out, int ldo, int m, int n, int k, const float* bias,
                               const void* residual, int ldr, const void* lora_a, const void* lora_b, const float* lora_scale, int adapters,
                               int rank, int groups, const int32_t* ids, int rows_per_id, uint32_t flags, void* ws, int64_t ws_bytes, void* stream) {
-  SDMI_REQUIRE(x && w && out && lora_a && lora_b && lora_scale && ids && ws, "lora_gemm: null pointer");
+  SDMI_REQUIRE(x && w && out && lora_a && lora_b && lora_scale && ids, "lora_gemm: null pointer");
   SDMI_REQUIRE(lora_shape_ok(m, n, k, rank, groups),
-               "lora_gemm: bad shape (m %d; n %d, k %d and the rank %d multiples of 8, rank up to 256; %d groups that divide n)", m, n, k, rank, groups);
+               "lora_gemm: bad shape (m %d; n %d, k %d and the rank %d multiples of 8, rank up to 256; %d groups of a multiple of 8 columns)", m, n, k, rank, groups);
   SDMI_REQUIRE(adapters > 0 && rows_per_id > 0, "lora_gemm: %d adapters, %d rows per id", adapters, rows_per_id);
   SDMI_REQUIRE((flags & ~(SDMI_F_BIAS | SDMI_F_RESIDUAL)) == 0, "lora_gemm: flags other than SDMI_F_BIAS and SDMI_F_RESIDUAL");
   SDMI_REQUIRE(!(flags & SDMI_F_BIAS) || bias, "lora_gemm: SDMI_F_BIAS without bias");
   SDMI_REQUIRE(!(flags & SDMI_F_RESIDUAL) || (residual && ldr % 8 == 0 && ldr >= n), "lora_gemm: SDMI_F_RESIDUAL: null residual or bad stride");
   SDMI_REQUIRE(ldx % 8 == 0 && ldw % 8 == 0 && ldo % 8 == 0 && ldx >= k && ldw >= k && ldo >= n, "lora_gemm: strides");
   SDMI_REQUIRE(ldx < (1 << 22) && ldw < (1 << 22), "lora_gemm: x / w row stride too large");  // 32-bit offsets inside a panel
-  SDMI_REQUIRE((((uintptr_t)x | (uintptr_t)w | (uintptr_t)out | (uintptr_t)lora_a | (uintptr_t)lora_b | (uintptr_t)ws |
-                 ((flags & SDMI_F_RESIDUAL) ? (uintptr_t)residual : 0)) & 15) == 0 &&
-                   (((uintptr_t)lora_scale | (uintptr_t)ids | ((flags & SDMI_F_BIAS) ? (uintptr_t)bias : 0)) & 3) == 0,
+  SDMI_REQUIRE((((uintptr_t)x | (uintptr_t)w | (uintptr_t)out | (uintptr_t)lora_a | (uintptr_t)lora_b |
+                 ((flags & SDMI_F_RESIDUAL) ? (uintptr_t)residual : 0) | ((flags & SDMI_F_BIAS) ? (uintptr_t)bias : 0)) & 15) == 0 &&
+                   (((uintptr_t)lora_scale | (uintptr_t)ids) & 3) == 0,
                "lora_gemm: pointer alignment");
-  SDMI_REQUIRE(ws_bytes >= sdmi_lora_gemm_ws_bytes(m, n, k, rank, groups), "lora_gemm: workspace of %lld bytes, %lld needed", (long long)ws_bytes,
-               (long long)sdmi_lora_gemm_ws_bytes(m, n, k, rank, groups));
+  const int64_t need = sdmi_lora_gemm_ws_bytes(m, n, k, rank, groups);
+  SDMI_REQUIRE(need == 0 || (ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= need), "lora_gemm: workspace of %lld bytes, %lld needed, 16-byte aligned",
+               (long long)(ws ? ws_bytes : 0), (long long)need);
   LoraParams p = {};
   p.x = (const u16*)x; p.w = (const u16*)w; p.out = (u16*)out; p.ldx = ldx; p.ldw = ldw; p.ldo = ldo;
   p.M = m; p.N = n; p.K = k; p.nk = (k + LBK - 1) / LBK;
@@ -307,11 +499,30 @@ extern "C" int sdmi_lora_gemm(const void* x, int ldx, const void* w, int ldw, vo
   p.ldr = ldr;
   p.la = (const u16*)lora_a; p.lb = (const u16*)lora_b; p.scale = lora_scale; p.ids = ids;
   p.adapters = adapters; p.rank = rank; p.groups = groups; p.rpi = rows_per_id;
-  p.t = (u16*)ws; p.ldt = groups * rank;
+  p.t = (u16*)ws; p.ldt = groups * rank; p.per = n / groups;
   hipStream_t st = (hipStream_t)stream;
-  hipLaunchKernelGGL(lora_shrink_kernel, dim3((m + 15) / 16, (groups * rank + 16 * SHR_NT - 1) / (16 * SHR_NT)), dim3(256), 0, st, p);
-  int rc = sdmi_check_launch("lora_gemm (low-rank factor)");
+  if (need == 0) return lora_rows_launch<true>(p, st);
+  if (p.ldt <= 16) lora_shrink_launch<1>(p, st);
+  else if (p.ldt <= 32) lora_shrink_launch<2>(p, st);
+  else lora_shrink_launch<4>(p, st);
+  const int rc = sdmi_check_launch("lora_gemm (low-rank factor)");
   if (rc != SDMI_OK) return rc;
+  if (m <= 64) return lora_rows_launch<false>(p, st);
+#ifdef LORA_VARIANT
+#if LORA_VARIANT == 1
+  return lora_launch<128, 128, 2, 2, 2>(p, st);
+#elif LORA_VARIANT == 2
+  return lora_launch<128, 64, 2, 2, 2>(p, st);
+#elif LORA_VARIANT == 3
+  return lora_launch<64, 64, 2, 2, 2>(p, st);
+#elif LORA_VARIANT == 4
+  return lora_launch<64, 64, 2, 2, 3>(p, st);
+#elif LORA_VARIANT == 5
+  return lora_launch<64, 128, 2, 2, 2>(p, st);
+#elif LORA_VARIANT == 6
+  return lora_launch<64, 128, 2, 2, 3>(p, st);
+#endif
+#endif
   if ((long long)((m + 127) / 128) * ((n + 63) / 64) >= 512) return lora_launch<128, 64, 2, 2, 2>(p, st);
   return lora_launch<64, 64, 2, 2, 3>(p, st);
 }

@@ -8,7 +8,7 @@ P = 0x10000000     # an aligned address that is never followed
 
 ATT = dict(q=P, ldq=128, sq=128, k=P, ldk=128, sk=1280, v=P, ldv=128, sv=1280, o=P, ldo=128, so=128, batch=2, contexts=2, heads=2, kv_heads=2, dim=64, nq=1, nkv=10,
            index=None, lens=None, qr=None, sqr=0, kr=None, skr=0, scale=0.125, ws=None, ws_bytes=0, stream=None)
-LORA = dict(x=P, ldx=64, w=P, ldw=64, out=P, ldo=64, m=4, n=64, k=64, bias=None, residual=None, ldr=0, a=P, b=P, scale=P, adapters=2, rank=8, groups=1, ids=P, rows=1,
+LORA = dict(x=P, ldx=64, w=P, ldw=64, out=P, ldo=64, m=100, n=64, k=64, bias=None, residual=None, ldr=0, a=P, b=P, scale=P, adapters=2, rank=8, groups=1, ids=P, rows=1,
             flags=0, ws=P, ws_bytes=1 << 20, stream=None)
 
 
@@ -26,7 +26,7 @@ def test_attention_refuses(change, word):
 
 
 @pytest.mark.parametrize("change,word", [
-    (dict(x=None), "null"), (dict(ids=None), "null"), (dict(ws=None), "null"), (dict(b=None), "null"), (dict(m=0), "shape"), (dict(n=60), "shape"), (dict(k=60), "shape"),
+    (dict(x=None), "null"), (dict(ids=None), "null"), (dict(ws=None), "workspace"), (dict(ws=P + 8), "workspace"), (dict(n=24, groups=2), "shape"), (dict(flags=1, bias=P + 4), "alignment"), (dict(b=None), "null"), (dict(m=0), "shape"), (dict(n=60), "shape"), (dict(k=60), "shape"),
     (dict(rank=12), "shape"), (dict(rank=0), "shape"), (dict(rank=264), "shape"), (dict(groups=0), "shape"), (dict(groups=3), "shape"), (dict(adapters=0), "adapters"),
     (dict(rows=0), "rows per id"), (dict(flags=8), "flags"), (dict(flags=1), "bias"), (dict(flags=4), "residual"), (dict(flags=4, residual=P, ldr=32), "residual"),
     (dict(ldx=32), "strides"), (dict(ldw=68), "strides"), (dict(ldo=60), "strides"), (dict(ldx=1 << 22), "too large"), (dict(x=P + 8), "alignment"),
@@ -44,3 +44,4 @@ def test_workspace_sizes():
     assert lib.sdmi_cross_attention_ws_bytes(1, 2, 2, 60, 1, 5000) == 0             # refused shapes need nothing
     assert lib.sdmi_lora_gemm_ws_bytes(100, 96, 64, 16, 3) >= 100 * 48 * 2
     assert lib.sdmi_lora_gemm_ws_bytes(100, 96, 64, 12, 3) == 0
+    assert lib.sdmi_lora_gemm_ws_bytes(1, 96, 64, 16, 1) == 0                       # one launch: nothing to hand over
