@@ -312,7 +312,7 @@ int64_t sdmi_cross_attention_ws_bytes(int batch, int heads, int kv_heads, int di
 int sdmi_lora_gemm(const void* x, int ldx, const void* w, int ldw, void* out, int ldo, int m, int n, int k, const float* bias,
                    const void* residual, int ldr, const void* lora_a, const void* lora_b, const float* lora_scale, int adapters,
                    int rank, int groups, const int32_t* ids, int rows_per_id, uint32_t flags, void* ws, int64_t ws_bytes, void* stream);
-int64_t sdmi_lora_gemm_ws_bytes(int m, int n, int k, int rank, int groups);
+int64_t sdmi_lora_gemm_ws_bytes(int m, int n, int k, int rank, int groups, int rows_per_id);
 
 /* ---- fused flash attention, ONE head of dim 512: the VAE mid block's attention (layers/SpatialTransformer.py:132-161,
  *      xformers.ops.memory_efficient_attention on (B, HW, 512)) without an N x N score buffer.  q/k/v/o are h16 token-major

@@ -78,7 +78,7 @@ PROTOTYPES = {
     "sdmi_cross_attention": (_i, [_vp, _i, _i64, _vp, _i, _i64, _vp, _i, _i64, _vp, _i, _i64, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _i64, _vp, _i64, _f, _vp, _i64, _vp]),
     "sdmi_cross_attention_ws_bytes": (_i64, [_i, _i, _i, _i, _i, _i]),
     "sdmi_lora_gemm": (_i, [_vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _vp, _i, _u32, _vp, _i64, _vp]),
-    "sdmi_lora_gemm_ws_bytes": (_i64, [_i, _i, _i, _i, _i]),
+    "sdmi_lora_gemm_ws_bytes": (_i64, [_i, _i, _i, _i, _i, _i]),
     "sdmi_inpaint_prepare": (_i, [_vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _i64, _vp]),
     "sdmi_posterior_sample": (_i, [_vp, _vp, _f, _vp, _i64, _i, _i, _vp]),
     "sdmi_attention_d512": (_i, [_vp, _i, _i64, _vp, _i, _i64, _vp, _i, _i64, _vp, _i, _i64, _i, _i, _f, _vp]),

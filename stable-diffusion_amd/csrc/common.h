@@ -117,6 +117,9 @@ __device__ __forceinline__ float wave_max(float v) {
   for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
   return v;
 }
+// A wave-uniform word that no kernel of the launch writes, through the scalar cache: s_load, counted by lgkmcnt (a vector load would
+// make the compiler wait for every LDS-DMA issued after it, and blocks on neighbouring CUs share the cached line)
+__device__ __forceinline__ int scalar_i32(const int* p) { return *(const __attribute__((address_space(4))) int*)(unsigned long long)p; }
 // Blocks b and b+8 share an XCD (round-robin dispatch): give each XCD a contiguous run of tiles so
 // neighbouring tiles (which share operand panels) hit the same L2.  Bijective for any nb.
 __device__ __forceinline__ int xcd_remap(int bid, int nb) {

@@ -39,76 +39,75 @@ __device__ __forceinline__ int lora_id(const LoraParams& p, int row) {
 }
 
 // ------------------------------------------------------------------------------------------------------------ t = scale x a^T
-// Block: RW x 16 rows by 16 NT columns of t, K cut over KW waves (32 of it a step), joined in wave order through the LDS; a wave
-// works for ONE adapter: blockIdx.z is the z-th distinct one among its 16 rows, every row keeps its own adapter's result, waves
-// beyond the last one have nothing to do.  Operands come straight from memory in fragment layout (8 consecutive k of one row
-// per lane); UN steps' loads are issued before the first product waits for one.
-template <int NT, int RW, int KW>
-__global__ __launch_bounds__(64 * RW * KW, 1) void lora_shrink_kernel(const LoraParams p) {
-  constexpr int UN = NT == 4 ? 5 : 10;
-  __shared__ float red[RW][KW > 1 ? KW - 1 : 1][KW > 1 ? NT * 4 : 1][64];
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, rw = wv / KW, kw = wv % KW, l15 = lane & 15, lq = lane >> 4;
-  const int row = (blockIdx.x * RW + rw) * 16 + l15, rowc = min(row, p.M - 1), n0 = blockIdx.y * (NT * 16), NR = p.ldt;
-  const int mine = row < p.M ? lora_id(p, row) : -1;
-  unsigned long long todo = __builtin_amdgcn_ballot_w64(mine >= 0);  // the same in every wave of a row tile
+// Block: 16 MR rows by 16 NT columns of t, K cut over KW waves (32 of it a step), joined in wave order through the LDS.  A block
+// works for ONE adapter: blockIdx.z is the z-th distinct one among its rows; every row keeps its own adapter's result, blocks
+// beyond the last one leave.  Operands come straight from memory in fragment layout (8 consecutive k of one row per lane); UN
+// steps' loads are issued before the first product waits for one.
+template <int MR, int NT, int KW>
+__global__ __launch_bounds__(64 * KW, 1) void lora_shrink_kernel(const LoraParams p) {
+  constexpr int UN = MR + NT <= 3 ? 5 : MR + NT <= 6 ? 4 : 3;
+  __shared__ float red[KW][MR * NT * 4][64];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, l15 = lane & 15, lq = lane >> 4;
+  const int row0 = blockIdx.x * (16 * MR), n0 = blockIdx.y * (NT * 16), NR = p.ldt;
+  const int mine = lane < 16 * MR && row0 + lane < p.M ? lora_id(p, row0 + lane) : -1;
+  unsigned long long todo = __builtin_amdgcn_ballot_w64(mine >= 0);  // the same in every wave
   int id = 0;
   for (int z = blockIdx.z; todo; --z) {
     id = __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo));
     if (z == 0) break;
     todo &= ~__builtin_amdgcn_ballot_w64(mine == id);
   }
-  f32x4 acc[NT];
+  if (!todo) return;
+  f32x4 acc[MR][NT];
 #pragma unroll
-  for (int j = 0; j < NT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  if (todo) {
-    const u16* const zp = (const u16*)g_lora_zero16;
-    const u16* xr = p.x + (long long)rowc * p.ldx + 8 * lq;
-    const u16* ar[NT];
+  for (int i = 0; i < MR; ++i)
 #pragma unroll
-    for (int j = 0; j < NT; ++j) ar[j] = p.la + ((long long)id * NR + min(n0 + 16 * j + l15, NR - 1)) * p.K;
-    for (int kb = kw * 32; kb < p.K; kb += 32 * KW * UN) {
-      hx8 xf[UN], af[UN][NT];
+    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const u16* const zp = (const u16*)g_lora_zero16;
+  const u16 *xr[MR], *ar[NT];
 #pragma unroll
-      for (int u = 0; u < UN; ++u) {
-        const int k = kb + 32 * KW * u;
-        const bool in = k + 8 * lq < p.K;  // K is a multiple of 8; past it x reads as zeros, and a as its first columns
-        xf[u] = *(const hx8*)(in ? xr + k : zp);
+  for (int i = 0; i < MR; ++i) xr[i] = p.x + (long long)min(row0 + 16 * i + l15, p.M - 1) * p.ldx + 8 * lq;
 #pragma unroll
-        for (int j = 0; j < NT; ++j) af[u][j] = *(const hx8*)(ar[j] + (in ? k + 8 * lq : 0));
-      }
-      __builtin_amdgcn_sched_barrier(0);
+  for (int j = 0; j < NT; ++j) ar[j] = p.la + ((long long)id * NR + min(n0 + 16 * j + l15, NR - 1)) * p.K;
+  for (int kb = wv * 32; kb < p.K; kb += 32 * KW * UN) {
+    hx8 xf[UN][MR], af[UN][NT];
 #pragma unroll
-      for (int u = 0; u < UN; ++u)
+    for (int u = 0; u < UN; ++u) {
+      const int k = kb + 32 * KW * u;
+      const bool in = k + 8 * lq < p.K;  // K is a multiple of 8; past it x reads as zeros, and a as its first columns
 #pragma unroll
-        for (int j = 0; j < NT; ++j) acc[j] = MFMA16(af[u][j], xf[u], acc[j], 0, 0, 0);
+      for (int i = 0; i < MR; ++i) xf[u][i] = *(const hx8*)(in ? xr[i] + k : zp);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) af[u][j] = *(const hx8*)(ar[j] + (in ? k + 8 * lq : 0));
     }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < UN; ++u)
+#pragma unroll
+      for (int i = 0; i < MR; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = MFMA16(af[u][j], xf[u][i], acc[i][j], 0, 0, 0);
   }
-  if constexpr (KW > 1) {
-    if (kw > 0) {
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
+  for (int i = 0; i < MR; ++i)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) red[rw][kw - 1][4 * j + i][lane] = acc[j][i];
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) red[wv][(i * NT + j) * 4 + e][lane] = acc[i][j][e];  // row 16 i + l15, column 16 j + 4 lq + e
+  __syncthreads();
+  const float sc = p.scale[id];
+  for (int q = wv; q < MR * NT; q += KW) {
+    const int i = q / NT, j = q - i * NT, n = n0 + 16 * j + 4 * lq;
+    float y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      y[e] = 0.f;
+#pragma unroll
+      for (int w = 0; w < KW; ++w) y[e] += red[w][q * 4 + e][lane];
+      y[e] *= sc;
     }
-    __syncthreads();
-  }
-  if (kw == 0 && todo && mine == id) {
-    const float sc = p.scale[id];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      float y[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        y[i] = acc[j][i];
-        if constexpr (KW > 1) {
-#pragma unroll
-          for (int w = 0; w < KW - 1; ++w) y[i] += red[rw][w][4 * j + i][lane];
-        }
-        y[i] *= sc;
-      }
-      const int n = n0 + 16 * j + 4 * lq;
-      if (n < NR) *(uint2*)(p.t + (long long)row * p.ldt + n) = make_uint2(pack2h(y[0], y[1]), pack2h(y[2], y[3]));
-    }
+    const int his = __shfl(mine, 16 * i + l15);
+    if (his == id && n < NR) *(uint2*)(p.t + (long long)(row0 + 16 * i + l15) * p.ldt + n) = make_uint2(pack2h(y[0], y[1]), pack2h(y[2], y[3]));
   }
 }
 
@@ -216,13 +215,18 @@ __device__ __forceinline__ void lora_dma16(const void* src, unsigned lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory", "m0");
 }
 
+// FR > 0 (ranks up to FR = 16 or 32, MIXED = false): the block computes t of its rows itself.  FR rows of the adapter's a ride along
+// with each K-tile and take one more product per 16 rows and step (the two waves that share rows take alternate steps); behind
+// the loop t is joined, scaled, rounded and multiplied with b, whose fragments were fetched before it.  One launch and one
+// reading of x less, for FR / (BM + BN) more bytes staged.
 // MIXED = false: a tile lies inside one request and one group (the grid is laid out by them), so its adapter is one scalar and the
 // adapter's K-tiles are strided like the others.  MIXED = true (requests of fewer rows than a tile): tiles of consecutive rows; the
 // first wave lists the distinct adapters of the block's rows, and the adapters' K-tiles are gathered piece by piece.
-template <int BM, int BN, int WM, int WN, int NSTAGE, bool MIXED>
-__global__ __launch_bounds__(64 * WM * WN, (WM * WN == 4 && NSTAGE * (BM + BN) * LBK * 2 <= 80 * 1024) || WM * WN == 8 ? 2 : 1) void lora_gemm_kernel(const LoraParams p) {
+template <int BM, int BN, int WM, int WN, int NSTAGE, bool MIXED, int FR>
+__global__ __launch_bounds__(64 * WM * WN, (WM * WN == 4 && NSTAGE * (BM + BN + FR) * LBK * 2 <= 54 * 1024) ? 3 : 2) void lora_gemm_kernel(const LoraParams p) {
   constexpr int NTH = 64 * WM * WN, RP = NTH / 8, TM = BM / WM, TN = BN / WN, MT = TM / 16, NT = TN / 16, PA = BM / RP, PB = BN / RP;
-  constexpr int STAGE = (BM + BN) * LBK;
+  constexpr int STAGE = (BM + BN + FR) * LBK;
+  static_assert(FR == 0 || (!MIXED && WN == 2 && NSTAGE == 2 && RP == 32), "t in the block: two waves to a row, all DMA landed at every wait");
   static_assert(BM % RP == 0 && BN % RP == 0 && RP % 16 == 0 && NT % 2 == 0, "tile / wave grid mismatch");
   extern __shared__ __attribute__((aligned(16))) u16 smem[];  // the ring; MIXED: then rowid[BM], the list of adapters [BM] and its length
   int* const rowid = (int*)(smem + NSTAGE * STAGE);
@@ -267,7 +271,7 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN == 4 && NSTAGE * (BM + BN) *
     g_lo = __builtin_amdgcn_readfirstlane(nt / p.tpg);
     bcol = g_lo * per + (nt - g_lo * p.tpg) * BN;
     cend = min(bcol + BN, (g_lo + 1) * per);
-    id0 = __builtin_amdgcn_readfirstlane(p.ids[req]);
+    id0 = scalar_i32(p.ids + req);
     id0 = id0 < p.adapters ? id0 : -1;
     nids = id0 >= 0 ? 1 : 0;
   }
@@ -280,14 +284,15 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN == 4 && NSTAGE * (BM + BN) *
   const u16* const lb = p.lb + ((long long)(id0 < 0 ? 0 : id0) * p.N + bcol) * p.rank;
   const unsigned lds0 = lds_addr_of(smem) + wv * 1024;
   const int nslots = nids * ng, r8 = p.rank >> 3, rk = nids ? p.rank : 0;
-  const int ntot = p.nk + (nslots * r8 + 7) / 8;
+  const int ntot = p.nk + (FR ? 0 : (nslots * r8 + 7) / 8);
+  const u16* const fa = FR ? p.la + ((long long)(id0 < 0 ? 0 : id0) * p.ldt + g_lo * p.rank) * p.K : nullptr;  // the adapter's rows
 
   // K-tile KT into ring slot SLOT; always PA + PB DMA instructions per wave (past the last tile: zeros), so that the counted waits
   // below hold
   auto stage = [&](int kt, int slot) {
     const unsigned la = lds0 + slot * (STAGE * 2);
     if (!MIXED || kt < p.nk || kt >= ntot) {
-      const bool ext = !MIXED && kt >= p.nk;
+      const bool ext = !MIXED && FR == 0 && kt >= p.nk;
       const int k0 = (ext ? kt - p.nk : kt) * LBK, klim = ext ? rk : p.K;
       const int lda = ext ? p.ldt : p.ldx, ldb = ext ? p.rank : p.ldw;
       const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc((void*)(ext ? ta : xa), 0, DMA_OOB, 0x00020000);
@@ -300,6 +305,11 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN == 4 && NSTAGE * (BM + BN) *
 #pragma unroll
       for (int i = 0; i < PB; ++i)
         dma_buf16(rb, in & (bcol + r0 + RP * i < cend) ? v + 2u * (unsigned)((r0 + RP * i) * ldb) : DMA_OOB, 0, la + (BM * LBK + i * RP * LBK) * 2);
+      if constexpr (FR > 0) {
+        if (wv < FR / 8)  // a wave moves 8 rows; the others issue one instruction less, and every wait is for all of them
+          dma_buf16(__builtin_amdgcn_make_buffer_rsrc((void*)fa, 0, DMA_OOB, 0x00020000), in & (r0 < rk) ? v + 2u * (unsigned)(r0 * p.K) : DMA_OOB, 0,
+                    la + (BM + BN) * LBK * 2);
+      }
     } else {
       const u16* const zp = (const u16*)g_lora_zero16;
       const int piece = (kt - p.nk) * 8 + lchunk, s = piece / r8, rc = piece - s * r8;
@@ -331,6 +341,32 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN == 4 && NSTAGE * (BM + BN) *
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  constexpr int FT = FR / 16;
+  f32x4 tacc[FT ? FT : 1][MT];
+  hx8 bf[FT ? NT : 1];
+  if constexpr (FR > 0) {
+#pragma unroll
+    for (int f = 0; f < FT; ++f)
+#pragma unroll
+      for (int i = 0; i < MT; ++i) tacc[f][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {  // b of this wave's columns, ranks 8 lq .. 8 lq + 7
+      const int c = wc * TN + j * 16 + l15;
+      bf[j] = *(const hx8*)(8 * lq < rk && bcol + c < cend ? lb + (long long)c * p.rank + 8 * lq : (const u16*)g_lora_zero16);
+    }
+  }
+  // t: this wave's share of a K-tile (step kk = wc), from the x fragments it has at hand
+  auto tmfma = [&](const hx8 (&af)[MT], int slot, int kk) {
+    if constexpr (FR > 0) {
+      const u16* cF = smem + slot * STAGE + (BM + BN) * LBK;
+#pragma unroll
+      for (int f = 0; f < FT; ++f) {
+        const hx8 ff = *(const hx8*)&cF[lora_off(16 * f + l15, lq + 4 * kk)];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) tacc[f][i] = MFMA16(ff, af[i], tacc[f][i], 0, 0, 0);
+      }
+    }
+  };
   auto frags = [&](hx8 (&af)[MT], hx8 (&wf)[NT], int slot, int kk) {
     const u16* cA = smem + slot * STAGE;
     const u16* cB = cA + BM * LBK;
@@ -352,20 +388,61 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN == 4 && NSTAGE * (BM + BN) *
   hx8 af0[MT], wf0[NT], af1[MT], wf1[NT];
   LORA_WAIT(NSTAGE - 1);
   frags(af0, wf0, 0, 0);
+  // the fragments a K-tile starts with are read at the end of the one before, under its last products.  The empty statement keeps
+  // the compiler from merging that read with this one into a read at the head of the loop, where its latency shows
+#define LORA_PIN() asm volatile("" ::: "memory")
+  LORA_PIN();
   int slot = 0;
 #pragma unroll 1
   for (int kt = 0; kt < ntot; ++kt) {
     const int nslot = slot + 1 == NSTAGE ? 0 : slot + 1;
     frags(af1, wf1, slot, 1);
+    if (FR > 0) {
+      if (wc == 0) tmfma(af0, slot, 0);
+      else tmfma(af1, slot, 1);
+    }
     mfma(af0, wf0);
     LORA_WAIT(NSTAGE - 2);
     stage(kt + NSTAGE, slot);
     frags(af0, wf0, nslot, 0);
+    LORA_PIN();
     mfma(af1, wf1);
     slot = nslot;
   }
+#undef LORA_PIN
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // the trailing DMAs land before the LDS goes to another block
 #undef LORA_WAIT
+  if constexpr (FR > 0) {
+    if (nids) {  // join t of the two waves that share these rows, in the ring's memory: [wc][f][row][rank], 20 floats to a row
+      float* const tp = (float*)smem;
+      static_assert(2 * FT * BM * 20 * 4 <= NSTAGE * STAGE * 2, "t in the ring");
+      __syncthreads();
+#pragma unroll
+      for (int f = 0; f < FT; ++f)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) *(f32x4*)&tp[((wc * FT + f) * BM + wr * TM + i * 16 + l15) * 20 + 4 * lq] = tacc[f][i];
+      __syncthreads();
+      const float sc = p.scale[id0];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        hx8 tf;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {  // ranks 8 lq + 4 h ..
+          const int f = FT == 2 ? lq >> 1 : 0, rr = 8 * (lq & 1) + 4 * h;
+          const float* q = &tp[(f * BM + wr * TM + i * 16 + l15) * 20 + rr];
+          const f32x4 t0 = *(const f32x4*)q, t1 = *(const f32x4*)(q + FT * BM * 20);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) tf[4 * h + e] = f2h16((t0[e] + t1[e]) * sc);
+        }
+        if (FT == 1 && lq >= 2) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) tf[e] = (h16)0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = MFMA16(bf[j], tf, acc[i][j], 0, 0, 0);
+      }
+    }
+  }
   // lanes l and l ^ 16 hold neighbouring 4-column pieces of a row: one exchange per pair of 16-column tiles leaves each with 8
   // columns of one of them, 16-byte residual loads and stores
   auto swz = [](float v) { return __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, v), 0x401F)); };
@@ -407,39 +484,46 @@ static bool lora_shape_ok(int m, int n, int k, int rank, int groups) {
   // a group's columns are whole 8-column pieces: the kernels' tiles start at its first
   return m > 0 && n > 0 && k > 0 && groups > 0 && groups <= 64 && n % groups == 0 && (n / groups) % 8 == 0 && k % 8 == 0 && rank > 0 && rank % 8 == 0 && rank <= 256;
 }
-static bool lora_fused(int m, int rank, int groups) { return m <= 16 && m * groups * rank <= 64; }
+// which kernels take a problem; the workspace holds t where a launch hands it to the next
+enum { LORA_ROWS_FUSED, LORA_ROWS, LORA_TILES_FUSED, LORA_TILES, LORA_MIXED };
+struct LoraPlan { int kind, bm; };
+static LoraPlan lora_plan(int m, int n, int rank, int groups, int rpi) {
+  if (m <= 16 && m * groups * rank <= 64) return {LORA_ROWS_FUSED, 0};
+  if (m <= 64) return {LORA_ROWS, 0};
+  LoraPlan pl;
+  pl.bm = (long long)((m + 127) / 128) * ((n + 63) / 64) >= 512 ? 128 : 64;
+  // a tile inside one request: when padding every request to whole tiles costs at most a quarter of the rows
+  const bool aligned = 4ll * ((rpi + pl.bm - 1) / pl.bm) * pl.bm <= 5ll * rpi;
+  pl.kind = !aligned ? LORA_MIXED : rank <= 32 ? LORA_TILES_FUSED : LORA_TILES;
+  return pl;
+}
+static bool lora_needs_t(int kind) { return kind != LORA_ROWS_FUSED && kind != LORA_TILES_FUSED; }
 
-extern "C" int64_t sdmi_lora_gemm_ws_bytes(int m, int n, int k, int rank, int groups) {
-  return lora_shape_ok(m, n, k, rank, groups) && !lora_fused(m, rank, groups) ? (int64_t)m * groups * rank * 2 : 0;
+extern "C" int64_t sdmi_lora_gemm_ws_bytes(int m, int n, int k, int rank, int groups, int rows_per_id) {
+  if (!lora_shape_ok(m, n, k, rank, groups) || rows_per_id <= 0 || !lora_needs_t(lora_plan(m, n, rank, groups, rows_per_id).kind)) return 0;
+  return (int64_t)m * groups * rank * 2;
 }
 
-template <int NT>
-static void lora_shrink_launch(const LoraParams& p, hipStream_t st) {
-  const int z = min(p.rpi >= 16 ? (p.rpi % 16 == 0 ? 1 : 2) : min((15 + p.rpi - 1) / p.rpi + 1, 16), p.adapters);  // requests that 16 rows can touch
-  const int tiles = (p.M + 15) / 16, ny = (p.ldt + 16 * NT - 1) / (16 * NT);
-  // enough row tiles for the chip: a wave sweeps all of K; else eight waves share it
-  if (tiles >= 1024) hipLaunchKernelGGL((lora_shrink_kernel<NT, 4, 1>), dim3((tiles + 3) / 4, ny, z), dim3(256), 0, st, p);
-  else hipLaunchKernelGGL((lora_shrink_kernel<NT, 1, 8>), dim3(tiles, ny, z), dim3(512), 0, st, p);
+template <int MR, int NT, int KW>
+static void lora_shrink_launch2(const LoraParams& p, hipStream_t st) {
+  constexpr int TR = 16 * MR;
+  const int touched = p.rpi >= TR ? (p.rpi % TR == 0 ? 1 : 2) : min((TR - 1 + p.rpi - 1) / p.rpi + 1, TR);  // requests that TR rows can touch
+  hipLaunchKernelGGL((lora_shrink_kernel<MR, NT, KW>), dim3((p.M + TR - 1) / TR, (p.ldt + 16 * NT - 1) / (16 * NT), min(touched, p.adapters)), dim3(64 * KW), 0, st, p);
+}
+static int lora_shrink_launch(const LoraParams& p, hipStream_t st) {
+  // 64-row blocks share each reading of a; with few rows smaller ones spread over more of the chip
+  const bool big = (long long)((p.M + 63) / 64) * ((p.ldt + 63) / 64) * (p.rpi >= 64 ? 1 : min(p.adapters, 4)) >= 128;
+  if (big && p.ldt > 32) lora_shrink_launch2<4, 4, 4>(p, st);
+  else if (big) lora_shrink_launch2<4, 2, 8>(p, st);
+  else if (p.ldt > 16) lora_shrink_launch2<1, 2, 8>(p, st);
+  else lora_shrink_launch2<1, 1, 8>(p, st);
+  return sdmi_check_launch("lora_gemm (low-rank factor)");
 }
 
-template <int BM, int BN, int WM, int WN, int NSTAGE, bool MIXED>
-static int lora_launch2(LoraParams p, hipStream_t st) {
-  constexpr int bytes = NSTAGE * (BM + BN) * LBK * 2 + (MIXED ? (2 * BM + 1) * 4 : 0);
-  static_assert(bytes <= 160 * 1024, "LDS of a CU");
-  if constexpr (bytes > 64 * 1024) {
-    static std::atomic<unsigned long long> done{0};
-    int dev = 0;
-    (void)hipGetDevice(&dev);
-    const unsigned long long bit = 1ull << (dev & 63);
-    if (!(done.load(std::memory_order_relaxed) & bit)) {
-      const hipError_t e = hipFuncSetAttribute((const void*)lora_gemm_kernel<BM, BN, WM, WN, NSTAGE, MIXED>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-      if (e != hipSuccess) {
-        sdmi_set_error("lora_gemm: %d bytes of LDS refused: %s", bytes, hipGetErrorString(e));
-        return SDMI_ELAUNCH;
-      }
-      done.fetch_or(bit, std::memory_order_relaxed);
-    }
-  }
+template <int BM, int BN, int WM, int WN, int NSTAGE, bool MIXED, int FR>
+static int lora_launch(LoraParams p, hipStream_t st) {
+  constexpr int bytes = NSTAGE * (BM + BN + FR) * LBK * 2 + (MIXED ? (2 * BM + 1) * 4 : 0);
+  static_assert(bytes <= 64 * 1024, "LDS without an attribute");
   long long tiles_m;
   if (MIXED) {
     p.tiles_n = (p.N + BN - 1) / BN;
@@ -450,15 +534,15 @@ static int lora_launch2(LoraParams p, hipStream_t st) {
     tiles_m = (long long)((p.M + p.rpi - 1) / p.rpi) * ((p.rpi + BM - 1) / BM);
   }
   SDMI_REQUIRE(tiles_m * p.tiles_n < (1ll << 31), "lora_gemm: grid too large");
-  hipLaunchKernelGGL((lora_gemm_kernel<BM, BN, WM, WN, NSTAGE, MIXED>), dim3((unsigned)(tiles_m * p.tiles_n)), dim3(64 * WM * WN), bytes, st, p);
-  sdmi_note_kernel("lora_shrink_kernel + lora_gemm_kernel<%d, %d, %s>", BM, BN, MIXED ? "true" : "false");
+  hipLaunchKernelGGL((lora_gemm_kernel<BM, BN, WM, WN, NSTAGE, MIXED, FR>), dim3((unsigned)(tiles_m * p.tiles_n)), dim3(64 * WM * WN), bytes, st, p);
+  sdmi_note_kernel("%slora_gemm_kernel<%d, %d, %s, %d>", FR ? "" : "lora_shrink_kernel + ", BM, BN, MIXED ? "true" : "false", FR);
   return sdmi_check_launch("lora_gemm");
 }
-template <int BM, int BN, int WM, int WN, int NSTAGE>
-static int lora_launch(const LoraParams& p, hipStream_t st) {
-  // a tile inside one request: when padding every request to whole tiles costs at most a quarter of the rows
-  const bool aligned = 4ll * ((p.rpi + BM - 1) / BM) * BM <= 5ll * p.rpi;
-  return aligned ? lora_launch2<BM, BN, WM, WN, NSTAGE, false>(p, st) : lora_launch2<BM, BN, WM, WN, NSTAGE, true>(p, st);
+template <int BM, int NSTAGE>
+static int lora_tiles_launch(const LoraParams& p, int kind, hipStream_t st) {
+  if (kind == LORA_MIXED) return lora_launch<BM, 64, 2, 2, NSTAGE, true, 0>(p, st);
+  if (kind == LORA_TILES) return lora_launch<BM, 64, 2, 2, NSTAGE, false, 0>(p, st);
+  return p.rank <= 16 ? lora_launch<BM, 64, 2, 2, 2, false, 16>(p, st) : lora_launch<BM, 64, 2, 2, 2, false, 32>(p, st);
 }
 template <bool FUSE>
 static int lora_rows_launch(const LoraParams& p, hipStream_t st) {
@@ -488,7 +572,7 @@ extern "C" int sdmi_lora_gemm(const void* x, int ldx, const void* w, int ldw, vo
                  ((flags & SDMI_F_RESIDUAL) ? (uintptr_t)residual : 0) | ((flags & SDMI_F_BIAS) ? (uintptr_t)bias : 0)) & 15) == 0 &&
                    (((uintptr_t)lora_scale | (uintptr_t)ids) & 3) == 0,
                "lora_gemm: pointer alignment");
-  const int64_t need = sdmi_lora_gemm_ws_bytes(m, n, k, rank, groups);
+  const int64_t need = sdmi_lora_gemm_ws_bytes(m, n, k, rank, groups, rows_per_id);
   SDMI_REQUIRE(need == 0 || (ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= need), "lora_gemm: workspace of %lld bytes, %lld needed, 16-byte aligned",
                (long long)(ws ? ws_bytes : 0), (long long)need);
   LoraParams p = {};
@@ -501,28 +585,12 @@ extern "C" int sdmi_lora_gemm(const void* x, int ldx, const void* w, int ldw, vo
   p.adapters = adapters; p.rank = rank; p.groups = groups; p.rpi = rows_per_id;
   p.t = (u16*)ws; p.ldt = groups * rank; p.per = n / groups;
   hipStream_t st = (hipStream_t)stream;
-  if (need == 0) return lora_rows_launch<true>(p, st);
-  if (p.ldt <= 16) lora_shrink_launch<1>(p, st);
-  else if (p.ldt <= 32) lora_shrink_launch<2>(p, st);
-  else lora_shrink_launch<4>(p, st);
-  const int rc = sdmi_check_launch("lora_gemm (low-rank factor)");
-  if (rc != SDMI_OK) return rc;
-  if (m <= 64) return lora_rows_launch<false>(p, st);
-#ifdef LORA_VARIANT
-#if LORA_VARIANT == 1
-  return lora_launch<128, 128, 2, 2, 2>(p, st);
-#elif LORA_VARIANT == 2
-  return lora_launch<128, 64, 2, 2, 2>(p, st);
-#elif LORA_VARIANT == 3
-  return lora_launch<64, 64, 2, 2, 2>(p, st);
-#elif LORA_VARIANT == 4
-  return lora_launch<64, 64, 2, 2, 3>(p, st);
-#elif LORA_VARIANT == 5
-  return lora_launch<64, 128, 2, 2, 2>(p, st);
-#elif LORA_VARIANT == 6
-  return lora_launch<64, 128, 2, 2, 3>(p, st);
-#endif
-#endif
-  if ((long long)((m + 127) / 128) * ((n + 63) / 64) >= 512) return lora_launch<128, 64, 2, 2, 2>(p, st);
-  return lora_launch<64, 64, 2, 2, 3>(p, st);
+  const LoraPlan pl = lora_plan(m, n, rank, groups, rows_per_id);
+  if (lora_needs_t(pl.kind)) {
+    const int rc = lora_shrink_launch(p, st);
+    if (rc != SDMI_OK) return rc;
+  }
+  if (pl.kind == LORA_ROWS_FUSED) return lora_rows_launch<true>(p, st);
+  if (pl.kind == LORA_ROWS) return lora_rows_launch<false>(p, st);
+  return pl.bm == 128 ? lora_tiles_launch<128, 2>(p, pl.kind, st) : lora_tiles_launch<64, 3>(p, pl.kind, st);
 }

@@ -153,9 +153,9 @@ __global__ __launch_bounds__(256, DP * QT <= 64 ? 3 : DP * QT <= 128 ? 2 : 1) vo
   const int sp = bid % p.splits;
   bid /= p.splits;
   const int hk = bid % p.kvh, bz = bid / p.kvh;
-  const int ctx = p.index ? p.index[bz] : (p.contexts == 1 ? 0 : bz);
+  const int ctx = p.index ? scalar_i32(p.index + bz) : (p.contexts == 1 ? 0 : bz);
   const bool ctx_ok = ctx >= 0 && ctx < p.contexts;
-  const int len = !ctx_ok ? 0 : p.lens ? min(max(p.lens[ctx], 0), p.nkv) : p.nkv;
+  const int len = !ctx_ok ? 0 : p.lens ? min(max(scalar_i32(p.lens + ctx), 0), p.nkv) : p.nkv;
   const int ntiles = (len + KT - 1) / KT;
   const int t0 = (int)((long long)ntiles * sp / p.splits), t1 = (int)((long long)ntiles * (sp + 1) / p.splits);
   const int cz = ctx_ok ? ctx : 0;

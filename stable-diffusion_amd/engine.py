@@ -661,7 +661,7 @@ def lora_gemm(a, wp, n_out, lora, ids, bias=None, residual=None, out=None):
     if nid == 0 or m % nid:
         raise L.SdmiError("lora_gemm: %d ids do not divide %d rows" % (nid, m))
     _own_device("lora_gemm", a.buf, wp, lora.a, lora.b, lora.scale, ids, bias, None if residual is None else residual.buf, res.buf)
-    need = L.load().sdmi_lora_gemm_ws_bytes(m, n_out, k, lora.rank, lora.groups)
+    need = L.load().sdmi_lora_gemm_ws_bytes(m, n_out, k, lora.rank, lora.groups, m // nid)
     ws = torch.empty((need,), dtype=torch.uint8, device=a.buf.device) if need else None      # the call's own: two graphs never share it
     L.call("sdmi_lora_gemm", a.ptr, a.ld, wp.data_ptr(), wp.stride(0), res.ptr, res.ld, m, n_out, k, 0 if bias is None else bias.data_ptr(), rp, rld,
            lora.a.data_ptr(), lora.b.data_ptr(), lora.scale.data_ptr(), lora.adapters, lora.rank, lora.groups, ip, m // nid, flags, ws.data_ptr() if need else 0, need,

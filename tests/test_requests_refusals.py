@@ -42,6 +42,6 @@ def test_workspace_sizes():
     assert lib.sdmi_cross_attention_ws_bytes(2, 5, 5, 64, 9216, 77) == 0            # one pass
     assert lib.sdmi_cross_attention_ws_bytes(1, 2, 2, 64, 1, 5000) > 0              # keys in pieces
     assert lib.sdmi_cross_attention_ws_bytes(1, 2, 2, 60, 1, 5000) == 0             # refused shapes need nothing
-    assert lib.sdmi_lora_gemm_ws_bytes(100, 96, 64, 16, 3) >= 100 * 48 * 2
-    assert lib.sdmi_lora_gemm_ws_bytes(100, 96, 64, 12, 3) == 0
-    assert lib.sdmi_lora_gemm_ws_bytes(1, 96, 64, 16, 1) == 0                       # one launch: nothing to hand over
+    assert lib.sdmi_lora_gemm_ws_bytes(100, 96, 64, 16, 3, 1) >= 100 * 48 * 2
+    assert lib.sdmi_lora_gemm_ws_bytes(100, 96, 64, 12, 3, 1) == 0
+    assert lib.sdmi_lora_gemm_ws_bytes(1, 96, 64, 16, 1, 1) == 0                       # one launch: nothing to hand over
