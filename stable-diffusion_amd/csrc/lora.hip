@@ -29,6 +29,7 @@ struct LoraParams {
   const float* scale;
   const int* ids;
   int adapters, rank, groups, rpi;
+  float inv_rpi;
   u16* t;  // [M][groups * rank]
   int ldt, tiles_n, per, tpg;  // per = N / groups; request-aligned tiles: tpg column tiles to a group
 };
@@ -38,16 +39,42 @@ __device__ __forceinline__ int lora_id(const LoraParams& p, int row) {
   return id >= 0 && id < p.adapters ? id : -1;
 }
 
+// the same for a wave-uniform row below 64: the quotient by a product (its distance from a whole number is at least 1 / 128 where
+// it is not 0) and the word through the scalar cache
+__device__ __forceinline__ int lora_row_id(const LoraParams& p, int row) {
+  const int id = scalar_i32(p.ids + __builtin_amdgcn_readfirstlane((int)((row + 0.5f) * p.inv_rpi)));
+  return id < p.adapters ? id : -1;
+}
+
+// ---- a wave's own panel of LDS: rows of 64 k, moved by DMA 8 rows (1 KB, whole 128-byte lines) an instruction.  Fragments read
+// straight from memory (16 rows x 64 B an instruction) ran at a fifth of this rate: 35 MB took 7.5 us.
+constexpr int LBK = 64;
+__device__ __forceinline__ int lora_off(int row, int chunk) { return row * LBK + ((chunk ^ ((row >> 1) & 7)) << 3); }
+// rows [0, 8 N8) x k [k0, k0 + 64) of a panel to LDS byte address `lds`; rows past `rows` and k past K read as zeros
+template <int N8>
+__device__ __forceinline__ void lora_panel(const u16* base, int ld, int rows, int k0, int K, unsigned lds, int lane) {
+  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, DMA_OOB, 0x00020000);
+#pragma unroll
+  for (int i = 0; i < N8; ++i) {
+    const int r = 8 * i + (lane >> 3), k = k0 + ((lane & 7) ^ ((r >> 1) & 7)) * 8;
+    dma_buf16(rs, (r < rows) & (k < K) ? 2u * (unsigned)(r * ld + k) : DMA_OOB, 0, lds + i * 1024);
+  }
+}
+
 // ------------------------------------------------------------------------------------------------------------ t = scale x a^T
-// Block: 16 MR rows by 16 NT columns of t, K cut over KW waves (32 of it a step), joined in wave order through the LDS.  A block
-// works for ONE adapter: blockIdx.z is the z-th distinct one among its rows; every row keeps its own adapter's result, blocks
-// beyond the last one leave.  Operands come straight from memory in fragment layout (8 consecutive k of one row per lane); UN
-// steps' loads are issued before the first product waits for one.
-template <int MR, int NT, int KW>
-__global__ __launch_bounds__(64 * KW, 1) void lora_shrink_kernel(const LoraParams p) {
-  constexpr int UN = MR + NT <= 3 ? 5 : MR + NT <= 6 ? 4 : 3;
-  __shared__ float red[KW][MR * NT * 4][64];
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, l15 = lane & 15, lq = lane >> 4;
+// Block: 16 MR rows by 16 NT columns of t; its eight waves take the K-steps of 64 in turn, each in a panel of its own (S steps in
+// flight, no barrier), and join in wave order through the LDS.  A block works for ONE adapter: blockIdx.z is the z-th distinct
+// one among its rows; every row keeps its own adapter's result, blocks beyond the last one leave.
+template <int MR, int NT>
+struct ShrinkShape {
+  static constexpr int S = 9 / (MR + NT) > 0 ? 9 / (MR + NT) : 1, WAVE = S * (MR + NT) * 2048;  // bytes of a wave's panel
+  static constexpr int red = MR * NT * 8192, bytes = 8 * WAVE > red ? 8 * WAVE : red;
+};
+template <int MR, int NT>
+__global__ __launch_bounds__(512, 1) void lora_shrink_kernel(const LoraParams p) {
+  typedef ShrinkShape<MR, NT> H;
+  extern __shared__ __attribute__((aligned(16))) u16 smem[];
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, lq = lane >> 4;
   const int row0 = blockIdx.x * (16 * MR), n0 = blockIdx.y * (NT * 16), NR = p.ldt;
   const int mine = lane < 16 * MR && row0 + lane < p.M ? lora_id(p, row0 + lane) : -1;
   unsigned long long todo = __builtin_amdgcn_ballot_w64(mine >= 0);  // the same in every wave
@@ -58,52 +85,57 @@ __global__ __launch_bounds__(64 * KW, 1) void lora_shrink_kernel(const LoraParam
     todo &= ~__builtin_amdgcn_ballot_w64(mine == id);
   }
   if (!todo) return;
+  const float sc = p.scale[id];
   f32x4 acc[MR][NT];
 #pragma unroll
   for (int i = 0; i < MR; ++i)
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const u16* const zp = (const u16*)g_lora_zero16;
-  const u16 *xr[MR], *ar[NT];
+  const u16* const xb = p.x + (long long)row0 * p.ldx;
+  const u16* const ab = p.la + ((long long)id * NR + n0) * p.K;
+  const unsigned lds = lds_addr_of(smem) + wv * H::WAVE;
+  const u16* const sm = smem + wv * (H::WAVE / 2);
+  for (int k1 = wv; k1 < p.nk; k1 += 8 * H::S) {
 #pragma unroll
-  for (int i = 0; i < MR; ++i) xr[i] = p.x + (long long)min(row0 + 16 * i + l15, p.M - 1) * p.ldx + 8 * lq;
-#pragma unroll
-  for (int j = 0; j < NT; ++j) ar[j] = p.la + ((long long)id * NR + min(n0 + 16 * j + l15, NR - 1)) * p.K;
-  for (int kb = wv * 32; kb < p.K; kb += 32 * KW * UN) {
-    hx8 xf[UN][MR], af[UN][NT];
-#pragma unroll
-    for (int u = 0; u < UN; ++u) {
-      const int k = kb + 32 * KW * u;
-      const bool in = k + 8 * lq < p.K;  // K is a multiple of 8; past it x reads as zeros, and a as its first columns
-#pragma unroll
-      for (int i = 0; i < MR; ++i) xf[u][i] = *(const hx8*)(in ? xr[i] + k : zp);
-#pragma unroll
-      for (int j = 0; j < NT; ++j) af[u][j] = *(const hx8*)(ar[j] + (in ? k + 8 * lq : 0));
+    for (int s = 0; s < H::S; ++s) {
+      const int k0 = (k1 + 8 * s) * LBK;  // past the last step: zeros
+      lora_panel<2 * MR>(xb, p.ldx, p.M - row0, k0, p.K, lds + s * (MR + NT) * 2048, lane);
+      lora_panel<2 * NT>(ab, p.K, NR - n0, k0, p.K, lds + (s * (MR + NT) + MR) * 2048, lane);
     }
-    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
-    for (int u = 0; u < UN; ++u)
+    for (int s = 0; s < H::S; ++s)
 #pragma unroll
-      for (int i = 0; i < MR; ++i)
+      for (int kk = 0; kk < 2; ++kk) {
+        hx8 xf[MR], af[NT];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = MFMA16(af[u][j], xf[u][i], acc[i][j], 0, 0, 0);
+        for (int i = 0; i < MR; ++i) xf[i] = *(const hx8*)&sm[s * (MR + NT) * 1024 + lora_off(16 * i + l15, lq + 4 * kk)];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) af[j] = *(const hx8*)&sm[(s * (MR + NT) + MR) * 1024 + lora_off(16 * j + l15, lq + 4 * kk)];
+#pragma unroll
+        for (int i = 0; i < MR; ++i)
+#pragma unroll
+          for (int j = 0; j < NT; ++j) acc[i][j] = MFMA16(af[j], xf[i], acc[i][j], 0, 0, 0);
+      }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the panel is read before the next steps land in it
   }
+  __syncthreads();
+  float* const red = (float*)smem;  // [wave][tile][4][64]: row 16 i + l15, column 16 j + 4 lq + e
 #pragma unroll
   for (int i = 0; i < MR; ++i)
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) red[wv][(i * NT + j) * 4 + e][lane] = acc[i][j][e];  // row 16 i + l15, column 16 j + 4 lq + e
+      for (int e = 0; e < 4; ++e) red[((wv * MR * NT + i * NT + j) * 4 + e) * 64 + lane] = acc[i][j][e];
   __syncthreads();
-  const float sc = p.scale[id];
-  for (int q = wv; q < MR * NT; q += KW) {
+  for (int q = wv; q < MR * NT; q += 8) {
     const int i = q / NT, j = q - i * NT, n = n0 + 16 * j + 4 * lq;
     float y[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       y[e] = 0.f;
 #pragma unroll
-      for (int w = 0; w < KW; ++w) y[e] += red[w][q * 4 + e][lane];
+      for (int w = 0; w < 8; ++w) y[e] += red[((w * MR * NT + q) * 4 + e) * 64 + lane];
       y[e] *= sc;
     }
     const int his = __shfl(mine, 16 * i + l15);
@@ -112,24 +144,46 @@ __global__ __launch_bounds__(64 * KW, 1) void lora_shrink_kernel(const LoraParam
 }
 
 // ------------------------------------------------------------------------------------------------------------ up to 64 rows
-// Block: 16 columns x all M <= 16 MT rows, K cut over 8 waves (32 of it a step), fragments straight from memory: w is read once by
-// the whole grid, x by every block (L2).  The adapters: thread (m, n) takes the dot product of t[m] and b[id][n], rank long, from
-// memory too.  FUSE: the block computes t of its rows itself (m * groups * rank <= 64 dot products of length K, one wave each
-// in turn) instead of reading what an earlier launch left.
+// Block: 16 columns x all M <= 16 MT rows; its eight waves take the K-steps in turn, as above: w is read once by the whole grid, x
+// by every block (L2).  The adapters: four lanes share a (row, column) pair and take the dot product of t[m] and b[id][n], rank
+// long, 16 bytes each at a time; the first 32 ranks of both are fetched before the product.  FUSE: the block computes t of its rows
+// itself (m * groups * rank <= 64 dot products of length K, one wave each in turn) instead of reading what an earlier launch left.
+template <int MT>
+struct RowsShape {
+  static constexpr int S = 9 / (MT + 1), WAVE = S * (MT + 1) * 2048, bytes = 8 * WAVE;  // the join needs 8 MT KB of it
+};
 template <int MT, bool FUSE>
 __global__ __launch_bounds__(512, 1) void lora_rows_kernel(const LoraParams p) {
-  constexpr int UN = MT == 4 ? 4 : 8;
-  __shared__ float red[8][MT * 4][64];
+  typedef RowsShape<MT> H;
+  constexpr int NP = MT * 16 * 16 / 128;  // (row, column) pairs a group of four lanes finishes
+  extern __shared__ __attribute__((aligned(16))) u16 smem[];
   __shared__ float st[FUSE ? 64 : 1];
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, l15 = lane & 15, lq = lane >> 4, n0 = blockIdx.x * 16;
-  const u16* const zp = (const u16*)g_lora_zero16;
+  const int t = threadIdx.x, lane = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6), l15 = lane & 15, lq = lane >> 4, n0 = blockIdx.x * 16;
+  // pair x of this lane group: column n0 + c, row x * 8 + (t >> 6)
+  const int c = (t >> 2) & 15, piece = t & 3, n = n0 + c, nc = min(n, p.N - 1), g = nc / p.per;
+  int id[NP];
+  uint4 b0[NP], t0[FUSE ? 1 : NP];
+#pragma unroll
+  for (int x = 0; x < NP; ++x) {
+    const int m = 8 * x + wv;
+    id[x] = m < p.M ? lora_row_id(p, m) : -1;
+  }
+#pragma unroll
+  for (int x = 0; x < NP; ++x) {
+    b0[x] = make_uint4(0u, 0u, 0u, 0u);
+    if constexpr (!FUSE) t0[x] = b0[x];
+    if (id[x] >= 0 && 8 * piece < p.rank) {
+      b0[x] = *(const uint4*)(p.lb + ((long long)id[x] * p.N + nc) * p.rank + 8 * piece);
+      if constexpr (!FUSE) t0[x] = *(const uint4*)(p.t + (long long)(8 * x + wv) * p.ldt + g * p.rank + 8 * piece);
+    }
+  }
   if constexpr (FUSE) {
     // only the groups that this block's columns lie in
     const int g0 = n0 / p.per, g1 = min(n0 + 15, p.N - 1) / p.per, ng = (g1 - g0 + 1) * p.rank;
     for (int d = wv; d < p.M * ng; d += 8) {
-      const int m = d / ng, r = g0 * p.rank + (d - m * ng), id = lora_id(p, m);
-      if (id < 0) continue;
-      const u16 *xr = p.x + (long long)m * p.ldx, *ar = p.la + ((long long)id * p.ldt + r) * p.K;
+      const int m = d / ng, r = g0 * p.rank + (d - m * ng), idm = lora_row_id(p, m);
+      if (idm < 0) continue;
+      const u16 *xr = p.x + (long long)m * p.ldx, *ar = p.la + ((long long)idm * p.ldt + r) * p.K;
       float s = 0.f;
       for (int k = 8 * lane; k < p.K; k += 512) {
         float xv[8], av[8];
@@ -139,77 +193,87 @@ __global__ __launch_bounds__(512, 1) void lora_rows_kernel(const LoraParams p) {
         for (int e = 0; e < 8; ++e) s = __builtin_fmaf(xv[e], av[e], s);
       }
       s = wave_sum(s);
-      if (lane == 0) st[m * p.ldt + r] = (float)f2h16(s * p.scale[id]);  // rounded as the stored t is
+      if (lane == 0) st[m * p.ldt + r] = (float)f2h16(s * p.scale[idm]);  // rounded as the stored t is
     }
   }
   f32x4 acc[MT];
 #pragma unroll
   for (int i = 0; i < MT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  {
-    const u16* wrow = p.w + (long long)min(n0 + l15, p.N - 1) * p.ldw;
-    const u16* xr[MT];
+  const u16* const wb = p.w + (long long)n0 * p.ldw;
+  const unsigned lds = lds_addr_of(smem) + wv * H::WAVE;
+  const u16* const sm = smem + wv * (H::WAVE / 2);
+  for (int k1 = wv; k1 < p.nk; k1 += 8 * H::S) {
 #pragma unroll
-    for (int i = 0; i < MT; ++i) xr[i] = p.x + (long long)min(16 * i + l15, p.M - 1) * p.ldx + 8 * lq;
-    for (int kb = wv * 32; kb < p.K; kb += 256 * UN) {
-      hx8 wf[UN], xf[UN][MT];
-#pragma unroll
-      for (int u = 0; u < UN; ++u) {
-        const int k = kb + 256 * u;
-        const bool in = k + 8 * lq < p.K;
-        wf[u] = *(const hx8*)(wrow + (in ? k + 8 * lq : 0));
-#pragma unroll
-        for (int i = 0; i < MT; ++i) xf[u][i] = *(const hx8*)(in ? xr[i] + k : zp);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int u = 0; u < UN; ++u)
-#pragma unroll
-        for (int i = 0; i < MT; ++i) acc[i] = MFMA16(wf[u], xf[u][i], acc[i], 0, 0, 0);
+    for (int s = 0; s < H::S; ++s) {
+      const int k0 = (k1 + 8 * s) * LBK;
+      lora_panel<2>(wb, p.ldw, p.N - n0, k0, p.K, lds + s * (MT + 1) * 2048, lane);
+      lora_panel<2 * MT>(p.x, p.ldx, p.M, k0, p.K, lds + (s * (MT + 1) + 1) * 2048, lane);
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int s = 0; s < H::S; ++s)
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        const hx8 wf = *(const hx8*)&sm[s * (MT + 1) * 1024 + lora_off(l15, lq + 4 * kk)];
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+          acc[i] = MFMA16(wf, *(const hx8*)&sm[(s * (MT + 1) + 1) * 1024 + lora_off(16 * i + l15, lq + 4 * kk)], acc[i], 0, 0, 0);
+      }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
+  __syncthreads();
+  float* const red = (float*)smem;  // [wave][4 i + e][64]: row 16 i + l15, column 4 lq + e
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) red[wv][4 * i + e][lane] = acc[i][e];  // row 16 i + l15, column 4 lq + e
+    for (int e = 0; e < 4; ++e) red[(wv * MT * 4 + 4 * i + e) * 64 + lane] = acc[i][e];
   __syncthreads();
-  // thread -> (row, column): 16 neighbouring threads share a row and read 16 consecutive b rows
-  const int c = threadIdx.x & 15, n = n0 + c;
-  if (n >= p.N) return;
-  const int g = n / p.per;
 #pragma unroll
-  for (int m0 = 0; m0 < MT * 16; m0 += 32) {
-    const int m = m0 + (threadIdx.x >> 4);
-    if (m >= p.M || m >= MT * 16) continue;
+  for (int x = 0; x < NP; ++x) {
+    const int m = 8 * x + wv;
+    if (m >= p.M) break;  // the rows of a wave rise
     float y = 0.f;
+    float bv[8], tv[8];
+    auto dot = [&]() {
 #pragma unroll
-    for (int w = 0; w < 8; ++w) y += red[w][4 * (m >> 4) + (c & 3)][(c >> 2) * 16 + (m & 15)];
-    const int id = lora_id(p, m);
-    if (id >= 0) {
-      const u16* br = p.lb + ((long long)id * p.N + n) * p.rank;
-      const u16* tr = p.t + (long long)m * p.ldt + g * p.rank;
-#pragma unroll 4
-      for (int r = 0; r < p.rank; r += 8) {
-        float bv[8], tv[8];
+      for (int e = 0; e < 8; ++e) y = __builtin_fmaf(tv[e], bv[e], y);
+    };
+    const int tb = m * p.ldt + g * p.rank;
+    if (id[x] >= 0) {
+      unpack8(b0[x], bv);  // zeros past the rank
+      if constexpr (FUSE) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) tv[e] = 8 * piece < p.rank ? st[tb + 8 * piece + e] : 0.f;
+      } else {
+        unpack8(t0[x], tv);
+      }
+      dot();
+      const u16* br = p.lb + ((long long)id[x] * p.N + nc) * p.rank;
+      for (int r = 32 + 8 * piece; r < p.rank; r += 32) {
         unpack8(*(const uint4*)(br + r), bv);
         if constexpr (FUSE) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) tv[e] = st[m * p.ldt + g * p.rank + r + e];
+          for (int e = 0; e < 8; ++e) tv[e] = st[tb + r + e];
         } else {
-          unpack8(*(const uint4*)(tr + r), tv);
+          unpack8(*(const uint4*)(p.t + tb + r), tv);
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y = __builtin_fmaf(tv[e], bv[e], y);
+        dot();
       }
     }
-    if (p.bias) y += p.bias[n];
-    if (p.residual) y += h2f(p.residual[(long long)m * p.ldr + n]);
-    p.out[(long long)m * p.ldo + n] = f2h(y);
+    // the eight shares of the product: two to each of the four lanes
+#pragma unroll
+    for (int w = 0; w < 2; ++w) y += red[((2 * piece + w) * MT * 4 + 4 * (m >> 4) + (c & 3)) * 64 + (c >> 2) * 16 + (m & 15)];
+    y += __shfl_xor(y, 1);
+    y += __shfl_xor(y, 2);
+    if (piece == 0 && n < p.N) {
+      if (p.bias) y += p.bias[n];
+      if (p.residual) y += h2f(p.residual[(long long)m * p.ldr + n]);
+      p.out[(long long)m * p.ldo + n] = f2h(y);
+    }
   }
 }
 
 // ------------------------------------------------------------------------------------------------------------ many rows
-constexpr int LBK = 64;
-__device__ __forceinline__ int lora_off(int row, int chunk) { return row * LBK + ((chunk ^ ((row >> 1) & 7)) << 3); }
 // 64 lanes x 16 B from 64 addresses to 1 KB of LDS at byte address `lds`; waited for by the loop's own s_waitcnt
 __device__ __forceinline__ void lora_dma16(const void* src, unsigned lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory", "m0");
@@ -504,26 +568,49 @@ extern "C" int64_t sdmi_lora_gemm_ws_bytes(int m, int n, int k, int rank, int gr
   return (int64_t)m * groups * rank * 2;
 }
 
-template <int MR, int NT, int KW>
-static void lora_shrink_launch2(const LoraParams& p, hipStream_t st) {
-  constexpr int TR = 16 * MR;
+// a kernel with more than 64 KB of dynamic LDS: allowed once per device
+template <typename F>
+static int lora_allow_lds(F* kernel, int bytes, std::atomic<unsigned long long>& done) {
+  if (bytes <= 64 * 1024) return SDMI_OK;
+  int dev = 0;
+  (void)hipGetDevice(&dev);
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return SDMI_OK;
+  const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != hipSuccess) {
+    sdmi_set_error("lora_gemm: %d bytes of LDS refused: %s", bytes, hipGetErrorString(e));
+    return SDMI_ELAUNCH;
+  }
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return SDMI_OK;
+}
+
+template <int MR, int NT>
+static int lora_shrink_launch2(const LoraParams& p, hipStream_t st) {
+  static std::atomic<unsigned long long> done{0};
+  constexpr int TR = 16 * MR, bytes = ShrinkShape<MR, NT>::bytes;
+  static_assert(bytes <= 160 * 1024, "LDS of a CU");
+  const int rc = lora_allow_lds(lora_shrink_kernel<MR, NT>, bytes, done);
+  if (rc != SDMI_OK) return rc;
   const int touched = p.rpi >= TR ? (p.rpi % TR == 0 ? 1 : 2) : min((TR - 1 + p.rpi - 1) / p.rpi + 1, TR);  // requests that TR rows can touch
-  hipLaunchKernelGGL((lora_shrink_kernel<MR, NT, KW>), dim3((p.M + TR - 1) / TR, (p.ldt + 16 * NT - 1) / (16 * NT), min(touched, p.adapters)), dim3(64 * KW), 0, st, p);
+  hipLaunchKernelGGL((lora_shrink_kernel<MR, NT>), dim3((p.M + TR - 1) / TR, (p.ldt + 16 * NT - 1) / (16 * NT), min(touched, p.adapters)), dim3(512), bytes, st, p);
+  return sdmi_check_launch("lora_gemm (low-rank factor)");
 }
 static int lora_shrink_launch(const LoraParams& p, hipStream_t st) {
-  // 64-row blocks share each reading of a; with few rows smaller ones spread over more of the chip
-  const bool big = (long long)((p.M + 63) / 64) * ((p.ldt + 63) / 64) * (p.rpi >= 64 ? 1 : min(p.adapters, 4)) >= 128;
-  if (big && p.ldt > 32) lora_shrink_launch2<4, 4, 4>(p, st);
-  else if (big) lora_shrink_launch2<4, 2, 8>(p, st);
-  else if (p.ldt > 16) lora_shrink_launch2<1, 2, 8>(p, st);
-  else lora_shrink_launch2<1, 1, 8>(p, st);
-  return sdmi_check_launch("lora_gemm (low-rank factor)");
+  // larger blocks share more of each reading of x and a; with few of them smaller ones spread over more of the chip
+  const int z = p.rpi >= 64 ? 1 : min(p.adapters, 4);
+  if (p.ldt > 32 && (long long)((p.M + 63) / 64) * ((p.ldt + 63) / 64) * z >= 128) return lora_shrink_launch2<4, 4>(p, st);
+  if (p.ldt > 16 && (long long)((p.M + 31) / 32) * ((p.ldt + 31) / 32) * z >= 128) return lora_shrink_launch2<2, 2>(p, st);
+  return p.ldt > 16 ? lora_shrink_launch2<1, 2>(p, st) : lora_shrink_launch2<1, 1>(p, st);
 }
 
 template <int BM, int BN, int WM, int WN, int NSTAGE, bool MIXED, int FR>
 static int lora_launch(LoraParams p, hipStream_t st) {
   constexpr int bytes = NSTAGE * (BM + BN + FR) * LBK * 2 + (MIXED ? (2 * BM + 1) * 4 : 0);
-  static_assert(bytes <= 64 * 1024, "LDS without an attribute");
+  static_assert(bytes <= 80 * 1024, "two blocks to a CU");
+  static std::atomic<unsigned long long> done{0};
+  const int rc = lora_allow_lds(lora_gemm_kernel<BM, BN, WM, WN, NSTAGE, MIXED, FR>, bytes, done);
+  if (rc != SDMI_OK) return rc;
   long long tiles_m;
   if (MIXED) {
     p.tiles_n = (p.N + BN - 1) / BN;
@@ -542,18 +629,23 @@ template <int BM, int NSTAGE>
 static int lora_tiles_launch(const LoraParams& p, int kind, hipStream_t st) {
   if (kind == LORA_MIXED) return lora_launch<BM, 64, 2, 2, NSTAGE, true, 0>(p, st);
   if (kind == LORA_TILES) return lora_launch<BM, 64, 2, 2, NSTAGE, false, 0>(p, st);
+  // 128 x 128 tiles, which move a quarter less, once there are four to a CU: 18432 x 1920 70 us against 78, 18432 x 320 14.8 against 14.4
+  if (BM == 128 && (long long)(p.M / 128) * (p.N / 128) >= 1024)
+    return p.rank <= 16 ? lora_launch<BM, BM, 2, 2, 2, false, 16>(p, st) : lora_launch<BM, BM, 2, 2, 2, false, 32>(p, st);
   return p.rank <= 16 ? lora_launch<BM, 64, 2, 2, 2, false, 16>(p, st) : lora_launch<BM, 64, 2, 2, 2, false, 32>(p, st);
 }
-template <bool FUSE>
-static int lora_rows_launch(const LoraParams& p, hipStream_t st) {
-  const dim3 grid((p.N + 15) / 16), block(512);
-  if (p.M <= 16) hipLaunchKernelGGL((lora_rows_kernel<1, FUSE>), grid, block, 0, st, p);
-  else if constexpr (!FUSE) {
-    if (p.M <= 32) hipLaunchKernelGGL((lora_rows_kernel<2, FUSE>), grid, block, 0, st, p);
-    else hipLaunchKernelGGL((lora_rows_kernel<4, FUSE>), grid, block, 0, st, p);
-  }
-  sdmi_note_kernel(FUSE ? "lora_rows_kernel" : "lora_shrink_kernel + lora_rows_kernel");
+template <int MT, bool FUSE>
+static int lora_rows_launch2(const LoraParams& p, hipStream_t st) {
+  static std::atomic<unsigned long long> done{0};
+  const int rc = lora_allow_lds(lora_rows_kernel<MT, FUSE>, RowsShape<MT>::bytes, done);
+  if (rc != SDMI_OK) return rc;
+  hipLaunchKernelGGL((lora_rows_kernel<MT, FUSE>), dim3((p.N + 15) / 16), dim3(512), RowsShape<MT>::bytes, st, p);
+  sdmi_note_kernel("%slora_rows_kernel<%d, %s>", FUSE ? "" : "lora_shrink_kernel + ", MT, FUSE ? "true" : "false");
   return sdmi_check_launch("lora_gemm (few rows)");
+}
+static int lora_rows_launch(const LoraParams& p, bool fuse, hipStream_t st) {
+  if (fuse) return lora_rows_launch2<1, true>(p, st);
+  return p.M <= 16 ? lora_rows_launch2<1, false>(p, st) : p.M <= 32 ? lora_rows_launch2<2, false>(p, st) : lora_rows_launch2<4, false>(p, st);
 }
 
 extern "C" int sdmi_lora_gemm(const void* x, int ldx, const void* w, int ldw, void* out, int ldo, int m, int n, int k, const float* bias,
@@ -582,7 +674,7 @@ extern "C" int sdmi_lora_gemm(const void* x, int ldx, const void* w, int ldw, vo
   p.residual = (flags & SDMI_F_RESIDUAL) ? (const u16*)residual : nullptr;
   p.ldr = ldr;
   p.la = (const u16*)lora_a; p.lb = (const u16*)lora_b; p.scale = lora_scale; p.ids = ids;
-  p.adapters = adapters; p.rank = rank; p.groups = groups; p.rpi = rows_per_id;
+  p.adapters = adapters; p.rank = rank; p.groups = groups; p.rpi = rows_per_id; p.inv_rpi = 1.0f / rows_per_id;
   p.t = (u16*)ws; p.ldt = groups * rank; p.per = n / groups;
   hipStream_t st = (hipStream_t)stream;
   const LoraPlan pl = lora_plan(m, n, rank, groups, rows_per_id);
@@ -590,7 +682,7 @@ extern "C" int sdmi_lora_gemm(const void* x, int ldx, const void* w, int ldw, vo
     const int rc = lora_shrink_launch(p, st);
     if (rc != SDMI_OK) return rc;
   }
-  if (pl.kind == LORA_ROWS_FUSED) return lora_rows_launch<true>(p, st);
-  if (pl.kind == LORA_ROWS) return lora_rows_launch<false>(p, st);
+  if (pl.kind == LORA_ROWS_FUSED) return lora_rows_launch(p, true, st);
+  if (pl.kind == LORA_ROWS) return lora_rows_launch(p, false, st);
   return pl.bm == 128 ? lora_tiles_launch<128, 2>(p, pl.kind, st) : lora_tiles_launch<64, 3>(p, pl.kind, st);
 }
