@@ -22,7 +22,7 @@ struct XattnParams {
   u16* o;
   long long sq, sk, sv, so;
   int ldq, ldk, ldv, ldo;
-  int contexts, heads, kvh, group, dim, nq, nkv, rows, rtiles, splits;  // rows = nq * group: the rows of one kv head
+  int batch, contexts, heads, kvh, group, dim, nq, nkv, rows, rtiles, splits;  // rows = nq * group: the rows of one kv head
   const int *index, *lens;
   const unsigned *qreg, *kreg;
   long long sqr, skr;
@@ -55,6 +55,7 @@ __device__ __forceinline__ void xa_step(const u16* sK, const u16* sV, const unsi
   const int r = lane & 31, hh = lane >> 5, dblk = (lane >> 4) & 1, tq = (lane & 15) >> 2, tp = lane & 3;
 #pragma unroll
   for (int b = 0; b < KS; ++b) {
+    if (MODE != XA_FULL && key0 + 32 * b >= klim) continue;  // nothing of this block is left (the same for the whole wave)
     f32x16 s[QT];
 #pragma unroll
     for (int x = 0; x < QT; ++x)
@@ -152,7 +153,9 @@ __global__ __launch_bounds__(256, DP * QT <= 64 ? 3 : DP * QT <= 128 ? 2 : 1) vo
   bid /= p.rtiles;
   const int sp = bid % p.splits;
   bid /= p.splits;
-  const int hk = bid % p.kvh, bz = bid / p.kvh;
+  // the samples of one head follow each other: an XCD's run of blocks then holds long and short contexts alike (with the heads of one
+  // sample together, two contexts of 9216 and 4600 keys took as long as two of 9216), and samples that share a context meet in its L2
+  const int bz = bid % p.batch, hk = bid / p.batch;
   const int ctx = p.index ? scalar_i32(p.index + bz) : (p.contexts == 1 ? 0 : bz);
   const bool ctx_ok = ctx >= 0 && ctx < p.contexts;
   const int len = !ctx_ok ? 0 : p.lens ? min(max(scalar_i32(p.lens + ctx), 0), p.nkv) : p.nkv;
@@ -233,12 +236,15 @@ __global__ __launch_bounds__(256, DP * QT <= 64 ? 3 : DP * QT <= 128 ? 2 : 1) vo
       for (int i = 0; i < 16; ++i) oacc[x][dt][i] = 0.f;
   }
   const int kr0 = wk * (KT / WK), tfull = min(t1, len / KT);  // tiles below tfull are whole
+  // the rows' own loads are waited for here, where the compiler sees it: it would else wait inside the loop for everything in
+  // flight, the next tile's DMA among it (long states: 171 -> see below)
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
   XA_LANDED();
   for (int tile = t0; tile < (REG ? t1 : tfull); ++tile) {
     const int cur = (tile - t0) & 1;
     if (tile + 1 < t1) stage(tile + 1, cur ^ 1);
     const u16* sK = smem + cur * S::BUF;
-    xa_step<DP, QT, S::KS, REG ? XA_REGIONS : XA_FULL>(sK, sK + KT * DP, sreg + cur * KT, qf, oacc, m, l, p.c, kr0, 0, 0, qset, lane);
+    xa_step<DP, QT, S::KS, REG ? XA_REGIONS : XA_FULL>(sK, sK + KT * DP, sreg + cur * KT, qf, oacc, m, l, p.c, kr0, tile * KT + kr0, len, qset, lane);
     XA_LANDED();
   }
   if (!REG && t0 < t1 && tfull < t1) {  // the one partial tile: all sets of waves are past it, its data has landed
@@ -349,11 +355,11 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(const XattnParams p, lo
 }
 
 // ------------------------------------------------------------------------------------------------------------ host
-struct XattnPlan { int kind, rtiles, splits; };  // kind 0: 128 rows a block, 1: 128 rows in 64-row waves by two key shares, 2: few rows
+struct XattnPlan { int kind, rtiles, splits; };  // kind 0: 128 rows a block, 1: 64 rows by two key shares, 2: few rows
 static XattnPlan xattn_plan(int batch, int kvh, int dim, int rows, int nkv) {
   XattnPlan pl;
-  pl.kind = rows <= 64 ? 2 : (dim <= 64 && nkv >= 512) ? 1 : 0;
-  const int per = pl.kind == 2 ? (dim <= 128 ? 32 : 64) : 128;
+  pl.kind = rows <= 64 ? 2 : (dim <= 96 && nkv >= 512) ? 1 : 0;
+  const int per = pl.kind == 2 ? (dim <= 128 ? 32 : 64) : pl.kind == 1 ? 64 : 128;
   pl.rtiles = (rows + per - 1) / per;
   const long long blocks = (long long)batch * kvh * pl.rtiles;
   // few rows over long states: cut the keys until the chip is full (512 blocks: two per CU), at least 256 keys to a piece
@@ -392,8 +398,8 @@ static int xattn_launch1(const XattnParams& p, int blocks, hipStream_t st) {
 }
 template <int DP>
 static int xattn_launch(const XattnParams& p, int kind, int blocks, hipStream_t st) {
-  if constexpr (DP <= 64)
-    if (kind == 1) return xattn_launch1<DP, 2, 2, 128>(p, blocks, st);
+  if constexpr (DP <= 96)
+    if (kind == 1) return xattn_launch1<DP, 1, 2, 64>(p, blocks, st);
   if (kind == 2) return xattn_launch1<DP, 1, DP <= 128 ? 4 : 2, DP <= 128 ? 128 : 64>(p, blocks, st);
   return xattn_launch1<DP, 1, 1, 64>(p, blocks, st);
 }
@@ -430,7 +436,7 @@ extern "C" int sdmi_cross_attention(const void* q, int ldq, int64_t sq, const vo
   XattnParams p = {};
   p.q = (const u16*)q; p.k = (const u16*)k; p.v = (const u16*)v; p.o = (u16*)o;
   p.sq = sq; p.sk = sk; p.sv = sv; p.so = so; p.ldq = ldq; p.ldk = ldk; p.ldv = ldv; p.ldo = ldo;
-  p.contexts = contexts; p.heads = heads; p.kvh = kv_heads; p.group = heads / kv_heads; p.dim = dim; p.nq = nq; p.nkv = nkv;
+  p.batch = batch; p.contexts = contexts; p.heads = heads; p.kvh = kv_heads; p.group = heads / kv_heads; p.dim = dim; p.nq = nq; p.nkv = nkv;
   p.rows = nq * p.group;
   p.index = index; p.lens = lens; p.qreg = query_regions; p.kreg = key_regions; p.sqr = sqr; p.skr = skr;
   p.c = scale * 1.44269504088896340736f;

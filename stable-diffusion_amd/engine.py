@@ -4,6 +4,7 @@ PyTorch is used for device memory (torch.empty), the current HIP stream and para
 arithmetic runs in libsdmi355.so.  There is no fallback: a missing library raises (see _lib.load).
 """
 import ctypes
+import functools
 import math
 import os
 import weakref
@@ -581,9 +582,15 @@ def _own_device(what, *tensors):
 def _int32(t, shape, what):
     if t is None:
         return 0
-    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous():
         raise L.SdmiError("%s: expected contiguous int32 %s, got %s %s" % (what, tuple(shape), t.dtype, tuple(t.shape)))
     return t.data_ptr()
+
+
+@functools.lru_cache(maxsize=4096)
+def _ws_need(name, *shape):
+    """A workspace size of the library: a function of the shape alone, asked for once."""
+    return getattr(L.load(), name)(*shape)
 
 
 def cross_attention(q, k, v, heads, kv_heads=None, dim=64, scale=None, index=None, lens=None, query_regions=None, key_regions=None, out=None):
@@ -604,14 +611,17 @@ def cross_attention(q, k, v, heads, kv_heads=None, dim=64, scale=None, index=Non
     if q.c != wq or k.c != wk or v.c != wk or v.n != n or v.h * v.w != nkv or o.n != b or o.h * o.w != nq or o.c != wq:
         raise L.SdmiError("cross_attention: q (%d,%d,%d) / k (%d,%d,%d) / v (%d,%d,%d) / out (%d,%d,%d) do not match %d heads on %d key heads of %d" %
                           (b, nq, q.c, n, nkv, k.c, v.n, v.hw, v.c, o.n, o.hw, o.c, heads, kv_heads, dim))
-    _own_device("cross_attention", q.buf, k.buf, v.buf, o.buf, index, lens, query_regions, key_regions)
-    ip, lp = _int32(index, (b,), "cross_attention: index"), _int32(lens, (n,), "cross_attention: lens")
-    qr, kr = _int32(query_regions, (b, nq), "cross_attention: query_regions"), _int32(key_regions, (n, nkv), "cross_attention: key_regions")
-    need = L.load().sdmi_cross_attention_ws_bytes(b, heads, kv_heads, dim, nq, nkv)
-    ws = torch.empty((need,), dtype=torch.uint8, device=q.buf.device) if need else None     # the call's own: two graphs never share it
-    ldq, ldk, ldv, ldo = q.ld, k.ld, v.ld, o.ld
-    L.call("sdmi_cross_attention", q.ptr, ldq, nq * ldq, k.ptr, ldk, nkv * ldk, v.ptr, ldv, nkv * ldv, o.ptr, ldo, nq * ldo, b, n, heads, kv_heads, dim, nq, nkv,
-           ip, lp, qr, nq, kr, nkv, dim ** -0.5 if scale is None else float(scale), ws.data_ptr() if need else 0, need, _stream())
+    qb, kb, vb, ob = q.buf, k.buf, v.buf, o.buf
+    _own_device("cross_attention", qb, kb, vb, ob, index, lens, query_regions, key_regions)
+    need = _ws_need("sdmi_cross_attention_ws_bytes", b, heads, kv_heads, dim, nq, nkv)
+    ws = torch.empty((need,), dtype=torch.uint8, device=qb.device) if need else None     # the call's own: two graphs never share it
+    ldq, ldk, ldo = qb.shape[-1], kb.shape[-1], ob.shape[-1]
+    ldv = ldk if vb is kb else vb.shape[-1]
+    L.call("sdmi_cross_attention", q.ptr, ldq, nq * ldq, kb.data_ptr() + 2 * k.off, ldk, nkv * ldk, vb.data_ptr() + 2 * v.off, ldv,
+           nkv * ldv, ob.data_ptr() + 2 * o.off, ldo, nq * ldo, b, n, heads, kv_heads, dim, nq, nkv,
+           _int32(index, (b,), "cross_attention: index"), _int32(lens, (n,), "cross_attention: lens"),
+           _int32(query_regions, (b, nq), "cross_attention: query_regions"), nq, _int32(key_regions, (n, nkv), "cross_attention: key_regions"), nkv,
+           dim ** -0.5 if scale is None else float(scale), ws.data_ptr() if need else 0, need, _stream())
     return o
 
 
@@ -661,11 +671,12 @@ def lora_gemm(a, wp, n_out, lora, ids, bias=None, residual=None, out=None):
     if nid == 0 or m % nid:
         raise L.SdmiError("lora_gemm: %d ids do not divide %d rows" % (nid, m))
     _own_device("lora_gemm", a.buf, wp, lora.a, lora.b, lora.scale, ids, bias, None if residual is None else residual.buf, res.buf)
-    need = L.load().sdmi_lora_gemm_ws_bytes(m, n_out, k, lora.rank, lora.groups, m // nid)
-    ws = torch.empty((need,), dtype=torch.uint8, device=a.buf.device) if need else None      # the call's own: two graphs never share it
-    L.call("sdmi_lora_gemm", a.ptr, a.ld, wp.data_ptr(), wp.stride(0), res.ptr, res.ld, m, n_out, k, 0 if bias is None else bias.data_ptr(), rp, rld,
-           lora.a.data_ptr(), lora.b.data_ptr(), lora.scale.data_ptr(), lora.adapters, lora.rank, lora.groups, ip, m // nid, flags, ws.data_ptr() if need else 0, need,
-           _stream())
+    need = _ws_need("sdmi_lora_gemm_ws_bytes", m, n_out, k, lora.rank, lora.groups, m // nid)
+    ab, ob = a.buf, res.buf
+    ws = torch.empty((need,), dtype=torch.uint8, device=ab.device) if need else None     # the call's own: two graphs never share it
+    L.call("sdmi_lora_gemm", a.ptr, ab.shape[-1], wp.data_ptr(), wp.stride(0), ob.data_ptr() + 2 * res.off, ob.shape[-1], m, n_out, k,
+           0 if bias is None else bias.data_ptr(), rp, rld, lora.a.data_ptr(), lora.b.data_ptr(), lora.scale.data_ptr(), lora.adapters, lora.rank, lora.groups,
+           ip, m // nid, flags, ws.data_ptr() if need else 0, need, _stream())
     if RANGE_AUDIT:
         _audit("lora_gemm %dx%dx%d" % (m, n_out, k), res)
     return res
