@@ -48,33 +48,26 @@ constexpr float XA_RAISE = 8.0f;  // the running maximum is raised once a score 
 
 enum { XA_FULL = 0, XA_TAIL = 1, XA_REGIONS = 2 };
 
-// One wave's share of a key tile: KS blocks of 32 keys (from row kr0 of the tile) against its QT x 32 rows.
-template <int DP, int QT, int KS, int MODE>
-__device__ __forceinline__ void xa_step(const u16* sK, const u16* sV, const unsigned* sR, const hx8 (&qf)[QT][DP / 16], f32x16 (&oacc)[QT][DP / 32],
-                                        float (&m)[QT], float (&l)[QT], float c, int kr0, int key0, int klim, const unsigned (&qset)[QT], int lane) {
+constexpr int XA_KT = 64;  // keys of a tile
+
+// One wave's share of a key tile: KS blocks of 32 keys (from row kr0 of the tile) against its 32 rows.
+template <int DP, int KS, int MODE>
+__device__ __forceinline__ void xa_step(const u16* sK, const u16* sV, const unsigned* sR, const hx8 (&qf)[DP / 16], f32x16 (&oacc)[DP / 32], float& m,
+                                        float& l, float c, int kr0, int key0, int klim, unsigned qset, int lane) {
   const int r = lane & 31, hh = lane >> 5, dblk = (lane >> 4) & 1, tq = (lane & 15) >> 2, tp = lane & 3;
 #pragma unroll
   for (int b = 0; b < KS; ++b) {
-    if (MODE != XA_FULL && key0 + 32 * b >= klim) continue;  // nothing of this block is left (the same for the whole wave)
-    f32x16 s[QT];
+    if (MODE != XA_FULL && KS > 1 && key0 + 32 * b >= klim) continue;  // nothing of this block is left (the same for the whole wave)
+    f32x16 s;
 #pragma unroll
-    for (int x = 0; x < QT; ++x)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[x][i] = 0.f;
+    for (int i = 0; i < 16; ++i) s[i] = 0.f;
     const int krow = kr0 + 32 * b + r;
 #pragma unroll
-    for (int ks = 0; ks < DP / 16; ++ks) {
-      const hx8 kf = *(const hx8*)&sK[krow * DP + (((2 * ks + hh) ^ xa_kx<DP>(krow)) << 3)];
-#pragma unroll
-      for (int x = 0; x < QT; ++x) s[x] = MFMA32(kf, qf[x][ks], s[x], 0, 0, 0);
-    }
+    for (int ks = 0; ks < DP / 16; ++ks) s = MFMA32(*(const hx8*)&sK[krow * DP + (((2 * ks + hh) ^ xa_kx<DP>(krow)) << 3)], qf[ks], s, 0, 0, 0);
     if constexpr (MODE == XA_TAIL) {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        if (key0 + 32 * b + 8 * (i >> 2) + 4 * hh + (i & 3) >= klim) {
-#pragma unroll
-          for (int x = 0; x < QT; ++x) s[x][i] = -__builtin_inff();
-        }
+        if (key0 + 32 * b + 8 * (i >> 2) + 4 * hh + (i & 3) >= klim) s[i] = -__builtin_inff();
     }
     if constexpr (MODE == XA_REGIONS) {  // keys past the end carry the empty set
 #pragma unroll
@@ -82,42 +75,36 @@ __device__ __forceinline__ void xa_step(const u16* sK, const u16* sV, const unsi
         const u32x4 kr = *(const u32x4*)&sR[kr0 + 32 * b + 8 * g + 4 * hh];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-#pragma unroll
-          for (int x = 0; x < QT; ++x)
-            if (!(kr[e] & qset[x])) s[x][4 * g + e] = -__builtin_inff();
+          if (!(kr[e] & qset)) s[4 * g + e] = -__builtin_inff();
       }
     }
-    hx8 pb[QT][2];
+    float mx = s[0];
 #pragma unroll
-    for (int x = 0; x < QT; ++x) {
-      float mx = s[x][0];
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+    mx *= c;
+    // both halves of the wave raise together: the exchange and the rescaling happen in this rare branch only
+    if (__builtin_amdgcn_ballot_w64(mx > m + XA_RAISE) != 0) {
+      const float mnew = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32)));
+      const float alpha = __builtin_amdgcn_exp2f(m - mnew);
+      l *= alpha;
 #pragma unroll
-      for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[x][i]);
-      mx *= c;
-      if (__builtin_amdgcn_ballot_w64(mx > m[x] + XA_RAISE) != 0) {
-        const float mnew = fmaxf(m[x], fmaxf(mx, __shfl_xor(mx, 32)));
-        const float alpha = __builtin_amdgcn_exp2f(m[x] - mnew);
-        l[x] *= alpha;
+      for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
-        for (int dt = 0; dt < DP / 32; ++dt)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) oacc[x][dt][i] *= alpha;
-        m[x] = mnew;
-      }
-      float rs = 0.f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[x][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][i], c, -m[x]));
-        rs += s[x][i];
-      }
-      l[x] += rs;
-#pragma unroll
-      for (int s2 = 0; s2 < 2; ++s2)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) pb[x][s2][j] = (h16)s[x][8 * s2 + j];
+        for (int i = 0; i < 16; ++i) oacc[dt][i] *= alpha;
+      m = mnew;
     }
+    float rs = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -m));
+      rs += s[i];
+    }
+    l += rs;
 #pragma unroll
     for (int s2 = 0; s2 < 2; ++s2) {
+      hx8 pb;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) pb[j] = (h16)s[8 * s2 + j];
       const int vrow = kr0 + 32 * b + 16 * s2 + 4 * hh + tq;  // and vrow + 8, whose swizzle is the same
 #pragma unroll
       for (int dt = 0; dt < DP / 32; ++dt) {
@@ -125,25 +112,24 @@ __device__ __forceinline__ void xa_step(const u16* sK, const u16* sV, const unsi
         union { struct { short4_t a, b; } h; hx8 v; } u;
         u.h.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((short4_t __attribute__((address_space(3)))*)vp);
         u.h.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((short4_t __attribute__((address_space(3)))*)(vp + 8 * DP));
-#pragma unroll
-        for (int x = 0; x < QT; ++x) oacc[x][dt] = MFMA32(u.v, pb[x][s2], oacc[x][dt], 0, 0, 0);
+        oacc[dt] = MFMA32(u.v, pb, oacc[dt], 0, 0, 0);
       }
     }
   }
 }
 
-// Block: 4 waves = WR row groups of QT x 32 rows by WK shares of every tile of KT keys; the shares' (m, l, O) merge in the LDS.
-template <int DP, int QT, int WK, int KT, bool REG>
+// Block: 4 waves = 4 / WK groups of 32 rows by WK shares of every tile; the shares' (m, l, O) merge in the LDS.
+template <int DP, int WK, bool REG>
 struct XaShape {
-  static constexpr int WR = 4 / WK, KS = KT / 32 / WK, ROWS = WR * QT * 32, BUF = 2 * KT * DP;  // BUF: elements of K and V of a tile
-  static constexpr int merge = WK == 1 ? 0 : 4 * QT * 32 * (DP * 4 + 8);
-  static constexpr int stage = 2 * (BUF * 2 + (REG ? KT * 4 : 0));
+  static constexpr int WR = 4 / WK, KS = XA_KT / 32 / WK, ROWS = WR * 32, BUF = 2 * XA_KT * DP;  // BUF: elements of K and V of a tile
+  static constexpr int merge = WK == 1 ? 0 : 4 * 32 * (DP * 4 + 8);
+  static constexpr int stage = 2 * (BUF * 2 + (REG ? XA_KT * 4 : 0));
   static constexpr int bytes = stage > merge ? stage : merge;
 };
-template <int DP, int QT, int WK, int KT, bool REG>
-__global__ __launch_bounds__(256, DP * QT <= 64 ? 3 : DP * QT <= 128 ? 2 : 1) void xattn_kernel(const XattnParams p) {
-  typedef XaShape<DP, QT, WK, KT, REG> S;
-  constexpr int CH = DP / 8, PT = KT * CH / 256;  // 16-byte pieces of a row; pieces of K (and of V) a thread moves per tile
+template <int DP, int WK, bool REG>
+__global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void xattn_kernel(const XattnParams p) {
+  typedef XaShape<DP, WK, REG> S;
+  constexpr int KT = XA_KT, CH = DP / 8, PT = KT * CH / 256;  // 16-byte pieces of a row; pieces of K (and of V) a thread moves per tile
   static_assert(KT * CH % 256 == 0 && S::KS >= 1, "tile / wave grid mismatch");
   extern __shared__ __attribute__((aligned(16))) u16 smem[];
   unsigned* const sreg = (unsigned*)(smem + 2 * S::BUF);
@@ -154,7 +140,7 @@ __global__ __launch_bounds__(256, DP * QT <= 64 ? 3 : DP * QT <= 128 ? 2 : 1) vo
   const int sp = bid % p.splits;
   bid /= p.splits;
   // the samples of one head follow each other: an XCD's run of blocks then holds long and short contexts alike (with the heads of one
-  // sample together, two contexts of 9216 and 4600 keys took as long as two of 9216), and samples that share a context meet in its L2
+  // sample together, contexts of 9216 and 4600 keys took as long as two of 9216), and samples that share a context meet in its L2
   const int bz = bid % p.batch, hk = bid / p.batch;
   const int ctx = p.index ? scalar_i32(p.index + bz) : (p.contexts == 1 ? 0 : bz);
   const bool ctx_ok = ctx >= 0 && ctx < p.contexts;
@@ -200,125 +186,100 @@ __global__ __launch_bounds__(256, DP * QT <= 64 ? 3 : DP * QT <= 128 ? 2 : 1) vo
       for (int i = 0; i < PT; ++i) dma_buf16(rv, voff[i], 0, dst + KT * DP * 2 + i * 4096);
     }
   };
-#define XA_LANDED() \
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory")
+  // every DMA of this wave has landed and its reads of the buffer that is staged next have returned; then meet the others
+#define XA_LANDED() asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory")
   if (t0 < t1) stage(t0, 0);
 
   // ---- this wave's rows: row rho of the kv head is query rho / group, head rho % group of the group
-  int qi[QT], head[QT], rho[QT];
-  hx8 qf[QT][DP / 16];
-  unsigned qset[QT];
+  const int rho = rt * S::ROWS + wr * 32 + r, rc = min(rho, p.rows - 1);
+  const int qi = rc / p.group, head = hk * p.group + rc % p.group;
+  const u16* Q = p.q + (long long)bz * p.sq + (long long)qi * p.ldq + head * p.dim;
+  hx8 qf[DP / 16];
 #pragma unroll
-  for (int x = 0; x < QT; ++x) {
-    rho[x] = rt * S::ROWS + (wr * QT + x) * 32 + r;
-    const int rc = min(rho[x], p.rows - 1);
-    qi[x] = rc / p.group;
-    head[x] = hk * p.group + rc % p.group;
-    const u16* Q = p.q + (long long)bz * p.sq + (long long)qi[x] * p.ldq + head[x] * p.dim;
+  for (int ks = 0; ks < DP / 16; ++ks) {
+    const int d = 16 * ks + 8 * hh;
 #pragma unroll
-    for (int ks = 0; ks < DP / 16; ++ks) {
-      const int d = 16 * ks + 8 * hh;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) qf[x][ks][e] = (h16)0.f;
-      if (d < p.dim) qf[x][ks] = *(const hx8*)(Q + d);
-    }
-    qset[x] = REG ? p.qreg[(long long)bz * p.sqr + qi[x]] : 0u;
+    for (int e = 0; e < 8; ++e) qf[ks][e] = (h16)0.f;
+    if (d < p.dim) qf[ks] = *(const hx8*)(Q + d);
   }
-  f32x16 oacc[QT][DP / 32];
-  float m[QT], l[QT];
+  const unsigned qset = REG ? p.qreg[(long long)bz * p.sqr + qi] : 0u;
+  f32x16 oacc[DP / 32];
+  float m = XA_LOWEST, l = 0.f;
 #pragma unroll
-  for (int x = 0; x < QT; ++x) {
-    m[x] = XA_LOWEST;
-    l[x] = 0.f;
+  for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
-    for (int dt = 0; dt < DP / 32; ++dt)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) oacc[x][dt][i] = 0.f;
-  }
+    for (int i = 0; i < 16; ++i) oacc[dt][i] = 0.f;
   const int kr0 = wk * (KT / WK), tfull = min(t1, len / KT);  // tiles below tfull are whole
   // the rows' own loads are waited for here, where the compiler sees it: it would else wait inside the loop for everything in
-  // flight, the next tile's DMA among it (long states: 171 -> see below)
+  // flight, the next tile's DMA among it
   __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
   XA_LANDED();
+#pragma unroll 1
   for (int tile = t0; tile < (REG ? t1 : tfull); ++tile) {
     const int cur = (tile - t0) & 1;
     if (tile + 1 < t1) stage(tile + 1, cur ^ 1);
     const u16* sK = smem + cur * S::BUF;
-    xa_step<DP, QT, S::KS, REG ? XA_REGIONS : XA_FULL>(sK, sK + KT * DP, sreg + cur * KT, qf, oacc, m, l, p.c, kr0, tile * KT + kr0, len, qset, lane);
+    xa_step<DP, S::KS, REG ? XA_REGIONS : XA_FULL>(sK, sK + KT * DP, sreg + cur * KT, qf, oacc, m, l, p.c, kr0, tile * KT + kr0, len, qset, lane);
     XA_LANDED();
   }
-  if (!REG && t0 < t1 && tfull < t1) {  // the one partial tile: all sets of waves are past it, its data has landed
+  if (!REG && t0 < t1 && tfull < t1) {  // the one partial tile: its data has landed
     const u16* sK = smem + ((t1 - 1 - t0) & 1) * S::BUF;
-    xa_step<DP, QT, S::KS, XA_TAIL>(sK, sK + KT * DP, sreg, qf, oacc, m, l, p.c, kr0, (t1 - 1) * KT + kr0, len, qset, lane);
+    xa_step<DP, S::KS, XA_TAIL>(sK, sK + KT * DP, sreg, qf, oacc, m, l, p.c, kr0, (t1 - 1) * KT + kr0, len, qset, lane);
   }
 #undef XA_LANDED
-#pragma unroll
-  for (int x = 0; x < QT; ++x) l[x] += __shfl_xor(l[x], 32);
+  l += __shfl_xor(l, 32);
 
+  float* const mo = (float*)smem;  // WK > 1: [wave][dt][16][64]
   if constexpr (WK > 1) {
     // merge: m and l of the rows, then each share's O scaled to the common maximum; share wk of a row group finishes the groups
     // g = wk, wk + WK, ... of every 32 columns, summing in the order of the shares
-    float* const mo = (float*)smem;                         // [wave][x][dt][16][64]
-    float2* const mml = (float2*)(mo + 4 * QT * 32 * DP);   // [wave][x][32]
+    float2* const mml = (float2*)(mo + 4 * 32 * DP);  // [wave][32]
     __syncthreads();
-#pragma unroll
-    for (int x = 0; x < QT; ++x)
-      if (hh == 0) mml[(wv * QT + x) * 32 + r] = make_float2(m[x], l[x]);
+    if (hh == 0) mml[wv * 32 + r] = make_float2(m, l);
     __syncthreads();
+    float mall = XA_LOWEST, lall = 0.f;
 #pragma unroll
-    for (int x = 0; x < QT; ++x) {
-      float mall = XA_LOWEST, lall = 0.f;
+    for (int w = 0; w < WK; ++w) mall = fmaxf(mall, mml[(wr * WK + w) * 32 + r].x);
 #pragma unroll
-      for (int w = 0; w < WK; ++w) mall = fmaxf(mall, mml[((wr * WK + w) * QT + x) * 32 + r].x);
-#pragma unroll
-      for (int w = 0; w < WK; ++w) {
-        const float2 v = mml[((wr * WK + w) * QT + x) * 32 + r];
-        lall += v.y * __builtin_amdgcn_exp2f(v.x - mall);
-      }
-      const float alpha = __builtin_amdgcn_exp2f(m[x] - mall);
-#pragma unroll
-      for (int dt = 0; dt < DP / 32; ++dt)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) mo[(((wv * QT + x) * (DP / 32) + dt) * 16 + i) * 64 + lane] = oacc[x][dt][i] * alpha;
-      m[x] = mall;
-      l[x] = lall;
+    for (int w = 0; w < WK; ++w) {
+      const float2 v = mml[(wr * WK + w) * 32 + r];
+      lall += v.y * __builtin_amdgcn_exp2f(v.x - mall);
     }
-    __syncthreads();
-#pragma unroll
-    for (int x = 0; x < QT; ++x)
-#pragma unroll
-      for (int dt = 0; dt < DP / 32; ++dt)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          if (g % WK != wk) continue;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float y = 0.f;
-#pragma unroll
-            for (int w = 0; w < WK; ++w) y += mo[((((wr * WK + w) * QT + x) * (DP / 32) + dt) * 16 + 4 * g + e) * 64 + lane];
-            oacc[x][dt][4 * g + e] = y;
-          }
-        }
-  }
-#pragma unroll
-  for (int x = 0; x < QT; ++x) {
-    if (rho[x] >= p.rows) continue;
-    const float inv = l[x] > 0.f ? 1.0f / l[x] : 0.f;
-    const long long prow = ((long long)bz * p.kvh + hk) * p.rows + rho[x];
-    float* po = p.po + (prow * p.splits + sp) * p.dim;
-    u16* O = p.o + (long long)bz * p.so + (long long)qi[x] * p.ldo + head[x] * p.dim;
-    if (p.splits > 1 && wk == 0 && hh == 0) p.pml[prow * p.splits + sp] = make_float2(m[x], l[x]);
+    const float alpha = __builtin_amdgcn_exp2f(m - mall);
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int d = 32 * dt + 8 * g + 4 * hh;
-        if (g % WK != wk || d >= p.dim) continue;
-        const f32x4 y = {oacc[x][dt][4 * g], oacc[x][dt][4 * g + 1], oacc[x][dt][4 * g + 2], oacc[x][dt][4 * g + 3]};
-        if (p.splits > 1) *(f32x4*)(po + d) = y;
-        else *(uint2*)(O + d) = make_uint2(pack2h(y[0] * inv, y[1] * inv), pack2h(y[2] * inv, y[3] * inv));
-      }
+      for (int i = 0; i < 16; ++i) mo[((wv * (DP / 32) + dt) * 16 + i) * 64 + lane] = oacc[dt][i] * alpha;
+    m = mall;
+    l = lall;
+    __syncthreads();
   }
+  if (rho >= p.rows) return;
+  const float inv = l > 0.f ? 1.0f / l : 0.f;
+  const long long prow = ((long long)bz * p.kvh + hk) * p.rows + rho;
+  float* po = p.po + (prow * p.splits + sp) * p.dim;
+  u16* O = p.o + (long long)bz * p.so + (long long)qi * p.ldo + head * p.dim;
+  if (p.splits > 1 && wk == 0 && hh == 0) p.pml[prow * p.splits + sp] = make_float2(m, l);
+#pragma unroll
+  for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+    for (int gi = 0; gi < 4 / WK; ++gi) {
+      const int g = WK * gi + wk, d = 32 * dt + 8 * g + 4 * hh;
+      f32x4 y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (WK == 1) {
+          y[e] = oacc[dt][4 * gi + e];
+        } else {
+          y[e] = 0.f;
+#pragma unroll
+          for (int w = 0; w < WK; ++w) y[e] += mo[(((wr * WK + w) * (DP / 32) + dt) * 16 + 4 * g + e) * 64 + lane];
+        }
+      }
+      if (d >= p.dim) continue;
+      if (p.splits > 1) *(f32x4*)(po + d) = y;
+      else *(uint2*)(O + d) = make_uint2(pack2h(y[0] * inv, y[1] * inv), pack2h(y[2] * inv, y[3] * inv));
+    }
 }
 
 // Joins the splits of a row, in split order: one wave per row, the splits' (m, l) on the lanes.
@@ -355,24 +316,29 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(const XattnParams p, lo
 }
 
 // ------------------------------------------------------------------------------------------------------------ host
-struct XattnPlan { int kind, rtiles, splits; };  // kind 0: 128 rows a block, 1: 64 rows by two key shares, 2: few rows
+struct XattnPlan { int wk, rtiles, splits; };
 static XattnPlan xattn_plan(int batch, int kvh, int dim, int rows, int nkv) {
   XattnPlan pl;
-  pl.kind = rows <= 64 ? 2 : (dim <= 96 && nkv >= 512) ? 1 : 0;
-  const int per = pl.kind == 2 ? (dim <= 128 ? 32 : 64) : pl.kind == 1 ? 64 : 128;
+  // one wave sweeps all keys for its 32 rows, or two waves share them.  The second gives blocks of 64 rows: fewer of them idle where
+  // there are few, and finer pieces where contexts differ (2304 rows to 9216 keys, heads of 64: 155 us against 190; of 80, to 4096: 88
+  // against 99; of 128: 139 against 124; 9216 rows to 77 keys: 15.6 against 12.4, for the merge is paid per block)
+  const bool few = rows <= 64;
+  pl.wk = few || (dim <= 96 && nkv >= 512) ? 2 : 1;
+  const int per = pl.wk == 2 ? 64 : 128;
   pl.rtiles = (rows + per - 1) / per;
   const long long blocks = (long long)batch * kvh * pl.rtiles;
-  // few rows over long states: cut the keys until the chip is full (512 blocks: two per CU), at least 256 keys to a piece
-  long long s = 512 / (blocks > 0 ? blocks : 1);
+  // few blocks over long states: cut the keys until the chip is full (512 blocks: two per CU), at least 256 keys to a piece.  With
+  // few rows the join is cheap and the quotient is rounded up (320 blocks of one row to 9216 keys: 161 us whole)
+  long long s = (few ? 511 + blocks : 512) / (blocks > 0 ? blocks : 1);
   if (s > nkv / 256) s = nkv / 256;
   if (s > 64) s = 64;
   pl.splits = s < 2 ? 1 : (int)s;
   return pl;
 }
 
-template <int DP, int QT, int WK, int KT, bool REG>
+template <int DP, int WK, bool REG>
 static int xattn_launch2(const XattnParams& p, int blocks, hipStream_t st) {
-  constexpr int bytes = XaShape<DP, QT, WK, KT, REG>::bytes;
+  constexpr int bytes = XaShape<DP, WK, REG>::bytes;
   static_assert(bytes <= 160 * 1024, "LDS of a CU");
   if constexpr (bytes > 64 * 1024) {
     static std::atomic<unsigned long long> done{0};
@@ -380,7 +346,7 @@ static int xattn_launch2(const XattnParams& p, int blocks, hipStream_t st) {
     (void)hipGetDevice(&dev);
     const unsigned long long bit = 1ull << (dev & 63);
     if (!(done.load(std::memory_order_relaxed) & bit)) {
-      const hipError_t e = hipFuncSetAttribute((const void*)xattn_kernel<DP, QT, WK, KT, REG>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+      const hipError_t e = hipFuncSetAttribute((const void*)xattn_kernel<DP, WK, REG>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
       if (e != hipSuccess) {
         sdmi_set_error("cross_attention: %d bytes of LDS refused: %s", bytes, hipGetErrorString(e));
         return SDMI_ELAUNCH;
@@ -388,20 +354,14 @@ static int xattn_launch2(const XattnParams& p, int blocks, hipStream_t st) {
       done.fetch_or(bit, std::memory_order_relaxed);
     }
   }
-  hipLaunchKernelGGL((xattn_kernel<DP, QT, WK, KT, REG>), dim3(blocks), dim3(256), bytes, st, p);
-  sdmi_note_kernel("xattn_kernel<%d, %d, %d, %d, %s>%s", DP, QT, WK, KT, REG ? "true" : "false", p.splits > 1 ? " + xattn_join_kernel" : "");
+  hipLaunchKernelGGL((xattn_kernel<DP, WK, REG>), dim3(blocks), dim3(256), bytes, st, p);
+  sdmi_note_kernel("xattn_kernel<%d, %d, %s>%s", DP, WK, REG ? "true" : "false", p.splits > 1 ? " + xattn_join_kernel" : "");
   return sdmi_check_launch("cross_attention");
 }
-template <int DP, int QT, int WK, int KT>
-static int xattn_launch1(const XattnParams& p, int blocks, hipStream_t st) {
-  return p.qreg ? xattn_launch2<DP, QT, WK, KT, true>(p, blocks, st) : xattn_launch2<DP, QT, WK, KT, false>(p, blocks, st);
-}
 template <int DP>
-static int xattn_launch(const XattnParams& p, int kind, int blocks, hipStream_t st) {
-  if constexpr (DP <= 96)
-    if (kind == 1) return xattn_launch1<DP, 1, 2, 64>(p, blocks, st);
-  if (kind == 2) return xattn_launch1<DP, 1, DP <= 128 ? 4 : 2, DP <= 128 ? 128 : 64>(p, blocks, st);
-  return xattn_launch1<DP, 1, 1, 64>(p, blocks, st);
+static int xattn_launch(const XattnParams& p, int wk, int blocks, hipStream_t st) {
+  if (wk == 2) return p.qreg ? xattn_launch2<DP, 2, true>(p, blocks, st) : xattn_launch2<DP, 2, false>(p, blocks, st);
+  return p.qreg ? xattn_launch2<DP, 1, true>(p, blocks, st) : xattn_launch2<DP, 1, false>(p, blocks, st);
 }
 
 static bool xattn_shape_ok(int batch, int heads, int kv_heads, int dim, int nq, int nkv) {
@@ -451,12 +411,12 @@ extern "C" int sdmi_cross_attention(const void* q, int ldq, int64_t sq, const vo
   SDMI_REQUIRE(blocks < (1ll << 31) && (prows + 3) / 4 < (1ll << 31), "cross_attention: grid too large");
   hipStream_t st = (hipStream_t)stream;
   int rc;
-  if (dim <= 32) rc = xattn_launch<32>(p, pl.kind, (int)blocks, st);
-  else if (dim <= 64) rc = xattn_launch<64>(p, pl.kind, (int)blocks, st);
-  else if (dim <= 96) rc = xattn_launch<96>(p, pl.kind, (int)blocks, st);
-  else if (dim <= 128) rc = xattn_launch<128>(p, pl.kind, (int)blocks, st);
-  else if (dim <= 160) rc = xattn_launch<160>(p, pl.kind, (int)blocks, st);
-  else rc = xattn_launch<256>(p, pl.kind, (int)blocks, st);
+  if (dim <= 32) rc = xattn_launch<32>(p, pl.wk, (int)blocks, st);
+  else if (dim <= 64) rc = xattn_launch<64>(p, pl.wk, (int)blocks, st);
+  else if (dim <= 96) rc = xattn_launch<96>(p, pl.wk, (int)blocks, st);
+  else if (dim <= 128) rc = xattn_launch<128>(p, pl.wk, (int)blocks, st);
+  else if (dim <= 160) rc = xattn_launch<160>(p, pl.wk, (int)blocks, st);
+  else rc = xattn_launch<256>(p, pl.wk, (int)blocks, st);
   if (rc != SDMI_OK || pl.splits == 1) return rc;
   hipLaunchKernelGGL(xattn_join_kernel, dim3((unsigned)((prows + 3) / 4)), dim3(256), 0, st, p, (long long)prows);
   return sdmi_check_launch("cross_attention (join)");
