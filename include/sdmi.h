@@ -289,7 +289,7 @@ int sdmi_attention_log2q(const void* q, int ldq, int64_t sq, const void* k, int 
  *        o[b][i] = sum_j softmax_j(scale q.k) v over the keys that i sees; a row that sees none is 0.
  *      Memory of keys at or past lens[context] is not read, and a key in no region may hold anything (NaN too); every other key
  *      has to be finite.  lens outside [0, nkv] count as the nearer end; an index outside [0, contexts) sees nothing.
- *      heads a multiple of kv_heads, dim a multiple of 8 up to 256, any nq >= 1 and nkv >= 0.  ws: scratch of
+ *      heads a multiple of kv_heads, dim a multiple of 8 up to 256, any nq >= 1 and nkv >= 0, scale in (0, 1e15].  ws: scratch of
  *      sdmi_cross_attention_ws_bytes for few rows over long states, whose keys are cut into pieces that a second launch joins
  *      in a fixed order; with NULL or fewer bytes they are not cut.  Calls that may overlap in time need a workspace each. */
 int sdmi_cross_attention(const void* q, int ldq, int64_t sq, const void* k, int ldk, int64_t sk, const void* v, int ldv, int64_t sv,
@@ -308,7 +308,8 @@ int64_t sdmi_cross_attention_ws_bytes(int batch, int heads, int kv_heads, int di
  *      Adapters of smaller rank are padded with zeros (sdmi_pack_linear, sdmi_f32_to_h16_rows write both layouts).  k, rank
  *      and n / groups multiples of 8, rank up to 256, up to 64 groups; flags: SDMI_F_BIAS, SDMI_F_RESIDUAL; ws: scratch of
  *      sdmi_lora_gemm_ws_bytes (0: may be NULL), one per call that may overlap in time.  All pointers but lora_scale and ids are
- *      16-byte aligned. */
+ *      16-byte aligned.  t is held in h16 (as every activation, it saturates); sums are fp32.  The adapters that ids name have to
+ *      be finite: rows of other requests meet them with factors of 0. */
 int sdmi_lora_gemm(const void* x, int ldx, const void* w, int ldw, void* out, int ldo, int m, int n, int k, const float* bias,
                    const void* residual, int ldr, const void* lora_a, const void* lora_b, const float* lora_scale, int adapters,
                    int rank, int groups, const int32_t* ids, int rows_per_id, uint32_t flags, void* ws, int64_t ws_bytes, void* stream);

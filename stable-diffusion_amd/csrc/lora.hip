@@ -546,7 +546,7 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN == 4 && NSTAGE * (BM + BN + 
 // ------------------------------------------------------------------------------------------------------------ host
 static bool lora_shape_ok(int m, int n, int k, int rank, int groups) {
   // a group's columns are whole 8-column pieces: the kernels' tiles start at its first
-  return m > 0 && n > 0 && k > 0 && groups > 0 && groups <= 64 && n % groups == 0 && (n / groups) % 8 == 0 && k % 8 == 0 && rank > 0 && rank % 8 == 0 && rank <= 256;
+  return m > 0 && m < (1 << 30) && n > 0 && n < (1 << 30) && k > 0 && groups > 0 && groups <= 64 && n % groups == 0 && (n / groups) % 8 == 0 && k % 8 == 0 && rank > 0 && rank % 8 == 0 && rank <= 256;
 }
 // which kernels take a problem; the workspace holds t where a launch hands it to the next
 enum { LORA_ROWS_FUSED, LORA_ROWS, LORA_TILES_FUSED, LORA_TILES, LORA_MIXED };
@@ -564,7 +564,7 @@ static LoraPlan lora_plan(int m, int n, int rank, int groups, int rpi) {
 static bool lora_needs_t(int kind) { return kind != LORA_ROWS_FUSED && kind != LORA_TILES_FUSED; }
 
 extern "C" int64_t sdmi_lora_gemm_ws_bytes(int m, int n, int k, int rank, int groups, int rows_per_id) {
-  if (!lora_shape_ok(m, n, k, rank, groups) || rows_per_id <= 0 || !lora_needs_t(lora_plan(m, n, rank, groups, rows_per_id).kind)) return 0;
+  if (!lora_shape_ok(m, n, k, rank, groups) || rows_per_id <= 0 || !lora_needs_t(lora_plan(m, n, rank, groups, min(rows_per_id, m)).kind)) return 0;
   return (int64_t)m * groups * rank * 2;
 }
 
@@ -620,7 +620,7 @@ static int lora_launch(LoraParams p, hipStream_t st) {
     p.tiles_n = p.groups * p.tpg;
     tiles_m = (long long)((p.M + p.rpi - 1) / p.rpi) * ((p.rpi + BM - 1) / BM);
   }
-  SDMI_REQUIRE(tiles_m * p.tiles_n < (1ll << 31), "lora_gemm: grid too large");
+  SDMI_REQUIRE(tiles_m * p.tiles_n < (1ll << 24), "lora_gemm: grid too large");  // a launch has fewer than 2^32 threads
   hipLaunchKernelGGL((lora_gemm_kernel<BM, BN, WM, WN, NSTAGE, MIXED, FR>), dim3((unsigned)(tiles_m * p.tiles_n)), dim3(64 * WM * WN), bytes, st, p);
   sdmi_note_kernel("%slora_gemm_kernel<%d, %d, %s, %d>", FR ? "" : "lora_shrink_kernel + ", BM, BN, MIXED ? "true" : "false", FR);
   return sdmi_check_launch("lora_gemm");
@@ -667,6 +667,7 @@ extern "C" int sdmi_lora_gemm(const void* x, int ldx, const void* w, int ldw, vo
   const int64_t need = sdmi_lora_gemm_ws_bytes(m, n, k, rank, groups, rows_per_id);
   SDMI_REQUIRE(need == 0 || (ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= need), "lora_gemm: workspace of %lld bytes, %lld needed, 16-byte aligned",
                (long long)(ws ? ws_bytes : 0), (long long)need);
+  rows_per_id = min(rows_per_id, m);  // one id for all rows
   LoraParams p = {};
   p.x = (const u16*)x; p.w = (const u16*)w; p.out = (u16*)out; p.ldx = ldx; p.ldw = ldw; p.ldo = ldo;
   p.M = m; p.N = n; p.K = k; p.nk = (k + LBK - 1) / LBK;

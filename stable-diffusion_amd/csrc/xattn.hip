@@ -366,7 +366,7 @@ static int xattn_launch(const XattnParams& p, int wk, int blocks, hipStream_t st
 
 static bool xattn_shape_ok(int batch, int heads, int kv_heads, int dim, int nq, int nkv) {
   return batch > 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && dim >= 8 && dim <= 256 && dim % 8 == 0 && nq > 0 && nkv >= 0 &&
-         (long long)nq * (heads / kv_heads) < (1ll << 30) && (long long)heads * dim < (1ll << 22);
+         nkv < (1 << 30) && (long long)nq * (heads / kv_heads) < (1ll << 30) && (long long)heads * dim < (1ll << 22);
 }
 
 extern "C" int64_t sdmi_cross_attention_ws_bytes(int batch, int heads, int kv_heads, int dim, int nq, int nkv) {
@@ -392,7 +392,8 @@ extern "C" int sdmi_cross_attention(const void* q, int ldq, int64_t sq, const vo
   SDMI_REQUIRE((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) & 15) == 0 && ((uintptr_t)o & 7) == 0, "cross_attention: pointer alignment");
   SDMI_REQUIRE(!query_regions == !key_regions, "cross_attention: regions of queries and of keys go together");
   SDMI_REQUIRE((((uintptr_t)index | (uintptr_t)lens | (uintptr_t)query_regions | (uintptr_t)key_regions) & 3) == 0, "cross_attention: pointer alignment");
-  SDMI_REQUIRE(scale > 0.f && scale < 1e30f, "cross_attention: scale must be positive and finite");
+  // scores of 16-bit floats up to 65504 then stay within the running maximum's start
+  SDMI_REQUIRE(scale > 0.f && scale <= 1e15f, "cross_attention: scale must be positive and at most 1e15");
   XattnParams p = {};
   p.q = (const u16*)q; p.k = (const u16*)k; p.v = (const u16*)v; p.o = (u16*)o;
   p.sq = sq; p.sk = sk; p.sv = sv; p.so = so; p.ldq = ldq; p.ldk = ldk; p.ldv = ldv; p.ldo = ldo;
@@ -408,7 +409,8 @@ extern "C" int sdmi_cross_attention(const void* q, int ldq, int64_t sq, const vo
   p.po = (float*)ws;
   p.pml = pl.splits > 1 ? (float2*)((float*)ws + prows * pl.splits * dim) : nullptr;
   const long long blocks = (long long)batch * kv_heads * pl.rtiles * pl.splits;
-  SDMI_REQUIRE(blocks < (1ll << 31) && (prows + 3) / 4 < (1ll << 31), "cross_attention: grid too large");
+  // a launch has fewer than 2^32 threads
+  SDMI_REQUIRE(blocks < (1ll << 24) && (pl.splits == 1 || (prows + 3) / 4 < (1ll << 24)), "cross_attention: grid too large");
   hipStream_t st = (hipStream_t)stream;
   int rc;
   if (dim <= 32) rc = xattn_launch<32>(p, pl.wk, (int)blocks, st);

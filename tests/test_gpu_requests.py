@@ -212,6 +212,42 @@ def test_attention_without_workspace_is_not_cut():
     _close(o, want, tol, "attention without a workspace")
 
 
+ATT_WIDTHS = [  # the two block shapes at every width, with regions as well
+    (2, 2, 2, 2, 32, 5, 700, [1, 1], [3, 650], 3),
+    (2, 2, 2, 1, 128, 20, 130, None, [129, 130], 3),
+    (2, 1, 2, 2, 160, 30, 700, None, [641], 3),
+    (1, 1, 3, 3, 256, 90, 140, None, None, 3),
+    (2, 2, 2, 2, 96, 20, 70, None, [70, 33], 0),
+    (1, 1, 2, 2, 32, 200, 1100, None, None, 0),
+    (2, 2, 2, 2, 104, 200, 600, [1, 1], [5, 577], 0),
+    (1, 1, 1, 1, 248, 65, 1000, None, None, 0),
+]
+
+
+@pytest.mark.parametrize("case", range(len(ATT_WIDTHS)))
+def test_attention_block_shapes(case):
+    batch, contexts, heads, kvh, dim, nq, nkv, index, lens, regions = ATT_WIDTHS[case]
+    q, k, v, kd, vd, qr, kr = _attention_case(200 + case, batch, contexts, heads, kvh, dim, nq, nkv, index, lens, regions)
+    got = _run_attention(q, kd, vd, heads, kvh, dim, index, lens, qr, kr)
+    want, tol = _attention_oracle(q, k, v, heads, kvh, dim, dim ** -0.5, index, lens, qr, kr)
+    _close(got, want, tol, "attention %s" % (ATT_WIDTHS[case],))
+
+
+def test_attention_refuses_tensors_of_another_kind():
+    a = E.Act(torch.zeros((2, 8, 64), dtype=H16, device=DEV), 2, 1, 8, 64)
+    sets = torch.zeros((2, 8), dtype=torch.int32, device=DEV)
+    for kw in (dict(lens=torch.zeros(2, dtype=torch.int32)), dict(lens=_i32([1, 2]).long()), dict(lens=_i32([1])), dict(index=_i32([[0, 1]])),
+               dict(query_regions=sets), dict(query_regions=sets, key_regions=sets[:, ::2]), dict(index=_i32([0, 9, 1, 9])[::2])):
+        with pytest.raises(L.SdmiError):
+            E.cross_attention(a, a, a, 1, **kw)
+    host = E.Act(torch.zeros((2, 8, 64), dtype=H16), 2, 1, 8, 64)
+    for q, k in ((a, host), (host, a), (host, host)):
+        with pytest.raises(L.SdmiError):
+            E.cross_attention(q, k, k, 1)
+    with pytest.raises(L.SdmiError):
+        E.cross_attention(a, a.cols(0, 32), a, 1)
+
+
 # ------------------------------------------------------------------------------------------------------------ adapters
 def _lora_oracle(x, w, a, b, scale, ids, per, groups, bias, residual):
     x, w, a, b = x.double(), w.double(), a.double(), b.double()
@@ -283,6 +319,58 @@ def test_lora(case):
     got = _run_lora(x, w, a, b, scale, ids, bi, res)
     want, tol = _lora_oracle(x, w, a, b, scale, ids, per, groups, bi, res)
     _close(got, want, tol, "lora %s" % ((per, len(ids)) + LORA[case][2:],))
+
+
+LORA_KINDS = [  # what the larger kernels and the ranks beyond their first tile do
+    (1, [i % 3 for i in range(12)], 136, 56, 1, 16, 3, True, True),
+    (4096, [1, 0], 72, 2048, 1, 16, 2, True, False),
+    (4096, [0, -1], 64, 2064, 2, 32, 1, False, True),
+    (2048, [1, 0], 72, 1032, 1, 8, 2, True, True),
+    (1000, [1, 0, 1, -1], 64, 1080, 3, 24, 2, True, False),
+    (2050, [0, 1], 64, 1024, 1, 40, 2, False, True),
+    (4100, [0, 1], 72, 512, 2, 64, 2, True, False),
+    (16, [(i * 7) % 9 - 1 for i in range(256)], 64, 1032, 1, 16, 8, False, True),
+    (1, [(i * i) % 11 for i in range(4100)], 64, 1080, 3, 72, 10, True, False),
+    (65, [1, 0, -1, 1], 328, 40, 1, 256, 2, False, False),
+]
+
+
+@pytest.mark.parametrize("case", range(len(LORA_KINDS)))
+def test_lora_kinds(case):
+    per, ids, k, n, groups, rank, adapters, bias, residual = LORA_KINDS[case]
+    x, w, a, b, scale, bi, res = _lora_case(100 + case, per * len(ids), k, n, groups, rank, adapters, bias, residual)
+    got = _run_lora(x, w, a, b, scale, ids, bi, res)
+    want, tol = _lora_oracle(x, w, a, b, scale, ids, per, groups, bi, res)
+    _close(got, want, tol, "lora %s" % ((per, len(ids)) + LORA_KINDS[case][2:],))
+
+
+@pytest.mark.parametrize("m", [3, 40, 200, 1000])
+def test_lora_one_id_for_any_number_of_rows(m):
+    x, w, a, b, scale, _, _ = _lora_case(9, m, 64, 72, 1, 16, 3, False, False)
+    xd, wd, ad, bd, sd, idd = x.to(DEV), w.to(DEV), a.to(DEV), b.to(DEV), scale.to(DEV), _i32([2])
+    out = torch.empty((m, 72), dtype=H16, device=DEV)
+    ws = torch.empty((m * 16,), dtype=H16, device=DEV)
+    L.call("sdmi_lora_gemm", xd.data_ptr(), 64, wd.data_ptr(), 64, out.data_ptr(), 72, m, 72, 64, 0, 0, 0, ad.data_ptr(), bd.data_ptr(), sd.data_ptr(), 3, 16, 1,
+           idd.data_ptr(), 2 ** 31 - 1, 0, ws.data_ptr(), 2 * ws.numel(), torch.cuda.current_stream().cuda_stream)
+    want, tol = _lora_oracle(x, w, a, b, scale, [2], m, 1, None, None)
+    _close(out, want, tol, "lora, %d rows of one request" % m)
+
+
+def test_lora_refuses_tensors_of_another_kind():
+    x, w, a, b, scale, _, _ = _lora_case(9, 24, 64, 72, 1, 16, 3, False, False)
+    xa, wd, pack = E.Act(x.to(DEV).view(1, 24, 64), 1, 1, 24, 64), w.to(DEV), E.LoraPack(a.to(DEV), b.to(DEV), scale.to(DEV))
+    good = dict(lora=pack, ids=_i32([0, 1]))
+    E.lora_gemm(xa, wd, 72, **good)
+    for kw in (dict(ids=_i32([0] * 5)), dict(ids=_i32([0, 1]).long()), dict(ids=torch.zeros(2, dtype=torch.int32)), dict(ids=_i32([])),
+               dict(lora=E.LoraPack(a, b, scale)), dict(bias=torch.zeros(72, dtype=H16, device=DEV)), dict(bias=torch.zeros(64, device=DEV)),
+               dict(residual=xa), dict(out=xa)):
+        with pytest.raises(L.SdmiError):
+            E.lora_gemm(xa, wd, 72, **{**good, **kw})
+    with pytest.raises(L.SdmiError):
+        E.lora_gemm(xa, wd.t(), 64, **good)
+    for bad in ((a.float(), b, scale), (a, b[:2], scale), (a, b, scale[:2]), (a[:, :12], b, scale), (a, b, scale.double())):
+        with pytest.raises(L.SdmiError):
+            E.LoraPack(*bad)
 
 
 def test_lora_last_id_covers_fewer_rows():

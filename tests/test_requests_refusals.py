@@ -18,7 +18,8 @@ LORA = dict(x=P, ldx=64, w=P, ldw=64, out=P, ldo=64, m=100, n=64, k=64, bias=Non
     (dict(nkv=-1), "shape"), (dict(contexts=0), "contexts"), (dict(contexts=3), "index"), (dict(ldq=120), "stride"), (dict(ldq=132), "multiples"), (dict(ldk=64), "stride"),
     (dict(ldo=66), "multiples"), (dict(ldk=1 << 22), "too large"), (dict(sk=1284), "alignment"), (dict(q=P + 8), "alignment"), (dict(o=P + 4), "alignment"),
     (dict(qr=P), "together"), (dict(kr=P), "together"), (dict(index=P + 2), "alignment"), (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"),
-    (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
+    (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(scale=2e15), "scale"), (dict(nkv=1 << 30), "shape"), (dict(nq=1 << 30), "shape"),
+    (dict(nq=(1 << 30) - 1), "grid"),
 ])
 def test_attention_refuses(change, word):
     with pytest.raises(L.SdmiError, match=word):
@@ -30,7 +31,8 @@ def test_attention_refuses(change, word):
     (dict(rank=12), "shape"), (dict(rank=0), "shape"), (dict(rank=264), "shape"), (dict(groups=0), "shape"), (dict(groups=3), "shape"), (dict(adapters=0), "adapters"),
     (dict(rows=0), "rows per id"), (dict(flags=8), "flags"), (dict(flags=1), "bias"), (dict(flags=4), "residual"), (dict(flags=4, residual=P, ldr=32), "residual"),
     (dict(ldx=32), "strides"), (dict(ldw=68), "strides"), (dict(ldo=60), "strides"), (dict(ldx=1 << 22), "too large"), (dict(x=P + 8), "alignment"),
-    (dict(flags=4, residual=P + 8, ldr=64), "alignment"), (dict(ids=P + 2), "alignment"), (dict(ws_bytes=8), "workspace"),
+    (dict(flags=4, residual=P + 8, ldr=64), "alignment"), (dict(ids=P + 2), "alignment"), (dict(ws_bytes=8), "workspace"), (dict(m=1 << 30), "shape"),
+    (dict(n=1 << 30, ldo=1 << 30), "shape"),
 ])
 def test_lora_refuses(change, word):
     with pytest.raises(L.SdmiError, match=word):
@@ -45,3 +47,6 @@ def test_workspace_sizes():
     assert lib.sdmi_lora_gemm_ws_bytes(100, 96, 64, 16, 3, 1) >= 100 * 48 * 2
     assert lib.sdmi_lora_gemm_ws_bytes(100, 96, 64, 12, 3, 1) == 0
     assert lib.sdmi_lora_gemm_ws_bytes(1, 96, 64, 16, 1, 1) == 0                       # one launch: nothing to hand over
+    for m in (1, 40, 100, 5000):                                                       # one id for all rows, however it is said
+        for rank in (16, 64):
+            assert lib.sdmi_lora_gemm_ws_bytes(m, 96, 64, rank, 1, 2 ** 31 - 1) == lib.sdmi_lora_gemm_ws_bytes(m, 96, 64, rank, 1, m)
