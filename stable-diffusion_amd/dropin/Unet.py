@@ -34,6 +34,7 @@ class TimeEmb(object):
 class Unet(nn.Module):
     def __init__(self):
         super().__init__()
+        self.adapters = None        # conditioning.AdapterSet (set_adapters)
         self.emb_channels = MODEL_CH
         temb = MODEL_CH * 4
         self.time_embed = nn.Sequential(nn.Linear(MODEL_CH, temb), nn.SiLU(), nn.Linear(temb, temb))
@@ -83,10 +84,20 @@ class Unet(nn.Module):
                     if isinstance(m, SpatialTransformer):
                         yield m.transformer_blocks[0].attn2
 
+    def set_adapters(self, adapters):
+        """adapters: a conditioning.AdapterSet built for this model, or None to switch them off.  AdapterSet.select(ids) then
+        chooses for each batch."""
+        if adapters is not None and not {id(m) for m, _ in adapters.layers} <= {id(m) for m in self.modules()}:
+            raise E.L.SdmiError("Unet.set_adapters: this set was built for another model")
+        if self.adapters is not None:
+            self.adapters.detach()
+        self.adapters = adapters.attach() if adapters is not None else None
+
     @torch.no_grad()
     def precompute_context(self, context):
         """Project the (2b, 77, 1024) text context through every cross-attention to_k / to_v once.  The result can be
-        passed as `context=` to forward() for every DDIM step of the same prompt (step-invariant hoisting)."""
+        passed as `context=` to forward() for every DDIM step of the same prompt (step-invariant hoisting).  context: that
+        tensor, or conditioning.EncoderStates (forward() takes either as well)."""
         if isinstance(context, list):
             context = context[0]
         return ContextKV(list(self._cross_attn_modules()), context)
@@ -224,8 +235,8 @@ class Unet(nn.Module):
             raise E.L.SdmiError("Unet.forward: context=None - every cross-attention's to_k / to_v is Linear(1024, inner) and "
                                 "cannot project the tokens themselves (the reference fails in to_k for the same call)")
         ctx = context if isinstance(context, ContextKV) else self.precompute_context(context)
-        if ctx._shape[0] != st.n:
-            raise E.L.SdmiError("Unet.forward: context holds %d samples, x holds %d" % (ctx._shape[0], st.n))
+        if not ctx.serves(st.n):
+            raise E.L.SdmiError("Unet.forward: context holds %d samples, x holds %d" % (ctx._shape[0] if ctx.states is None else ctx.states.batch, st.n))
         emb, ldrb, cat, skip_c = st.emb, st.ldrb, st.cat, st.skip_c
         nin = len(self.input_blocks)
         c1_of = lambda k: cat[k].c - skip_c[k]

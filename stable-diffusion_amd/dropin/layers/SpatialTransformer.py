@@ -1,11 +1,18 @@
 """Drop-in for the reference's layers/SpatialTransformer.py: same module tree and parameter names
 (SURVEY.md 8(b)); tokens stay (B, HW, C) bf16 views end to end, q/k/v projections are fused into one GEMM,
 attention is the flash kernel of csrc/attention.hip reading heads in place, residual adds / biases / GEGLU live in
-GEMM epilogues.  No xformers, no einops, no permutes."""
+GEMM epilogues.  No xformers, no einops, no permutes.
+
+Beyond the reference: a context may be stable_diffusion_amd.conditioning.EncoderStates (states of another length for each
+prompt, shared by samples, with regions), and an attention layer may carry low-rank adapters of the batch's samples
+(`adapters`, a conditioning.LayerAdapters)."""
+import math
+
 import torch
 from torch import nn
 
 from stable_diffusion_amd import engine as E
+from stable_diffusion_amd.conditioning import EncoderStates
 
 
 def zero_module(module):
@@ -17,35 +24,63 @@ def zero_module(module):
 class ContextKV(object):
     """Pre-projected text context: the to_k|to_v outputs of every cross-attention layer, computed by ONE stacked GEMM
     (they depend only on the prompt, not on the latent or the timestep: 32 Linears per UNet step in the reference,
-    layers/SpatialTransformer.py:73-74).  `kv[id(attn_module)]` is that layer's (B, 77, 2*inner) view."""
+    layers/SpatialTransformer.py:73-74).  `kv[id(attn_module)]` is that layer's (B, 77, 2*inner) view.
+    states: the EncoderStates the tokens came from (lengths, contexts and regions for the attention), None for plain tokens.
+    Layers whose to_k / to_v have adapters are projected again with them, into the same columns."""
 
     def __init__(self, attn_modules, context):
         self._modules = list(attn_modules)
         self._ws = tuple(w for m in self._modules for w in (m.to_k.weight, m.to_v.weight))
         self._ntot = sum(w.shape[0] for w in self._ws)
         self._allkv = None
+        self.states = context.clone() if isinstance(context, EncoderStates) else None
+        self.kv = {}
         self.update(context)
-        self.kv, off = {}, 0
-        for m in self._modules:
-            n2 = m.to_k.weight.shape[0] + m.to_v.weight.shape[0]
-            self.kv[id(m)] = self._allkv.cols(off, n2)
-            off += n2
 
     def update(self, context):
         """Project a new prompt INTO THE SAME BUFFERS (same batch and token count): a HIP graph captured over a forward
         that read this object stays valid, which is how the sampler reuses one captured step across images."""
+        if isinstance(context, EncoderStates) != (self.states is not None):
+            raise E.L.SdmiError("ContextKV.update: plain tokens and EncoderStates do not take each other's place")
+        if self.states is not None:
+            context = self.states.copy_(context).tokens
         ctx = context if isinstance(context, E.Act) else E.tokens_from_f32(context)
         if self._allkv is not None:
             assert (ctx.n, ctx.h * ctx.w) == self._shape, "ContextKV.update: batch / token count changed"
         self._shape = (ctx.n, ctx.h * ctx.w)
         self._allkv = E.gemm(ctx, E.packed_linear(self._ws), self._ntot, out=self._allkv)
+        off = 0
+        for m in self._modules:
+            n2 = m.to_k.weight.shape[0] + m.to_v.weight.shape[0]
+            if id(m) not in self.kv:
+                self.kv[id(m)] = self._allkv.cols(off, n2)
+            off += n2
+            if m.adapters is not None and m.adapters.pack("kv") is not None:
+                m.project_context(ctx, self.shared, out=self.kv[id(m)])
         return self
+
+    @property
+    def shared(self):
+        return self.states is not None and (self.states.index is not None or self.states.batch != self.states.tokens.shape[0])
+
+    def serves(self, n):
+        """Whether a batch of n samples can read this context."""
+        return (self._shape[0] if self.states is None else self.states.batch) in (n, None)
+
+
+class _StatesIn(object):
+    """EncoderStates entering a single layer: its tokens as an activation beside them."""
+
+    def __init__(self, states):
+        self.states, self.act = states, E.tokens_from_f32(states.tokens)
+
+    shared = ContextKV.shared
 
 
 def _as_ctx(context):
     if context is None or isinstance(context, (E.Act, ContextKV)):
         return context
-    return E.tokens_from_f32(context)
+    return _StatesIn(context) if isinstance(context, EncoderStates) else E.tokens_from_f32(context)
 
 
 class GEGLU(nn.Module):
@@ -102,6 +137,28 @@ class MemoryEfficientCrossAttention(nn.Module):
         self.to_v = nn.Linear(context_dim, inner, bias=False)
         self.to_out = nn.Sequential(nn.Linear(inner, query_dim), nn.Dropout(dropout))
         self.attention_op = None
+        self.adapters = None        # conditioning.LayerAdapters (AdapterSet.attach)
+
+    def _pack(self, kind):
+        return None if self.adapters is None else self.adapters.pack(kind)
+
+    def _project(self, a, ln, kind, ws, scales=None):
+        """The stacked projections `ws` of (LayerNorm of) the tokens, with the adapters this layer has for them."""
+        pack = self._pack(kind)
+        n = sum(w.shape[0] for w in ws)
+        if pack is None:
+            return E.gemm_ln(a, ln, ws, scales=scales) if ln is not None else E.gemm(a, E.packed_linear(ws, scales=scales), n)
+        # t = x a^T needs the normalised tokens themselves: the LayerNorm is a launch of its own here
+        x = E.layernorm(a, ln.weight, ln.bias, ln.eps) if ln is not None else a
+        return E.lora_gemm(x, E.packed_linear(ws, scales=scales), n, pack, self.adapters.owner.ids_for(a.n))
+
+    def project_context(self, ctx, shared=False, out=None):
+        """to_k | to_v of the context's tokens, with the adapters this layer has for them."""
+        ws, pack = (self.to_k.weight, self.to_v.weight), self._pack("kv")
+        n = ws[0].shape[0] + ws[1].shape[0]
+        if pack is None:
+            return E.gemm(ctx, E.packed_linear(ws), n, out=out)
+        return E.lora_gemm(ctx, E.packed_linear(ws), n, pack, self.adapters.owner.ids_for_contexts(ctx.n, shared), out=out)
 
     def run(self, a, context=None, residual=None, ln=None, rowstats=False):
         """ln: the LayerNorm module in front of this layer (BasicTransformerBlock.norm1/2): `a` is then the UN-normalised
@@ -110,28 +167,36 @@ class MemoryEfficientCrossAttention(nn.Module):
         inner = 64 * self.heads
         # the query projection carries 1/8 * log2(e), folded into to_q before its rounding to 16 bits: scores leave the
         # QK^T MFMAs in the log2 domain (sdmi_attention_log2q)
-        qs = lambda ws: (E.Q_LOG2_SCALE,) + (None,) * (len(ws) - 1)
-        proj = (lambda ws: E.gemm_ln(a, ln, ws, scales=qs(ws))) if ln is not None else \
-               (lambda ws: E.gemm(a, E.packed_linear(ws, scales=qs(ws)), sum(w.shape[0] for w in ws)))
+        sc = E.Q_LOG2_SCALE
+        states, o = None, None
         if context is None:          # self-attention: one fused q|k|v GEMM
             if self.to_k.weight.shape[1] != a.c:
                 raise E.L.SdmiError("attention without context: to_k expects %d channels, the tokens have %d (the reference "
                                     "fails in to_k as well)" % (self.to_k.weight.shape[1], a.c))
-            qkv = proj((self.to_q.weight, self.to_k.weight, self.to_v.weight))
+            qkv = self._project(a, ln, "qkv", (self.to_q.weight, self.to_k.weight, self.to_v.weight), (sc, None, None))
             q, k, v = qkv.cols(0, inner), qkv.cols(inner, inner), qkv.cols(2 * inner, inner)
-            o = None
         else:
             if isinstance(context, ContextKV):
-                kv = context.kv[id(self)]
+                kv, states = context.kv[id(self)], context.states
             else:
-                kv = E.gemm(context, E.packed_linear((self.to_k.weight, self.to_v.weight)), 2 * inner)
+                shared = False
+                if isinstance(context, _StatesIn):
+                    states, shared, context = context.states, context.shared, context.act
+                kv = self.project_context(context, shared)
             k, v = kv.cols(0, inner), kv.cols(inner, inner)
             # LayerNorm + to_q inside the attention kernel where the engine offers it (one launch less)
-            o = E.cross_attention_lnq(a, ln, self.to_q.weight, k, v, self.heads) if ln is not None else None
-            q = proj((self.to_q.weight,)) if o is None else None
-        if o is None:
+            if ln is not None and states is None and self._pack("q") is None:
+                o = E.cross_attention_lnq(a, ln, self.to_q.weight, k, v, self.heads)
+            q = self._project(a, ln, "q", (self.to_q.weight,), (sc,)) if o is None else None
+        if states is not None:       # q carries log2(e) / 8 already
+            o = E.cross_attention(q, k, v, self.heads, scale=math.log(2.0), index=states.index, lens=states.lens, query_regions=states.regions(a.h, a.w),
+                                  key_regions=states.key_regions)
+        elif o is None:
             o = E.attention(q, k, v, self.heads, log2q=True)
         lin = self.to_out[0]
+        pack = self._pack("out")
+        if pack is not None:
+            return E.lora_gemm(o, E.packed_linear((lin.weight,)), lin.weight.shape[0], pack, self.adapters.owner.ids_for(a.n), bias=lin.bias, residual=residual)
         return E.gemm(o, E.packed_linear((lin.weight,)), lin.weight.shape[0], bias=lin.bias, residual=residual, rowstats=rowstats)
 
     def forward(self, x, context=None, mask=None):

@@ -67,6 +67,12 @@ class Sampler(object):
         graphs and cached tables are keyed on it, so they are rebuilt instead of replaying stale packed weights."""
         return tuple((p.data_ptr(), p._version) for p in module.parameters()) if module is not None else ()
 
+    def _adapter_key(self):
+        """What of the adapters a captured step has baked in: the set, which is kept alive beside the graph so that its id stays
+        its own, and the length of the ids, which says where they live."""
+        ad = getattr(self.unet, "adapters", None)
+        return None if ad is None else (id(ad), 0 if ad.ids is None else ad.ids.numel())
+
     def _time_tables(self, steps, bc, dev):
         key = (tuple(int(s) for s in steps), bc, str(dev), self._usig)
         if getattr(self, "_tt_key", None) != key:
@@ -85,15 +91,24 @@ class Sampler(object):
             self._emb_cur = cur = TimeEmb(torch.empty_like(table[0]))
         return cur
 
-    def make_context(self, uncond, cond):
+    def make_context(self, uncond, cond, batch=None):
         """Step-invariant text-context K/V of the CFG batch [uncond | cond] (one object per half when dual_stream).
         The objects are owned by the sampler and refilled IN PLACE for every prompt of the same batch size: the captured
-        UNet step reads their buffers, so they must not move between images."""
-        key = (tuple(uncond.shape), str(uncond.device), self.dual_stream, self.cfg_group is not None)
+        UNet step reads their buffers, so they must not move between images.  Either side may be EncoderStates; batch: samples
+        of a half, for states that say nothing of it."""
+        from .conditioning import EncoderStates
+        states = isinstance(cond, EncoderStates) or isinstance(uncond, EncoderStates)
+        if states:
+            cond, uncond = EncoderStates.of(cond), EncoderStates.of(uncond)
+        sig = lambda v: v.signature() if states else (tuple(v.shape), str(v.device))
+        key = (sig(uncond), sig(cond), self.dual_stream, self.cfg_group is not None, batch if states else None)
+        own = (lambda v: v) if states else (lambda v: v.contiguous())
         if self.cfg_group is not None:
-            halves = ((uncond, cond)[self.cfg_role].contiguous(),)      # this rank's half only
+            halves = (own((uncond, cond)[self.cfg_role]),)      # this rank's half only
+        elif self.dual_stream:
+            halves = (own(uncond), own(cond))
         else:
-            halves = (uncond.contiguous(), cond.contiguous()) if self.dual_stream else (torch.cat([uncond, cond]).contiguous(),)
+            halves = (EncoderStates.cat(uncond, cond, batch) if states else torch.cat([uncond, cond]).contiguous(),)
         if getattr(self, "_cc_key", None) != key:
             self._cc = tuple(self.unet.precompute_context(h) for h in halves)
             self._cc_key = key
@@ -170,7 +185,7 @@ class Sampler(object):
         # the graph is valid while the buffers it read are alive and in place: key on the objects that own them (the
         # sampler keeps xc, the TimeEmb row and the ContextKV alive; a caller's own buffers must outlive the graph)
         key = (xc.data_ptr(), t_buf.table.data_ptr() if hasattr(t_buf, "table") else t_buf.data_ptr(), id(cc), tuple(xc.shape), same_halves,
-               getattr(self, "_usig", None) or self.weights_signature(self.unet))
+               getattr(self, "_usig", None) or self.weights_signature(self.unet), self._adapter_key())
         if self._gkey != key:
             self._unet_eval(xc, t_buf, cc, same_halves)         # warm-up: weight pre-pack, allocator pools
             torch.cuda.synchronize()
@@ -179,15 +194,15 @@ class Sampler(object):
             # multi-GPU run polling its events) must not invalidate it
             with torch.cuda.graph(g, capture_error_mode="thread_local"):
                 out = self._unet_eval(xc, t_buf, cc, same_halves)
-            self._graph, self._gout, self._gkey, self._gkeep = g, out, key, (xc, t_buf, cc)
+            self._graph, self._gout, self._gkey, self._gkeep = g, out, key, (xc, t_buf, cc, getattr(self.unet, "adapters", None))
         self._graph.replay()
         return self._gout
 
     @torch.no_grad()
     def sample(self, num_ddim_timesteps, cond, uncond, c_concat, x_T, noises, scale, eta=1.0, temperature=1.0,
                decode=True, use_graph=False, trace=None):
-        """cond/uncond (b,77,1024), c_concat (b,5,h,w), x_T (b,4,h,w), noises: sequence of (b,4,h,w) in loop order;
-        all fp32 cuda tensors.  Returns (latent, uint8 images (b,H,W,3) or None)."""
+        """cond/uncond (b,77,1024), c_concat (b,5,h,w), x_T (b,4,h,w), noises: sequence of (b,4,h,w) in loop order; all fp32
+        cuda tensors.  cond and uncond may be conditioning.EncoderStates; adapters: Unet.set_adapters and AdapterSet.select.  Returns (latent, uint8 images (b,H,W,3) or None)."""
         ts, a_t, a_prev, sig, s1m = ddim_schedule(num_ddim_timesteps, eta)
         total = ts.shape[0]
         self._usig = self.weights_signature(self.unet)      # once per image: keys the captured step and the cached tables
@@ -199,7 +214,7 @@ class Sampler(object):
         xc[:b, 4:] = c_concat
         xc[b:, 4:] = c_concat
         # text-context K/V projections do not depend on the step: project once per prompt
-        cc = self.make_context(uncond, cond)
+        cc = self.make_context(uncond, cond, b)
         # the timestep-embedding MLPs depend on t only: one table per schedule step, computed once per schedule and kept
         # across images; a step copies its row into the static buffer the (graph-captured) UNet reads
         emb_table = self._time_tables(np.flip(ts), 2 * b, dev)
