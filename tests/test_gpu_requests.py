@@ -332,6 +332,11 @@ LORA_KINDS = [  # what the larger kernels and the ranks beyond their first tile 
     (16, [(i * 7) % 9 - 1 for i in range(256)], 64, 1032, 1, 16, 8, False, True),
     (1, [(i * i) % 11 for i in range(4100)], 64, 1080, 3, 72, 10, True, False),
     (65, [1, 0, -1, 1], 328, 40, 1, 256, 2, False, False),
+    (33, [(i * 5) % 7 - 1 for i in range(130)], 72, 136, 1, 16, 6, False, True),        # rows taken in the order of their adapters, past one chunk of them
+    (1, [(i * 389) % 1100 for i in range(300)], 64, 72, 1, 8, 1100, True, False),       # too many adapters to order
+    (1, [(i * 389) % 1023 for i in range(300)], 64, 72, 1, 8, 1023, True, False),
+    (1, [-1, 7] * 40, 64, 72, 1, 8, 7, True, True),
+    (1, [2] * 65 + [0] * 63 + [1] + [2] * 64, 64, 80, 2, 24, 3, False, False),
 ]
 
 
@@ -349,7 +354,7 @@ def test_lora_one_id_for_any_number_of_rows(m):
     x, w, a, b, scale, _, _ = _lora_case(9, m, 64, 72, 1, 16, 3, False, False)
     xd, wd, ad, bd, sd, idd = x.to(DEV), w.to(DEV), a.to(DEV), b.to(DEV), scale.to(DEV), _i32([2])
     out = torch.empty((m, 72), dtype=H16, device=DEV)
-    ws = torch.empty((m * 16,), dtype=H16, device=DEV)
+    ws = torch.empty((max(L.load().sdmi_lora_gemm_ws_bytes(m, 72, 64, 16, 1, 2 ** 31 - 1), 2) // 2,), dtype=H16, device=DEV)
     L.call("sdmi_lora_gemm", xd.data_ptr(), 64, wd.data_ptr(), 64, out.data_ptr(), 72, m, 72, 64, 0, 0, 0, ad.data_ptr(), bd.data_ptr(), sd.data_ptr(), 3, 16, 1,
            idd.data_ptr(), 2 ** 31 - 1, 0, ws.data_ptr(), 2 * ws.numel(), torch.cuda.current_stream().cuda_stream)
     want, tol = _lora_oracle(x, w, a, b, scale, [2], m, 1, None, None)
@@ -378,7 +383,7 @@ def test_lora_last_id_covers_fewer_rows():
     ids = [2, 0, 1]                                         # 64 + 64 + 22 rows
     xd, wd, ad, bd, sd, idd = x.to(DEV), w.to(DEV), a.to(DEV), b.to(DEV), scale.to(DEV), _i32(ids)
     out = torch.full((152, 80), 5.0, dtype=H16, device=DEV)
-    ws = torch.empty((150 * 16,), dtype=H16, device=DEV)
+    ws = torch.empty((max(L.load().sdmi_lora_gemm_ws_bytes(150, 72, 64, 16, 1, 64), 2) // 2,), dtype=H16, device=DEV)
     L.call("sdmi_lora_gemm", xd.data_ptr(), 64, wd.data_ptr(), 64, out.data_ptr(), 80, 150, 72, 64, 0, 0, 0, ad.data_ptr(), bd.data_ptr(), sd.data_ptr(), 3, 16, 1,
            idd.data_ptr(), 64, 0, ws.data_ptr(), 2 * ws.numel(), torch.cuda.current_stream().cuda_stream)
     want, tol = _lora_oracle(x, w, a, b, scale, ids, 64, 1, None, None)
