@@ -231,11 +231,11 @@ __global__ __launch_bounds__(512, 1) void lora_shrink_kernel(const LoraParams p)
 // ------------------------------------------------------------------------------------------------------------ up to 64 rows
 // Block: 16 columns x all M <= 16 MT rows; its eight waves take the K-steps in turn, as above: w is read once by the whole grid, x
 // by every block (L2).  The adapters: four lanes share a (row, column) pair and take the dot product of t[m] and b[id][n], rank
-// long, 16 bytes each at a time; the first 32 ranks of both are fetched before the product.  FUSE: the block computes t of its rows
+// long, 16 bytes each at a time; the first 32 ranks of both are fetched before the product, behind the first K-steps' DMA.  FUSE: the block computes t of its rows
 // itself (m * groups * rank <= 64 dot products of length K, one wave each in turn) instead of reading what an earlier launch left.
 template <int MT>
 struct RowsShape {
-  static constexpr int S = 9 / (MT + 1), WAVE = S * (MT + 1) * 2048, bytes = 8 * WAVE;  // the join needs 8 MT KB of it
+  static constexpr int S = MT == 4 ? 2 : 9 / (MT + 1), WAVE = S * (MT + 1) * 2048, bytes = 8 * WAVE;  // the join needs 8 MT KB of it
 };
 template <int MT, bool FUSE>
 __global__ __launch_bounds__(512, 1) void lora_rows_kernel(const LoraParams p) {
@@ -246,6 +246,18 @@ __global__ __launch_bounds__(512, 1) void lora_rows_kernel(const LoraParams p) {
   const int t = threadIdx.x, lane = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6), l15 = lane & 15, lq = lane >> 4, n0 = blockIdx.x * 16;
   // pair x of this lane group: column n0 + c, row x * 8 + (t >> 6)
   const int c = (t >> 2) & 15, piece = t & 3, n = n0 + c, nc = min(n, p.N - 1), g = nc / p.per;
+  const u16* const wb = p.w + (long long)n0 * p.ldw;
+  const unsigned lds = lds_addr_of(smem) + wv * H::WAVE;
+  const u16* const sm = smem + wv * (H::WAVE / 2);
+  auto stage = [&](int k1) {
+#pragma unroll
+    for (int s = 0; s < H::S; ++s) {
+      const int k0 = (k1 + 8 * s) * LBK;
+      lora_panel<2>(wb, p.ldw, p.N - n0, k0, p.K, lds + s * (MT + 1) * 2048, lane);
+      lora_panel<2 * MT>(p.x, p.ldx, p.M, k0, p.K, lds + (s * (MT + 1) + 1) * 2048, lane);
+    }
+  };
+  if (wv < p.nk) stage(wv);  // in flight while the ids and the adapters' rows are fetched
   int id[NP];
   uint4 b0[NP], t0[FUSE ? 1 : NP];
 #pragma unroll
@@ -284,16 +296,7 @@ __global__ __launch_bounds__(512, 1) void lora_rows_kernel(const LoraParams p) {
   f32x4 acc[MT];
 #pragma unroll
   for (int i = 0; i < MT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const u16* const wb = p.w + (long long)n0 * p.ldw;
-  const unsigned lds = lds_addr_of(smem) + wv * H::WAVE;
-  const u16* const sm = smem + wv * (H::WAVE / 2);
-  for (int k1 = wv; k1 < p.nk; k1 += 8 * H::S) {
-#pragma unroll
-    for (int s = 0; s < H::S; ++s) {
-      const int k0 = (k1 + 8 * s) * LBK;
-      lora_panel<2>(wb, p.ldw, p.N - n0, k0, p.K, lds + s * (MT + 1) * 2048, lane);
-      lora_panel<2 * MT>(p.x, p.ldx, p.M, k0, p.K, lds + (s * (MT + 1) + 1) * 2048, lane);
-    }
+  for (int k1 = wv; k1 < p.nk;) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
     for (int s = 0; s < H::S; ++s)
@@ -305,6 +308,8 @@ __global__ __launch_bounds__(512, 1) void lora_rows_kernel(const LoraParams p) {
           acc[i] = MFMA16(wf, *(const hx8*)&sm[(s * (MT + 1) + 1) * 1024 + lora_off(16 * i + l15, lq + 4 * kk)], acc[i], 0, 0, 0);
       }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    k1 += 8 * H::S;
+    if (k1 < p.nk) stage(k1);
   }
   __syncthreads();
   float* const red = (float*)smem;  // [wave][4 i + e][64]: row 16 i + l15, column 4 lq + e

@@ -14,11 +14,10 @@ import torch
 from . import _lib as L
 
 
-
+@functools.lru_cache(maxsize=None)
 def act_dtype():
     """torch dtype of the library's 16-bit storage type (fp16 unless built with -DSDMI_BF16)."""
     return torch.bfloat16 if L.load().sdmi_act_dtype() == 1 else torch.float16
-
 
 
 def _stream():
