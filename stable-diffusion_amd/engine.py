@@ -21,7 +21,7 @@ def act_dtype():
 
 
 def _stream():
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())     # current_stream().cuda_stream without its object: 2.5 -> 0.3 us
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())     # current_stream().cuda_stream without its object: 2.5 -> 0.3 us
 
 
 def _ptr(t):
@@ -572,7 +572,7 @@ def cross_attention_lnq(a, ln_mod, to_q_weight, k, v, heads, out=None):
 
 def _own_device(what, *tensors):
     """The kernels run on the current device's current stream: every tensor has to live there."""
-    cur = torch.cuda.current_device()
+    cur = torch._C._cuda_getDevice()
     for t in tensors:
         if t is not None and t.get_device() != cur:
             raise L.SdmiError("%s: a tensor is on %s, the current device is cuda:%d" % (what, t.device, cur))
@@ -630,15 +630,15 @@ class LoraPack(object):
     __slots__ = ("a", "b", "scale", "adapters", "rank", "groups")
 
     def __init__(self, a, b, scale):
-        h = act_dtype()
-        if a.dim() != 3 or b.dim() != 3 or a.dtype != h or b.dtype != h or not a.is_contiguous() or not b.is_contiguous() or a.shape[0] != b.shape[0] or \
-                b.shape[2] == 0 or a.shape[1] % b.shape[2]:
+        h, sa, sb = act_dtype(), a.shape, b.shape
+        if len(sa) != 3 or len(sb) != 3 or a.dtype is not h or b.dtype is not h or not a.is_contiguous() or not b.is_contiguous() or sa[0] != sb[0] or \
+                sb[2] == 0 or sa[1] % sb[2]:
             raise L.SdmiError("LoraPack: a (adapters, groups * rank, k) and b (adapters, n, rank) are contiguous %s, got %s %s and %s %s" %
                               (h, a.dtype, tuple(a.shape), b.dtype, tuple(b.shape)))
-        if scale.dtype != torch.float32 or tuple(scale.shape) != (a.shape[0],) or not scale.is_contiguous():
+        if scale.dtype is not torch.float32 or scale.shape != (sa[0],) or not scale.is_contiguous():
             raise L.SdmiError("LoraPack: scale is contiguous fp32 (%d,), got %s %s" % (a.shape[0], scale.dtype, tuple(scale.shape)))
         self.a, self.b, self.scale = a, b, scale
-        self.adapters, self.rank, self.groups = a.shape[0], b.shape[2], a.shape[1] // b.shape[2]
+        self.adapters, self.rank, self.groups = sa[0], sb[2], sa[1] // sb[2]
 
 
 def lora_gemm(a, wp, n_out, lora, ids, bias=None, residual=None, out=None):
@@ -654,7 +654,7 @@ def lora_gemm(a, wp, n_out, lora, ids, bias=None, residual=None, out=None):
         res.stats.pop(res.off, None)
         if (res.n * res.hw, res.c) != (m, n_out):
             raise L.SdmiError("lora_gemm: `out` holds %d rows x %d channels, the product has %d x %d" % (res.n * res.hw, res.c, m, n_out))
-    if wp.shape != (n_out, k) or wp.stride(1) != 1 or wp.dtype != a.buf.dtype or lora.a.shape[2] != k or lora.b.shape[1] != n_out:
+    if wp.shape != (n_out, k) or wp.stride(1) != 1 or wp.dtype is not a.buf.dtype or lora.a.shape[2] != k or lora.b.shape[1] != n_out:
         raise L.SdmiError("lora_gemm: weight %s %s, adapters a %s / b %s for %d -> %d channels" %
                           (wp.dtype, tuple(wp.shape), tuple(lora.a.shape), tuple(lora.b.shape), k, n_out))
     flags = rp = rld = 0
