@@ -297,6 +297,15 @@ int sdmi_cross_attention(const void* q, int ldq, int64_t sq, const void* k, int 
                          const int32_t* index, const int32_t* lens, const uint32_t* query_regions, int64_t sqr,
                          const uint32_t* key_regions, int64_t skr, float scale, void* ws, int64_t ws_bytes, void* stream);
 int64_t sdmi_cross_attention_ws_bytes(int batch, int heads, int kv_heads, int dim, int nq, int nkv);
+/*      The same call with its arguments in one block of 8-byte words, for callers whose foreign-function interface pays for each
+ *      argument (29 of them through ctypes cost as much as the launch). */
+typedef struct sdmi_cross_attention_args {
+  const void* q; int64_t ldq, sq; const void* k; int64_t ldk, sk; const void* v; int64_t ldv, sv; void* o; int64_t ldo, so;
+  int64_t batch, contexts, heads, kv_heads, dim, nq, nkv;
+  const int32_t *index, *lens; const uint32_t* query_regions; int64_t sqr; const uint32_t* key_regions; int64_t skr;
+  double scale; void* ws; int64_t ws_bytes; void* stream;
+} sdmi_cross_attention_args;
+int sdmi_cross_attention_packed(const sdmi_cross_attention_args* args);
 
 /* ---- low-rank adapters of many requests beside one shared projection (no counterpart in the reference, whose Linears at
  *      layers/SpatialTransformer.py:62-66 have one set of weights):
@@ -314,6 +323,12 @@ int sdmi_lora_gemm(const void* x, int ldx, const void* w, int ldw, void* out, in
                    const void* residual, int ldr, const void* lora_a, const void* lora_b, const float* lora_scale, int adapters,
                    int rank, int groups, const int32_t* ids, int rows_per_id, uint32_t flags, void* ws, int64_t ws_bytes, void* stream);
 int64_t sdmi_lora_gemm_ws_bytes(int m, int n, int k, int rank, int groups, int rows_per_id);
+typedef struct sdmi_lora_gemm_args {  /* as sdmi_cross_attention_args */
+  const void* x; int64_t ldx; const void* w; int64_t ldw; void* out; int64_t ldo, m, n, k; const float* bias; const void* residual;
+  int64_t ldr; const void *lora_a, *lora_b; const float* lora_scale; int64_t adapters, rank, groups; const int32_t* ids;
+  int64_t rows_per_id, flags; void* ws; int64_t ws_bytes; void* stream;
+} sdmi_lora_gemm_args;
+int sdmi_lora_gemm_packed(const sdmi_lora_gemm_args* args);
 
 /* ---- fused flash attention, ONE head of dim 512: the VAE mid block's attention (layers/SpatialTransformer.py:132-161,
  *      xformers.ops.memory_efficient_attention on (B, HW, 512)) without an N x N score buffer.  q/k/v/o are h16 token-major

@@ -5,6 +5,7 @@ PyTorch / CPU fallback (a silent fallback would void every parity claim).
 """
 import ctypes as C
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("SDMI_LIB_PATH") or os.path.join(_HERE, "libsdmi355.so")   # env: A/B another build of the library
@@ -30,6 +31,10 @@ class EpilogueExt(C.Structure):
 _vp, _i, _i64, _f, _u32 = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_uint32
 
 # name -> (restype, argtypes); mirrors include/sdmi.h declaration by declaration
+# the blocks of 8-byte words that the *_packed entry points take (sdmi_cross_attention_args, sdmi_lora_gemm_args)
+CROSS_ATTENTION_ARGS = struct.Struct("QqqQqqQqqQqq7qQQQqQqdQqQ")
+LORA_GEMM_ARGS = struct.Struct("QqQqQ4qQQqQQQ3qQ2qQqQ")
+
 PROTOTYPES = {
     "sdmi_version": (_i, []),
     "sdmi_act_dtype": (_i, []),
@@ -77,8 +82,10 @@ PROTOTYPES = {
     "sdmi_cross_attention_lnq": (_i, [_vp, _i, _i64, _i, _vp, _i, _vp, _vp, _vp, _i, _f, _vp, _i, _i64, _vp, _i, _i64, _vp, _i, _i64, _i, _i, _i, _i, _vp]),
     "sdmi_cross_attention": (_i, [_vp, _i, _i64, _vp, _i, _i64, _vp, _i, _i64, _vp, _i, _i64, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _i64, _vp, _i64, _f, _vp, _i64, _vp]),
     "sdmi_cross_attention_ws_bytes": (_i64, [_i, _i, _i, _i, _i, _i]),
+    "sdmi_cross_attention_packed": (_i, [C.c_char_p]),      # CROSS_ATTENTION_ARGS.pack(...)
     "sdmi_lora_gemm": (_i, [_vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _vp, _i, _u32, _vp, _i64, _vp]),
     "sdmi_lora_gemm_ws_bytes": (_i64, [_i, _i, _i, _i, _i, _i]),
+    "sdmi_lora_gemm_packed": (_i, [C.c_char_p]),            # LORA_GEMM_ARGS.pack(...)
     "sdmi_inpaint_prepare": (_i, [_vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _i64, _vp]),
     "sdmi_posterior_sample": (_i, [_vp, _vp, _f, _vp, _i64, _i, _i, _vp]),
     "sdmi_attention_d512": (_i, [_vp, _i, _i64, _vp, _i, _i64, _vp, _i, _i64, _vp, _i, _i64, _i, _i, _f, _vp]),

@@ -77,6 +77,9 @@ static inline int sdmi_opt(SdmiOpt id) { return g_sdmi_opt[id]; }
     }                                      \
   } while (0)
 
+// a 64-bit argument that an `int` one has to hold
+static inline bool sdmi_fits_int(int64_t v) { return v >= INT32_MIN && v <= INT32_MAX; }
+
 __device__ __forceinline__ float h2f(u16 v) { return (float)__builtin_bit_cast(h16, v); }
 __device__ __forceinline__ h16 f2h16(float f) {
 #ifdef SDMI_BF16

@@ -797,3 +797,12 @@ extern "C" int sdmi_lora_gemm(const void* x, int ldx, const void* w, int ldw, vo
   if (pl.kind == LORA_ROWS) return lora_rows_launch(p, false, st);
   return pl.bm == 128 ? lora_tiles_launch<128, 2>(p, pl.kind, st) : lora_tiles_launch<64, 3>(p, pl.kind, st);
 }
+
+extern "C" int sdmi_lora_gemm_packed(const sdmi_lora_gemm_args* a) {
+  SDMI_REQUIRE(a, "lora_gemm: null pointer");
+  SDMI_REQUIRE(sdmi_fits_int(a->ldx) && sdmi_fits_int(a->ldw) && sdmi_fits_int(a->ldo) && sdmi_fits_int(a->m) && sdmi_fits_int(a->n) && sdmi_fits_int(a->k) && sdmi_fits_int(a->ldr) &&
+                   sdmi_fits_int(a->adapters) && sdmi_fits_int(a->rank) && sdmi_fits_int(a->groups) && sdmi_fits_int(a->rows_per_id) && a->flags >= 0 && a->flags <= 0xffffffffll,
+               "lora_gemm: bad shape (a size or row stride past 32 bits)");
+  return sdmi_lora_gemm(a->x, (int)a->ldx, a->w, (int)a->ldw, a->out, (int)a->ldo, (int)a->m, (int)a->n, (int)a->k, a->bias, a->residual, (int)a->ldr, a->lora_a, a->lora_b,
+                        a->lora_scale, (int)a->adapters, (int)a->rank, (int)a->groups, a->ids, (int)a->rows_per_id, (uint32_t)a->flags, a->ws, a->ws_bytes, a->stream);
+}

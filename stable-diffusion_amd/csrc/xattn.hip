@@ -423,3 +423,13 @@ extern "C" int sdmi_cross_attention(const void* q, int ldq, int64_t sq, const vo
   hipLaunchKernelGGL(xattn_join_kernel, dim3((unsigned)((prows + 3) / 4)), dim3(256), 0, st, p, (long long)prows);
   return sdmi_check_launch("cross_attention (join)");
 }
+
+extern "C" int sdmi_cross_attention_packed(const sdmi_cross_attention_args* a) {
+  SDMI_REQUIRE(a, "cross_attention: null pointer");
+  SDMI_REQUIRE(sdmi_fits_int(a->ldq) && sdmi_fits_int(a->ldk) && sdmi_fits_int(a->ldv) && sdmi_fits_int(a->ldo) && sdmi_fits_int(a->batch) && sdmi_fits_int(a->contexts) &&
+                   sdmi_fits_int(a->heads) && sdmi_fits_int(a->kv_heads) && sdmi_fits_int(a->dim) && sdmi_fits_int(a->nq) && sdmi_fits_int(a->nkv),
+               "cross_attention: bad shape (a size or row stride past 32 bits)");
+  return sdmi_cross_attention(a->q, (int)a->ldq, a->sq, a->k, (int)a->ldk, a->sk, a->v, (int)a->ldv, a->sv, a->o, (int)a->ldo, a->so, (int)a->batch, (int)a->contexts,
+                              (int)a->heads, (int)a->kv_heads, (int)a->dim, (int)a->nq, (int)a->nkv, a->index, a->lens, a->query_regions, a->sqr, a->key_regions, a->skr,
+                              (float)a->scale, a->ws, a->ws_bytes, a->stream);
+}

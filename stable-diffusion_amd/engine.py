@@ -579,8 +579,6 @@ def _own_device(what, *tensors):
 
 
 def _int32(t, shape, what):
-    if t is None:
-        return 0
     if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous():
         raise L.SdmiError("%s: expected contiguous int32 %s, got %s %s" % (what, tuple(shape), t.dtype, tuple(t.shape)))
     return t.data_ptr()
@@ -601,8 +599,10 @@ def cross_attention(q, k, v, heads, kv_heads=None, dim=64, scale=None, index=Non
     A row that sees no key is 0."""
     kv_heads = heads if kv_heads is None else kv_heads
     b, nq, n, nkv, wq, wk = q.n, q.h * q.w, k.n, k.h * k.w, heads * dim, kv_heads * dim
+    qp, kp, vp = q.ptr, k.ptr, v.ptr
+    qb, kb, vb = q.buf, k.buf, v.buf
     if out is None:
-        o = new_act(b, q.h, q.w, wq, q.buf.device)
+        o = Act(qb.new_empty((b, nq, wq)), b, q.h, q.w, wq)
     else:
         o = out
         o.rstats = o.normed = None          # whatever an earlier producer left is stale now
@@ -610,17 +610,20 @@ def cross_attention(q, k, v, heads, kv_heads=None, dim=64, scale=None, index=Non
     if q.c != wq or k.c != wk or v.c != wk or v.n != n or v.h * v.w != nkv or o.n != b or o.h * o.w != nq or o.c != wq:
         raise L.SdmiError("cross_attention: q (%d,%d,%d) / k (%d,%d,%d) / v (%d,%d,%d) / out (%d,%d,%d) do not match %d heads on %d key heads of %d" %
                           (b, nq, q.c, n, nkv, k.c, v.n, v.hw, v.c, o.n, o.hw, o.c, heads, kv_heads, dim))
-    qb, kb, vb, ob = q.buf, k.buf, v.buf, o.buf
+    ob, h = o.buf, act_dtype()
+    if qb.dtype is not h or kb.dtype is not h or vb.dtype is not h or ob.dtype is not h:
+        raise L.SdmiError("cross_attention: q %s, k %s, v %s, out %s: the kernels take %s" % (qb.dtype, kb.dtype, vb.dtype, ob.dtype, h))
     _own_device("cross_attention", qb, kb, vb, ob, index, lens, query_regions, key_regions)
     need = _ws_need("sdmi_cross_attention_ws_bytes", b, heads, kv_heads, dim, nq, nkv)
-    ws = torch.empty((need,), dtype=torch.uint8, device=qb.device) if need else None     # the call's own: two graphs never share it
+    ws = qb.new_empty(((need + 1) // 2,)) if need else None     # the call's own: two graphs never share it
     ldq, ldk, ldo = qb.shape[-1], kb.shape[-1], ob.shape[-1]
     ldv = ldk if vb is kb else vb.shape[-1]
-    L.call("sdmi_cross_attention", q.ptr, ldq, nq * ldq, kb.data_ptr() + 2 * k.off, ldk, nkv * ldk, vb.data_ptr() + 2 * v.off, ldv,
-           nkv * ldv, ob.data_ptr() + 2 * o.off, ldo, nq * ldo, b, n, heads, kv_heads, dim, nq, nkv,
-           _int32(index, (b,), "cross_attention: index"), _int32(lens, (n,), "cross_attention: lens"),
-           _int32(query_regions, (b, nq), "cross_attention: query_regions"), nq, _int32(key_regions, (n, nkv), "cross_attention: key_regions"), nkv,
-           dim ** -0.5 if scale is None else float(scale), ws.data_ptr() if need else 0, need, _stream())
+    L.call("sdmi_cross_attention_packed", L.CROSS_ATTENTION_ARGS.pack(
+        qp, ldq, nq * ldq, kp, ldk, nkv * ldk, vp, ldv, nkv * ldv, ob.data_ptr() + 2 * o.off, ldo, nq * ldo, b, n, heads, kv_heads, dim, nq, nkv,
+        0 if index is None else _int32(index, (b,), "cross_attention: index"), 0 if lens is None else _int32(lens, (n,), "cross_attention: lens"),
+        0 if query_regions is None else _int32(query_regions, (b, nq), "cross_attention: query_regions"), nq,
+        0 if key_regions is None else _int32(key_regions, (n, nkv), "cross_attention: key_regions"), nkv,
+        dim ** -0.5 if scale is None else scale, ws.data_ptr() if need else 0, need, _stream()))
     return o
 
 
@@ -645,18 +648,19 @@ def lora_gemm(a, wp, n_out, lora, ids, bias=None, residual=None, out=None):
     """Token GEMM with a low-rank adapter per request (sdmi_lora_gemm): rows = n*hw of `a`, W packed [n_out][a.c], lora: LoraPack.
     ids: int32 device tensor whose length divides the rows: entry i is the adapter of rows [i * rows / len(ids), ...), anything
     outside [0, adapters) for none; read by the kernel (a captured graph sees later contents)."""
+    ap, ab = a.ptr, a.buf
     m, k, nid = a.n * a.h * a.w, a.c, ids.numel()
     if out is None:
-        res = new_act(a.n, a.h, a.w, n_out, a.buf.device)
+        res = Act(ab.new_empty((a.n, a.h * a.w, n_out)), a.n, a.h, a.w, n_out)
     else:
         res = out
         res.rstats = res.normed = None      # whatever an earlier producer left is stale now
         res.stats.pop(res.off, None)
         if (res.n * res.hw, res.c) != (m, n_out):
             raise L.SdmiError("lora_gemm: `out` holds %d rows x %d channels, the product has %d x %d" % (res.n * res.hw, res.c, m, n_out))
-    if wp.shape != (n_out, k) or wp.stride(1) != 1 or wp.dtype is not a.buf.dtype or lora.a.shape[2] != k or lora.b.shape[1] != n_out:
-        raise L.SdmiError("lora_gemm: weight %s %s, adapters a %s / b %s for %d -> %d channels" %
-                          (wp.dtype, tuple(wp.shape), tuple(lora.a.shape), tuple(lora.b.shape), k, n_out))
+    if wp.shape != (n_out, k) or wp.stride(1) != 1 or wp.dtype is not lora.a.dtype or ab.dtype is not lora.a.dtype or lora.a.shape[2] != k or lora.b.shape[1] != n_out:
+        raise L.SdmiError("lora_gemm: tokens %s, weight %s %s, adapters %s a %s / b %s for %d -> %d channels" %
+                          (ab.dtype, wp.dtype, tuple(wp.shape), lora.a.dtype, tuple(lora.a.shape), tuple(lora.b.shape), k, n_out))
     flags = rp = rld = 0
     if residual is not None:
         if (residual.n * residual.hw, residual.c) != (m, n_out):
@@ -669,13 +673,14 @@ def lora_gemm(a, wp, n_out, lora, ids, bias=None, residual=None, out=None):
     ip = _int32(ids, (nid,), "lora_gemm: ids")
     if nid == 0 or m % nid:
         raise L.SdmiError("lora_gemm: %d ids do not divide %d rows" % (nid, m))
-    _own_device("lora_gemm", a.buf, wp, lora.a, lora.b, lora.scale, ids, bias, None if residual is None else residual.buf, res.buf)
+    _own_device("lora_gemm", ab, wp, lora.a, lora.b, lora.scale, ids, bias, None if residual is None else residual.buf, res.buf)
     need = _ws_need("sdmi_lora_gemm_ws_bytes", m, n_out, k, lora.rank, lora.groups, m // nid)
-    ab, ob = a.buf, res.buf
-    ws = torch.empty((need,), dtype=torch.uint8, device=ab.device) if need else None     # the call's own: two graphs never share it
-    L.call("sdmi_lora_gemm", a.ptr, ab.shape[-1], wp.data_ptr(), wp.stride(0), ob.data_ptr() + 2 * res.off, ob.shape[-1], m, n_out, k,
-           0 if bias is None else bias.data_ptr(), rp, rld, lora.a.data_ptr(), lora.b.data_ptr(), lora.scale.data_ptr(), lora.adapters, lora.rank, lora.groups,
-           ip, m // nid, flags, ws.data_ptr() if need else 0, need, _stream())
+    ob = res.buf
+    ws = ab.new_empty(((need + 1) // 2,)) if need else None     # the call's own: two graphs never share it
+    L.call("sdmi_lora_gemm_packed", L.LORA_GEMM_ARGS.pack(
+        ap, ab.shape[-1], wp.data_ptr(), wp.stride(0), ob.data_ptr() + 2 * res.off, ob.shape[-1], m, n_out, k, 0 if bias is None else bias.data_ptr(), rp, rld,
+        lora.a.data_ptr(), lora.b.data_ptr(), lora.scale.data_ptr(), lora.adapters, lora.rank, lora.groups, ip, m // nid, flags,
+        ws.data_ptr() if need else 0, need, _stream()))
     if RANGE_AUDIT:
         _audit("lora_gemm %dx%dx%d" % (m, n_out, k), res)
     return res

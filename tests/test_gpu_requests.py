@@ -246,6 +246,10 @@ def test_attention_refuses_tensors_of_another_kind():
             E.cross_attention(q, k, k, 1)
     with pytest.raises(L.SdmiError):
         E.cross_attention(a, a.cols(0, 32), a, 1)
+    wide = E.Act(a.buf.float(), 2, 1, 8, 64)
+    for q, k, out in ((wide, a, None), (a, wide, None), (a, a, wide)):
+        with pytest.raises(L.SdmiError):
+            E.cross_attention(q, k, k, 1, out=out)
 
 
 # ------------------------------------------------------------------------------------------------------------ adapters
@@ -371,8 +375,9 @@ def test_lora_refuses_tensors_of_another_kind():
                dict(residual=xa), dict(out=xa)):
         with pytest.raises(L.SdmiError):
             E.lora_gemm(xa, wd, 72, **{**good, **kw})
-    with pytest.raises(L.SdmiError):
-        E.lora_gemm(xa, wd.t(), 64, **good)
+    for x2, w2, n in ((xa, wd.t(), 64), (xa, wd.float(), 72), (E.Act(xa.buf.float(), 1, 1, 24, 64), wd, 72), (E.Act(xa.buf.float(), 1, 1, 24, 64), wd.float(), 72), (xa, wd[0], 72)):
+        with pytest.raises(L.SdmiError):
+            E.lora_gemm(x2, w2, n, **good)
     for bad in ((a.float(), b, scale), (a, b[:2], scale), (a, b, scale[:2]), (a[:, :12], b, scale), (a, b, scale.double())):
         with pytest.raises(L.SdmiError):
             E.LoraPack(*bad)

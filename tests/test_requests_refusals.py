@@ -39,6 +39,48 @@ def test_lora_refuses(change, word):
         L.call("sdmi_lora_gemm", *{**LORA, **change}.values())
 
 
+def _packed(fmt, args):
+    return fmt.pack(*(0 if v is None else v for v in args.values()))
+
+
+@pytest.mark.parametrize("change", [dict(q=None), dict(dim=60), dict(contexts=3), dict(ldk=64), dict(sk=1284), dict(o=P + 4), dict(kr=P), dict(index=P + 2), dict(scale=-1.0),
+                                    dict(nkv=1 << 32), dict(ldq=(1 << 32) + 128), dict(batch=-(1 << 40))])
+def test_attention_in_one_block_refuses_the_same(change):
+    with pytest.raises(L.SdmiError, match="cross_attention: ") as packed:
+        L.call("sdmi_cross_attention_packed", _packed(L.CROSS_ATTENTION_ARGS, {**ATT, **change}))
+    if all(not isinstance(v, int) or abs(v) < 1 << 31 for v in change.values()):
+        with pytest.raises(L.SdmiError) as plain:
+            L.call("sdmi_cross_attention", *{**ATT, **change}.values())
+        assert str(packed.value).split(": ", 1)[1] == str(plain.value).split(": ", 1)[1]
+
+
+@pytest.mark.parametrize("change", [dict(x=None), dict(ws=None), dict(rank=12), dict(groups=3), dict(rows=0), dict(flags=8), dict(flags=4), dict(ldw=68), dict(ids=P + 2),
+                                    dict(ws_bytes=8), dict(m=1 << 32), dict(rows=1 << 31), dict(flags=1 << 32), dict(flags=-1)])
+def test_lora_in_one_block_refuses_the_same(change):
+    with pytest.raises(L.SdmiError, match="lora_gemm: ") as packed:
+        L.call("sdmi_lora_gemm_packed", _packed(L.LORA_GEMM_ARGS, {**LORA, **change}))
+    if all(v is None or 0 <= v < 1 << 31 for v in change.values()):
+        with pytest.raises(L.SdmiError) as plain:
+            L.call("sdmi_lora_gemm", *{**LORA, **change}.values())
+        assert str(packed.value).split(": ", 1)[1] == str(plain.value).split(": ", 1)[1]
+
+
+def test_blocks_are_the_headers_structs():
+    """Every field of the two structs is one word of the format, in order."""
+    import os
+    import re
+    from conftest import ROOT
+    src = open(os.path.join(ROOT, "include", "sdmi.h")).read()
+    for name, fmt in (("sdmi_cross_attention_args", L.CROSS_ATTENTION_ARGS), ("sdmi_lora_gemm_args", L.LORA_GEMM_ARGS)):
+        body = re.sub(r"/\*.*?\*/", "", re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), src, re.S).group(1), flags=re.S)
+        want = ""
+        for decl in filter(None, (d.strip() for d in body.split(";"))):
+            for i, field in enumerate(decl.split(",")):
+                want += "Q" if "*" in field else ("d" if decl.startswith("double") else "q")
+        have = re.sub(r"(\d+)(.)", lambda m: m.group(2) * int(m.group(1)), fmt.format)
+        assert have == want and fmt.size == 8 * len(want), name
+
+
 def test_workspace_sizes():
     lib = L.load()
     assert lib.sdmi_cross_attention_ws_bytes(2, 5, 5, 64, 9216, 77) == 0            # one pass
