@@ -511,6 +511,9 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN == 4 && NSTAGE * (BM + BN + 
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // the column that this lane's row of product j stands for: the products 2 i and 2 i + 1 share 32 columns in fours, so that a lane
+  // ends up with eight neighbouring ones (a pair of 16-column products would need an exchange between lanes: 3 us of 70)
+  auto col = [&](int j) { return 32 * (j >> 1) + 8 * (l15 >> 2) + 4 * (j & 1) + (l15 & 3); };
   constexpr int FT = FR / 16;
   f32x4 tacc[FT ? FT : 1][MT];
   hx8 bf[FT ? NT : 1];
@@ -521,7 +524,7 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN == 4 && NSTAGE * (BM + BN + 
       for (int i = 0; i < MT; ++i) tacc[f][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < NT; ++j) {  // b of this wave's columns, ranks 8 lq .. 8 lq + 7
-      const int c = wc * TN + j * 16 + l15;
+      const int c = wc * TN + col(j);
       bf[j] = *(const hx8*)(8 * lq < rk && bcol + c < cend ? lb + (long long)c * p.rank + 8 * lq : (const u16*)g_lora_zero16);
     }
   }
@@ -543,7 +546,7 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN == 4 && NSTAGE * (BM + BN + 
 #pragma unroll
     for (int i = 0; i < MT; ++i) af[i] = *(const hx8*)&cA[lora_off(wr * TM + i * 16 + l15, lq + 4 * kk)];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) wf[j] = *(const hx8*)&cB[lora_off(wc * TN + j * 16 + l15, lq + 4 * kk)];
+    for (int j = 0; j < NT; ++j) wf[j] = *(const hx8*)&cB[lora_off(wc * TN + col(j), lq + 4 * kk)];
   };
   auto mfma = [&](const hx8 (&af)[MT], const hx8 (&wf)[NT]) {
 #pragma unroll
@@ -613,12 +616,9 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN == 4 && NSTAGE * (BM + BN + 
       }
     }
   }
-  // lanes l and l ^ 16 hold neighbouring 4-column pieces of a row: one exchange per pair of 16-column tiles leaves each with 8
-  // columns of one of them, 16-byte residual loads and stores
-  auto swz = [](float v) { return __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, v), 0x401F)); };
 #pragma unroll
   for (int j = 0; j < NT; j += 2) {
-    const int n = bcol + wc * TN + (j + (lq & 1)) * 16 + (lq >> 1) * 8;
+    const int n = bcol + wc * TN + 16 * j + 8 * lq;
     const bool okn = n < cend;
     f32x4 b0 = {0.f, 0.f, 0.f, 0.f}, b1 = b0;
     if (p.bias && okn) {
@@ -627,16 +627,21 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN == 4 && NSTAGE * (BM + BN + 
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-      float y[8];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float keep = (lq & 1) ? acc[i][j + 1][e] : acc[i][j][e], give = (lq & 1) ? acc[i][j][e] : acc[i][j + 1][e];
-        const float got = swz(give);
-        y[e] = ((lq & 1) ? got : keep) + b0[e];
-        y[4 + e] = ((lq & 1) ? keep : got) + b1[e];
-      }
       const int m = MIXED ? rowmap[wr * TM + i * 16 + l15] : brow + wr * TM + i * 16 + l15;
       if ((MIXED ? m >= 0 : m < rend) && okn) {
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          y[e] = acc[i][j][e];
+          y[4 + e] = acc[i][j + 1][e];
+        }
+        if (p.bias) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            y[e] += b0[e];
+            y[4 + e] += b1[e];
+          }
+        }
         if (p.residual) {
           float r[8];
           unpack8(*(const uint4*)(p.residual + (long long)m * p.ldr + n), r);
