@@ -5,6 +5,7 @@ Layout:
   _lib.py    ctypes binding of that C-ABI (raises if the library is missing: no CPU fallback)
   engine.py  NHWC-bf16 activation views, weight pre-pack cache, op wrappers
   dropin/    Unet.py / AutoencoderKL.py / layers/*.py: the reference's module surface (top-level module names)
+  conditioning.py what the requests of a batch bring along: encoder states of their own lengths, low-rank adapters
   sampler.py DDIM + classifier-free guidance loop on the fused update kernel
   shard.py   one-process-per-GPU image sharding + RCCL all-gather
   synth.py   deterministic synthetic weights / inputs

@@ -12,8 +12,15 @@
 // the exponent's fma in fp32; q and k are multiplied as they are).  S^T = K Q^T and O^T += V^T P^T on v_mfma_f32_32x32x16: the
 // query is on the lane in both, so the statistics are lane-local plus one exchange of the wave's halves, and P leaves the
 // first product in the operand layout of the second (k order inside a 16-key step as the accumulator has it; V is read
-// through ds_read_b64_tr_b16 in that order).  P is rounded to 16 bits for the matrix cores (half a step of a value <= 1);
+// through ds_read_b64_tr_b16 in that order).  P is rounded to 16 bits for the matrix cores (half a step of its value);
 // S, m, l and O stay in fp32.
+//
+// What bounds it (MI355X, fp16, device times): long states the exponentials and the rescaled sums, two vector instructions' time
+// for each MFMA's - 2 x 10 heads of 64, 2304 rows to 9216 keys 157 us, 690 TFLOP/s; 96 x 96 rows 325 us, 670; heads of 128 to 4096 keys
+// 126 us, 611; 160: 147 us, 657; 80: 87 us, 554; 256 (one wave to a SIMD): 155 us, 499.  The prompt's lengths the start of a block (Q, the
+// first tile, the store: memory latencies behind one another, two to four blocks to a CU to cover them) - 2 x 5 heads, 9216 rows to
+// 77 keys 12.1 us, 16 x 20 heads, 576 rows to 231 shared keys 24 us, 2304 rows to 154 keys in regions 15.6 us.  One row the reading
+// of the keys - 320 rows to 9216 keys (755 MB) 138 + 5 us, 5.3 TB/s; 8 x 16 heads of 128 on 4, 4096 keys (38 MB where half exist) 13.6 + 4 us.
 #include "common.h"
 #include <atomic>
 
