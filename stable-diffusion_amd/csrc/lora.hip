@@ -664,7 +664,7 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN == 4 && NSTAGE * (BM + BN + 
 // ------------------------------------------------------------------------------------------------------------ host
 static bool lora_shape_ok(int m, int n, int k, int rank, int groups) {
   // a group's columns are whole 8-column pieces: the kernels' tiles start at its first
-  return m > 0 && m < (1 << 30) && n > 0 && n < (1 << 30) && k > 0 && groups > 0 && groups <= 64 && n % groups == 0 && (n / groups) % 8 == 0 && k % 8 == 0 && rank > 0 && rank % 8 == 0 && rank <= 256;
+  return m > 0 && m < (1 << 30) && n > 0 && n < (1 << 27) && k > 0 && groups > 0 && groups <= 64 && n % groups == 0 && (n / groups) % 8 == 0 && k % 8 == 0 && rank > 0 && rank % 8 == 0 && rank <= 256;
 }
 // which kernels take a problem; the workspace holds t where a launch hands it to the next
 enum { LORA_ROWS_FUSED, LORA_ROWS, LORA_TILES_FUSED, LORA_TILES, LORA_MIXED };
@@ -710,6 +710,7 @@ static int lora_shrink_launch2(const LoraParams& p, hipStream_t st) {
   static std::atomic<unsigned long long> done{0};
   constexpr int TR = 16 * MR, bytes = ShrinkShape<MR, NT>::bytes;
   static_assert(bytes <= 160 * 1024, "LDS of a CU");
+  SDMI_REQUIRE((p.M + TR - 1) / TR < (1 << 23), "lora_gemm: grid too large");  // a launch has fewer than 2^32 threads
   const int rc = lora_allow_lds(lora_shrink_kernel<MR, NT>, bytes, done);
   if (rc != SDMI_OK) return rc;
   const int touched = p.rpi >= TR ? (p.rpi % TR == 0 ? 1 : 2) : min((TR - 1 + p.rpi - 1) / p.rpi + 1, TR);  // requests that TR rows can touch

@@ -89,8 +89,9 @@ class Unet(nn.Module):
         chooses for each batch."""
         if adapters is not None and not {id(m) for m, _ in adapters.layers} <= {id(m) for m in self.modules()}:
             raise E.L.SdmiError("Unet.set_adapters: this set was built for another model")
-        if self.adapters is not None:
-            self.adapters.detach()
+        for m in self.modules():
+            if hasattr(m, "to_q"):
+                m.adapters = None
         self.adapters = adapters.attach() if adapters is not None else None
 
     @torch.no_grad()

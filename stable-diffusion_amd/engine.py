@@ -584,6 +584,13 @@ def _int32(t, shape, what):
     return t.data_ptr()
 
 
+def _apart(what, out, *inputs):
+    """`out` was given: it must not share columns of a buffer with an operand that other blocks are still reading."""
+    for a in inputs:
+        if a.buf.data_ptr() == out.buf.data_ptr() and a.off < out.off + out.c and out.off < a.off + a.c:
+            raise L.SdmiError("%s: `out` lies in an operand's memory" % what)
+
+
 @functools.lru_cache(maxsize=4096)
 def _ws_need(name, *shape):
     """A workspace size of the library: a function of the shape alone, asked for once."""
@@ -611,6 +618,8 @@ def cross_attention(q, k, v, heads, kv_heads=None, dim=64, scale=None, index=Non
         raise L.SdmiError("cross_attention: q (%d,%d,%d) / k (%d,%d,%d) / v (%d,%d,%d) / out (%d,%d,%d) do not match %d heads on %d key heads of %d" %
                           (b, nq, q.c, n, nkv, k.c, v.n, v.hw, v.c, o.n, o.hw, o.c, heads, kv_heads, dim))
     ob, h = o.buf, act_dtype()
+    if out is not None:
+        _apart("cross_attention", o, q, k, v)
     if qb.dtype is not h or kb.dtype is not h or vb.dtype is not h or ob.dtype is not h:
         raise L.SdmiError("cross_attention: q %s, k %s, v %s, out %s: the kernels take %s" % (qb.dtype, kb.dtype, vb.dtype, ob.dtype, h))
     _own_device("cross_attention", qb, kb, vb, ob, index, lens, query_regions, key_regions)
@@ -658,6 +667,7 @@ def lora_gemm(a, wp, n_out, lora, ids, bias=None, residual=None, out=None):
         res.stats.pop(res.off, None)
         if (res.n * res.hw, res.c) != (m, n_out):
             raise L.SdmiError("lora_gemm: `out` holds %d rows x %d channels, the product has %d x %d" % (res.n * res.hw, res.c, m, n_out))
+        _apart("lora_gemm", res, a)
     if wp.shape != (n_out, k) or wp.stride(1) != 1 or wp.dtype is not lora.a.dtype or ab.dtype is not lora.a.dtype or lora.a.shape[2] != k or lora.b.shape[1] != n_out:
         raise L.SdmiError("lora_gemm: tokens %s, weight %s %s, adapters %s a %s / b %s for %d -> %d channels" %
                           (ab.dtype, wp.dtype, tuple(wp.shape), lora.a.dtype, tuple(lora.a.shape), tuple(lora.b.shape), k, n_out))

@@ -67,11 +67,12 @@ class Sampler(object):
         graphs and cached tables are keyed on it, so they are rebuilt instead of replaying stale packed weights."""
         return tuple((p.data_ptr(), p._version) for p in module.parameters()) if module is not None else ()
 
-    def _adapter_key(self):
-        """What of the adapters a captured step has baked in: the set, which is kept alive beside the graph so that its id stays
-        its own, and the length of the ids, which says where they live."""
-        ad = getattr(self.unet, "adapters", None)
-        return None if ad is None else (id(ad), 0 if ad.ids is None else ad.ids.numel())
+    @staticmethod
+    def adapters_of(module):
+        """What of its adapters a captured step has baked in: each layer's (kept alive beside the graph, so that their ids stay
+        their own) and the lengths of the sets' ids, which say where those live."""
+        found = [m.adapters for m in module.modules() if hasattr(m, "to_q") and getattr(m, "adapters", None) is not None] if module is not None else []
+        return found, tuple((id(a), 0 if a.owner.ids is None else a.owner.ids.numel()) for a in found)
 
     def _time_tables(self, steps, bc, dev):
         key = (tuple(int(s) for s in steps), bc, str(dev), self._usig)
@@ -184,8 +185,9 @@ class Sampler(object):
             return self._unet_eval(xc, t_buf, cc, same_halves)
         # the graph is valid while the buffers it read are alive and in place: key on the objects that own them (the
         # sampler keeps xc, the TimeEmb row and the ContextKV alive; a caller's own buffers must outlive the graph)
+        adapters, akey = getattr(self, "_adapters", None) or self.adapters_of(self.unet)
         key = (xc.data_ptr(), t_buf.table.data_ptr() if hasattr(t_buf, "table") else t_buf.data_ptr(), id(cc), tuple(xc.shape), same_halves,
-               getattr(self, "_usig", None) or self.weights_signature(self.unet), self._adapter_key())
+               getattr(self, "_usig", None) or self.weights_signature(self.unet), akey)
         if self._gkey != key:
             self._unet_eval(xc, t_buf, cc, same_halves)         # warm-up: weight pre-pack, allocator pools
             torch.cuda.synchronize()
@@ -194,7 +196,7 @@ class Sampler(object):
             # multi-GPU run polling its events) must not invalidate it
             with torch.cuda.graph(g, capture_error_mode="thread_local"):
                 out = self._unet_eval(xc, t_buf, cc, same_halves)
-            self._graph, self._gout, self._gkey, self._gkeep = g, out, key, (xc, t_buf, cc, getattr(self.unet, "adapters", None))
+            self._graph, self._gout, self._gkey, self._gkeep = g, out, key, (xc, t_buf, cc, adapters)
         self._graph.replay()
         return self._gout
 
@@ -206,6 +208,7 @@ class Sampler(object):
         ts, a_t, a_prev, sig, s1m = ddim_schedule(num_ddim_timesteps, eta)
         total = ts.shape[0]
         self._usig = self.weights_signature(self.unet)      # once per image: keys the captured step and the cached tables
+        self._adapters = self.adapters_of(self.unet)
         b, _, h, w = x_T.shape
         dev = x_T.device
         xc = self._static_xc((2 * b, 4 + c_concat.shape[1], h, w), dev)

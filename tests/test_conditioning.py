@@ -181,6 +181,13 @@ def test_sampler_replays_one_step_for_other_states_and_adapters(net, dual):
             xe, _ = eager.sample(*args, decode=False, use_graph=False)
             assert torch.isfinite(xe).all() and torch.equal(xg, xe), step
             seen.append(xe)
+        sets[0].detach()                # taken out layer by layer, behind the model's back
+        xg, _ = graph.sample(*args, decode=False, use_graph=True)
+        xe, _ = eager.sample(*args, decode=False, use_graph=False)
+        assert torch.equal(xg, xe) and not torch.equal(xe, seen[-1])
+        sets[0].attach()
+        xg, _ = graph.sample(*args, decode=False, use_graph=True)
+        assert torch.equal(xg, seen[-1])
         unet.set_adapters(None)
         xg, _ = graph.sample(*args, decode=False, use_graph=True)
         xe, _ = eager.sample(*args, decode=False, use_graph=False)
@@ -282,6 +289,12 @@ def test_adapters_refuse(monkeypatch):
     assert twin.transformer_blocks[0].attn1.adapters.pack("qkv") is not None
     s.detach()
     assert block.attn1.adapters is None and block.attn2.adapters is None
+    from stable_diffusion_amd.sampler import Sampler
+    assert Sampler.adapters_of(m) == ([], ())
+    s.attach()
+    held, key = Sampler.adapters_of(m)
+    s.select([0, 0, 0, 1])
+    assert [la for _, la in s.layers] == held and Sampler.adapters_of(m)[1] != key
 
 
 def test_a_set_belongs_to_its_model(monkeypatch):

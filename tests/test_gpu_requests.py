@@ -246,6 +246,10 @@ def test_attention_refuses_tensors_of_another_kind():
             E.cross_attention(q, k, k, 1)
     with pytest.raises(L.SdmiError):
         E.cross_attention(a, a.cols(0, 32), a, 1)
+    both = E.Act(torch.zeros((2, 8, 192), dtype=H16, device=DEV), 2, 1, 8, 192)
+    for out in (a, both.cols(32, 64), both.cols(127, 64)):
+        with pytest.raises(L.SdmiError, match="memory"):
+            E.cross_attention(a if out is a else both.cols(0, 64), both.cols(64, 64), both.cols(128, 64), 1, out=out)
     wide = E.Act(a.buf.float(), 2, 1, 8, 64)
     for q, k, out in ((wide, a, None), (a, wide, None), (a, a, wide)):
         with pytest.raises(L.SdmiError):
@@ -375,6 +379,9 @@ def test_lora_refuses_tensors_of_another_kind():
                dict(residual=xa), dict(out=xa)):
         with pytest.raises(L.SdmiError):
             E.lora_gemm(xa, wd, 72, **{**good, **kw})
+    square = torch.zeros((64, 64), dtype=H16, device=DEV)
+    with pytest.raises(L.SdmiError, match="memory"):
+        E.lora_gemm(xa, square, 64, E.LoraPack(pack.a, pack.b[:, :64].contiguous(), pack.scale), good["ids"], out=xa)
     for x2, w2, n in ((xa, wd.t(), 64), (xa, wd.float(), 72), (E.Act(xa.buf.float(), 1, 1, 24, 64), wd, 72), (E.Act(xa.buf.float(), 1, 1, 24, 64), wd.float(), 72), (xa, wd[0], 72)):
         with pytest.raises(L.SdmiError):
             E.lora_gemm(x2, w2, n, **good)

@@ -32,7 +32,8 @@ def test_attention_refuses(change, word):
     (dict(rows=0), "rows per id"), (dict(flags=8), "flags"), (dict(flags=1), "bias"), (dict(flags=4), "residual"), (dict(flags=4, residual=P, ldr=32), "residual"),
     (dict(ldx=32), "strides"), (dict(ldw=68), "strides"), (dict(ldo=60), "strides"), (dict(ldx=1 << 22), "too large"), (dict(x=P + 8), "alignment"),
     (dict(flags=4, residual=P + 8, ldr=64), "alignment"), (dict(ids=P + 2), "alignment"), (dict(ws_bytes=8), "workspace"), (dict(m=1 << 30), "shape"),
-    (dict(n=1 << 30, ldo=1 << 30), "shape"),
+    (dict(n=1 << 27, ldo=1 << 27), "shape"),
+    (dict(m=(1 << 30) - 64, rows=(1 << 30) - 64, rank=40, ws_bytes=1 << 40), "grid"),
 ])
 def test_lora_refuses(change, word):
     with pytest.raises(L.SdmiError, match=word):
