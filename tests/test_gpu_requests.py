@@ -163,6 +163,21 @@ def test_attention_large_scores_and_other_scale(nq, nkv):
     _close(got, want, tol, "attention, scores of hundreds")
 
 
+@pytest.mark.parametrize("nq,nkv", [(1, 6000), (200, 6000), (200, 900)])
+@pytest.mark.parametrize("far", [12.0, 16.0, 20.0])
+def test_attention_small_weights_add_up(nq, nkv, far):
+    """One key far above thousands whose p = 2^-far is at or below the 16-bit type's smallest normal number: they count, in the
+    numerator and in the sum."""
+    rs = np.random.RandomState(int(far))
+    q, k, v = torch.zeros(1, nq, 64), torch.zeros(1, nkv, 64), _h(rs, 1, nkv, 64)
+    q[:, :, 0], k[:, nkv // 2, 0] = 1.0, 1.0
+    v[:, :, 0] = 1.0                                         # column 0 comes out as 1 if and only if both agree
+    q, k = q.to(H16), k.to(H16)
+    got = _run_attention(q, k, v, 1, 1, 64, None, None, None, None, scale=far * math.log(2.0))
+    want, tol = _attention_oracle(q, k, v, 1, 1, 64, float(np.float32(far * math.log(2.0))), None, None, None, None)
+    _close(got, want, tol, "attention, %d weights of 2^-%g" % (nkv, far))
+
+
 @pytest.mark.parametrize("nq", [3, 200])
 def test_attention_no_keys_gives_zeros(nq):
     q = _h(np.random.RandomState(1), 2, nq, 128)
