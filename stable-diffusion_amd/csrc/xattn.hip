@@ -16,10 +16,10 @@
 // S, m, l and O stay in fp32.
 //
 // What bounds it (MI355X, fp16, device times): long states the exponentials and the rescaled sums, two vector instructions' time
-// for each MFMA's - 2 x 10 heads of 64, 2304 rows to 9216 keys 157 us, 690 TFLOP/s; 96 x 96 rows 325 us, 670; heads of 128 to 4096 keys
-// 126 us, 611; 160: 147 us, 657; 80: 87 us, 554; 256 (one wave to a SIMD): 155 us, 499.  The prompt's lengths the start of a block (Q, the
+// for each MFMA's - 2 x 10 heads of 64, 2304 rows to 9216 keys 142 us, 766 TFLOP/s; 96 x 96 rows 310 us, 701; heads of 128 to 4096 keys
+// 126 us, 615; 160: 130 us, 742; 80: 78 us, 616; 256 (one wave to a SIMD): 155 us, 497.  The prompt's lengths the start of a block (Q, the
 // first tile, the store: memory latencies behind one another, two to four blocks to a CU to cover them) - 2 x 5 heads, 9216 rows to
-// 77 keys 12.1 us, 16 x 20 heads, 576 rows to 231 shared keys 24 us, 2304 rows to 154 keys in regions 15.6 us.  One row the reading
+// 77 keys 12.1 us, 16 x 20 heads, 576 rows to 231 shared keys 24 us, 2304 rows to 154 keys in regions 15.0 us.  One row the reading
 // of the keys - 320 rows to 9216 keys (755 MB) 138 + 5 us, 5.3 TB/s; 8 x 16 heads of 128 on 4, 4096 keys (38 MB where half exist) 13.6 + 4 us.
 #include "common.h"
 #include <atomic>
@@ -57,6 +57,15 @@ enum { XA_FULL = 0, XA_TAIL = 1, XA_REGIONS = 2 };
 
 constexpr int XA_KT = 64;  // keys of a tile
 
+// A SIMD's waves are in different phases: one whose matrix instructions are ready goes before one that exponentiates, or the two kinds
+// wait for each other.  Heads up to 96 wide (two vector instructions' time to a matrix one's): P V first of all, 2304 rows to 9216
+// keys 152 -> 137 us, heads of 80 to 4096 keys 86 -> 76.  128 and 160: Q K^T first, 126 -> 125 and 146 -> 131 (P V first: 132 and 140).
+// 256: a SIMD has one wave (with any of them 156 -> 158).
+enum { XA_SCORES, XA_SOFTMAX, XA_OUTPUT };
+template <int DP, int PHASE> __device__ __forceinline__ void xa_priority() {
+  if constexpr (DP <= 160) __builtin_amdgcn_s_setprio(PHASE == XA_SCORES ? 2 : PHASE == XA_SOFTMAX ? 0 : DP <= 96 ? 3 : 1);
+}
+
 // One wave's share of a key tile: KS blocks of 32 keys (from row kr0 of the tile) against its 32 rows.
 template <int DP, int KS, int MODE>
 __device__ __forceinline__ void xa_step(const u16* sK, const u16* sV, const unsigned* sR, const hx8 (&qf)[DP / 16], f32x16 (&oacc)[DP / 32], float& m,
@@ -69,8 +78,10 @@ __device__ __forceinline__ void xa_step(const u16* sK, const u16* sV, const unsi
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = 0.f;
     const int krow = kr0 + 32 * b + r;
+    xa_priority<DP, XA_SCORES>();
 #pragma unroll
     for (int ks = 0; ks < DP / 16; ++ks) s = MFMA32(*(const hx8*)&sK[krow * DP + (((2 * ks + hh) ^ xa_kx<DP>(krow)) << 3)], qf[ks], s, 0, 0, 0);
+    xa_priority<DP, XA_SOFTMAX>();
     if constexpr (MODE == XA_TAIL) {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
@@ -107,6 +118,7 @@ __device__ __forceinline__ void xa_step(const u16* sK, const u16* sV, const unsi
       rs += s[i];
     }
     l += rs;
+    xa_priority<DP, XA_OUTPUT>();
 #pragma unroll
     for (int s2 = 0; s2 < 2; ++s2) {
       hx8 pb;
