@@ -339,8 +339,8 @@ struct XattnPlan { int wk, rtiles, splits; };
 static XattnPlan xattn_plan(int batch, int kvh, int dim, int rows, int nkv) {
   XattnPlan pl;
   // one wave sweeps all keys for its 32 rows, or two waves share them.  The second gives blocks of 64 rows: fewer of them idle where
-  // there are few, and finer pieces where contexts differ (2304 rows to 9216 keys, heads of 64: 155 us against 190; of 80, to 4096: 88
-  // against 99; of 128: 139 against 124; 9216 rows to 77 keys: 15.6 against 12.4, for the merge is paid per block)
+  // there are few, and finer pieces where contexts differ (2304 rows to 9216 keys, heads of 64: 144 us against 175; of 80, to 4096: 78
+  // against 92; of 128: 140 against 124; 2304 rows to 154 keys: 19.7 against 14.8, for the merge is paid per block)
   const bool few = rows <= 64;
   pl.wk = few || (dim <= 96 && nkv >= 512) ? 2 : 1;
   const int per = pl.wk == 2 ? 64 : 128;
