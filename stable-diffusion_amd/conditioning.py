@@ -102,9 +102,7 @@ class EncoderStates(object):
     @staticmethod
     def cat(a, b, batch=None):
         """The batch [a | b] (as the CFG batch [uncond | cond]); batch: samples of a side that has one context for any number.
-        The contexts of b follow those of a."""
-        if (a.key_regions is None) != (b.key_regions is None):
-            raise L.SdmiError("EncoderStates.cat: regions on both sides or on none")
+        The contexts of b follow those of a; beside a side with regions, one without is in all of them."""
         ba, bb = (s.batch if s.batch is not None else batch for s in (a, b))
         if ba is None or bb is None:
             raise L.SdmiError("EncoderStates.cat: one context for a batch of any size: say of which (batch)")
@@ -122,8 +120,14 @@ class EncoderStates(object):
             ib = b.index if b.index is not None else own(b, nb, bb)
             # an index outside its own side sees nothing, and not the other side's contexts
             index = torch.cat([torch.where(ia < na, ia, full(ba, -1)), torch.where((ib >= 0) & (ib < nb), ib + na, full(bb, -1))])
-        if a.key_regions is not None:
-            kr, qr = torch.cat([pad(a.key_regions), pad(b.key_regions)]), torch.cat([a.query_regions, b.query_regions])
+        with_regions = a if a.key_regions is not None else b
+        if with_regions.key_regions is not None:
+            hw = with_regions.query_regions.shape[1:]
+            keys = lambda s: s.key_regions if s.key_regions is not None else full(s.tokens.shape[0], -1)[:, None].expand(-1, s.tokens.shape[1])
+            queries = lambda s, m: s.query_regions if s.query_regions is not None else full(m, -1)[:, None, None].expand(-1, *hw)
+            if a.query_regions is not None and b.query_regions is not None and a.query_regions.shape[1:] != b.query_regions.shape[1:]:
+                raise L.SdmiError("EncoderStates.cat: query_regions of %s and %s" % (tuple(a.query_regions.shape), tuple(b.query_regions.shape)))
+            kr, qr = torch.cat([pad(keys(a)), pad(keys(b))]), torch.cat([queries(a, ba), queries(b, bb)])
         return EncoderStates(torch.cat([pad(a.tokens), pad(b.tokens)]), lens_ab, index, kr, qr)
 
 

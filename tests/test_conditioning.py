@@ -210,6 +210,24 @@ def test_sampler_takes_one_context_for_the_batch_and_plain_negatives(net):
         _gate(g, want.cpu(), 1.5e-2, 1.5e-2, "one context")
 
 
+@pytest.mark.gpu
+def test_sampler_takes_regions_beside_plain_negatives(net):
+    """Both halves in one batch (the plain one in every region) and one by one (the plain one without regions)."""
+    from stable_diffusion_amd.sampler import Sampler
+    unet, _ = net
+    rs = np.random.RandomState(6)
+    inp = make_inputs(2, 16, 2, seed=43)
+    dev = lambda v: v.to(DEV)
+    rest = (dev(inp["c_concat"]), dev(inp["x_T"]), [dev(n) for n in inp["noises"]], 7.5)
+    cond = EncoderStates(dev(_rand(rs, 2, 100, 1024)), [100, 60], None, T(rs.randint(1, 4, (2, 100))), T(rs.randint(0, 4, (2, 16, 16))))
+    one = Sampler(unet, None, dual_stream=False).sample(2, cond, dev(inp["uncond"]), *rest, decode=False)[0]
+    two = Sampler(unet, None, dual_stream=True).sample(2, cond, dev(inp["uncond"]), *rest, decode=False)[0]
+    _gate(two, one.cpu(), 1.5e-2, 1.5e-2, "regions beside plain negatives")
+    graph = Sampler(unet, None, dual_stream=False)
+    for _ in range(2):
+        assert torch.equal(graph.sample(2, cond, dev(inp["uncond"]), *rest, decode=False, use_graph=True)[0], one)
+
+
 # ------------------------------------------------------------------------------------------------------------ refusals and layout
 def test_cat_keeps_each_side_to_its_own_contexts(monkeypatch):
     monkeypatch.setattr(E, "_need_cuda", lambda t, what: None)
@@ -226,8 +244,11 @@ def test_cat_keeps_each_side_to_its_own_contexts(monkeypatch):
     assert r.regions(3, 2).tolist() == [[0, 2, 6, 8, 12, 14]] and r.regions(1, 1).tolist() == [[0]]
     with pytest.raises(L.SdmiError, match="no level"):
         r.regions(4, 2)
-    with pytest.raises(L.SdmiError, match="both sides"):
-        EncoderStates.cat(r, EncoderStates(torch.zeros(1, 5, 8)), batch=1)
+    whole = EncoderStates.cat(EncoderStates(torch.zeros(1, 4, 8)), r, batch=2)          # in every region beside one that has some
+    assert whole.batch == 3 and whole.lens.tolist() == [4, 5] and whole.index.tolist() == [0, 0, 1]
+    assert whole.key_regions.tolist() == [[-1, -1, -1, -1, 0], [1] * 5] and whole.query_regions[:2].eq(-1).all() and torch.equal(whole.query_regions[2:], r.query_regions)
+    with pytest.raises(L.SdmiError, match="query_regions of"):
+        EncoderStates.cat(r, EncoderStates(torch.zeros(1, 5, 8), key_regions=torch.ones(1, 5, dtype=torch.int64), query_regions=torch.zeros(1, 3, 5, dtype=torch.int64)))
     assert EncoderStates(torch.zeros(1, 2, 8), key_regions=torch.tensor([[0xffffffff, 1]]), query_regions=torch.zeros(2, 1, 1, dtype=torch.int32)).key_regions.tolist() == [[-1, 1]]
 
 
