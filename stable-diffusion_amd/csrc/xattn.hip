@@ -228,6 +228,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void xattn_k
   for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
     for (int i = 0; i < 16; ++i) oacc[dt][i] = 0.f;
+  // a wave without rows only helps to move the tiles (4 x 8 heads of 256, 4 rows to 2048 keys: 24.5 -> 22.6 us)
+  const bool live = rt * S::ROWS + wr * 32 < p.rows;
   const int kr0 = wk * (KT / WK), tfull = min(t1, len / KT);  // tiles below tfull are whole
   // the rows' own loads are waited for here, where the compiler sees it: it would else wait inside the loop for everything in
   // flight, the next tile's DMA among it
@@ -238,10 +240,10 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void xattn_k
     const int cur = (tile - t0) & 1;
     if (tile + 1 < t1) stage(tile + 1, cur ^ 1);
     const u16* sK = smem + cur * S::BUF;
-    xa_step<DP, S::KS, REG ? XA_REGIONS : XA_FULL>(sK, sK + KT * DP, sreg + cur * KT, qf, oacc, m, l, p.c, kr0, tile * KT + kr0, len, qset, lane);
+    if (live) xa_step<DP, S::KS, REG ? XA_REGIONS : XA_FULL>(sK, sK + KT * DP, sreg + cur * KT, qf, oacc, m, l, p.c, kr0, tile * KT + kr0, len, qset, lane);
     XA_LANDED();
   }
-  if (!REG && t0 < t1 && tfull < t1) {  // the one partial tile: its data has landed
+  if (!REG && live && t0 < t1 && tfull < t1) {  // the one partial tile: its data has landed
     const u16* sK = smem + ((t1 - 1 - t0) & 1) * S::BUF;
     xa_step<DP, S::KS, XA_TAIL>(sK, sK + KT * DP, sreg, qf, oacc, m, l, p.c, kr0, (t1 - 1) * KT + kr0, len, qset, lane);
   }
