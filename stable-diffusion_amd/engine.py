@@ -570,12 +570,14 @@ def cross_attention_lnq(a, ln_mod, to_q_weight, k, v, heads, out=None):
     return o
 
 
-def _own_device(what, *tensors):
+def _own_device(what, first, *others):
     """The kernels run on the current device's current stream: every tensor has to live there."""
-    cur = torch._C._cuda_getDevice()
-    for t in tensors:
-        if t is not None and t.get_device() != cur:
-            raise L.SdmiError("%s: a tensor is on %s, the current device is cuda:%d" % (what, t.device, cur))
+    d = first.get_device()
+    if d < 0 or d != torch._C._cuda_getDevice():
+        raise L.SdmiError("%s: a tensor is on %s, not on the current device" % (what, first.device))
+    for t in others:
+        if t is not None and t.get_device() != d:
+            raise L.SdmiError("%s: a tensor is on %s, another on %s" % (what, first.device, t.device))
 
 
 def _int32(t, shape, what):

@@ -40,6 +40,18 @@ def test_lora_refuses(change, word):
         L.call("sdmi_lora_gemm", *{**LORA, **change}.values())
 
 
+def test_no_cpu_fallback():
+    import torch
+    from stable_diffusion_amd import engine as E
+    h = E.act_dtype()
+    a = E.Act(torch.zeros((2, 8, 64), dtype=h), 2, 1, 8, 64)
+    with pytest.raises(L.SdmiError, match="cpu"):
+        E.cross_attention(a, a, a, 1)
+    pack = E.LoraPack(torch.zeros((1, 8, 64), dtype=h), torch.zeros((1, 64, 8), dtype=h), torch.ones(1))
+    with pytest.raises(L.SdmiError, match="cpu"):
+        E.lora_gemm(a, torch.zeros((64, 64), dtype=h), 64, pack, torch.zeros(2, dtype=torch.int32))
+
+
 def _packed(fmt, args):
     return fmt.pack(*(0 if v is None else v for v in args.values()))
 
