@@ -154,6 +154,35 @@ def test_states_of_whole_contexts_are_plain_contexts(net):
     _gate(shared, unet(x, timesteps=t, context=ctx[:1].expand(2, -1, -1).contiguous().to(DEV)).cpu(), 7e-3, 6e-3, "one shared context")
 
 
+@pytest.mark.gpu
+def test_a_callers_own_graph_sees_new_states_and_adapters(net):
+    """Unet.forward captured by the caller: what EncoderStates.copy_ and AdapterSet.select write reaches the replays."""
+    unet, sd = net
+    rs = np.random.RandomState(12)
+    dev = lambda v: v.to(DEV)
+    x, t = dev(_rand(rs, 2, 9, 16, 16)), torch.tensor([481, 481]).to(DEV)
+    make = lambda lens, index: EncoderStates(dev(_rand(rs, 2, 60, 1024)), lens, index, T(rs.randint(1, 4, (2, 60))), T(rs.randint(0, 4, (2, 16, 16))))
+    states, adapters = make([60, 20], [0, 1]), AdapterSet(unet, _unet_adapters(rs, sd, 0.2)).select([0, 1], [1, 0])
+    try:
+        unet.set_adapters(adapters)
+        unet(x, timesteps=t, context=states)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = unet(x, timesteps=t, context=states)
+        for step, (lens, index, ids, cids) in enumerate((([60, 20], [0, 1], [0, 1], [1, 0]), ([7, 59], [1, 1], [1, -1], [-1, 0]), ([0, 60], [0, 1], [-1, -1], [1, 1]))):
+            states.copy_(make(lens, index))
+            adapters.select(ids, cids)
+            want = unet(x, timesteps=t, context=states).clone()
+            torch.cuda.synchronize()
+            for _ in range(2):
+                g.replay()
+                torch.cuda.synchronize()
+                assert torch.equal(out, want), step
+    finally:
+        unet.set_adapters(None)
+
+
 # ------------------------------------------------------------------------------------------------------------ the sampler
 @pytest.mark.gpu
 @pytest.mark.parametrize("dual", [True, False])
