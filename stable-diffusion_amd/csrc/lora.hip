@@ -655,7 +655,10 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN == 4 && NSTAGE * (BM + BN + 
 #pragma unroll
           for (int e = 0; e < 8; ++e) y[e] += r[e];
         }
-        *(uint4*)(p.out + (long long)m * p.ldo + n) = pack8(y);
+        // past the L2, which holds the operands: with the attention that reads the result next, 96 x 96 to_q 26.3 -> 24.0 us, 48 x 48
+        // q|k|v 219 -> 214
+        const uint4 o = pack8(y);
+        __builtin_nontemporal_store((u32x4){o.x, o.y, o.z, o.w}, (u32x4*)(p.out + (long long)m * p.ldo + n));
       }
     }
   }
