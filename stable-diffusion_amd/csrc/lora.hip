@@ -22,6 +22,7 @@
 //     adapters of rank 128, 1024 -> 1024: 9.6 us for t and the order, 12.0 for the product.
 #include "common.h"
 #include <atomic>
+#include <type_traits>
 
 __device__ __attribute__((aligned(16))) unsigned g_lora_zero16[4] = {0u, 0u, 0u, 0u};
 
@@ -623,45 +624,54 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN == 4 && NSTAGE * (BM + BN + 
       }
     }
   }
+  // A projection without a residual goes to an attention, which reads it once: past the L2, which keeps the operands (with that
+  // attention, 96 x 96 to_q 26.3 -> 24.0 us, 48 x 48 q|k|v 219 -> 214).  One that joins the residual stream is what the next product
+  // reads over and over: 9216 x 1280 -> 1280 -> 1280 takes 100 us, past the L2 107; 18432 x 320 -> 320 -> 2560 68, 70.  (Two copies of the
+  // code: the compiler joins two stores that differ in nothing else.)
+  auto finish = [&](auto with_residual) {
+    constexpr bool RES = decltype(with_residual)::value;
 #pragma unroll
-  for (int j = 0; j < NT; j += 2) {
-    const int n = bcol + wc * TN + 16 * j + 8 * lq;
-    const bool okn = n < cend;
-    f32x4 b0 = {0.f, 0.f, 0.f, 0.f}, b1 = b0;
-    if (p.bias && okn) {
-      b0 = *(const f32x4*)(p.bias + n);
-      b1 = *(const f32x4*)(p.bias + n + 4);
-    }
+    for (int j = 0; j < NT; j += 2) {
+      const int n = bcol + wc * TN + 16 * j + 8 * lq;
+      const bool okn = n < cend;
+      f32x4 b0 = {0.f, 0.f, 0.f, 0.f}, b1 = b0;
+      if (p.bias && okn) {
+        b0 = *(const f32x4*)(p.bias + n);
+        b1 = *(const f32x4*)(p.bias + n + 4);
+      }
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const int m = MIXED ? rowmap[wr * TM + i * 16 + l15] : brow + wr * TM + i * 16 + l15;
-      if ((MIXED ? m >= 0 : m < rend) && okn) {
-        float y[8];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          y[e] = acc[i][j][e];
-          y[4 + e] = acc[i][j + 1][e];
-        }
-        if (p.bias) {
+      for (int i = 0; i < MT; ++i) {
+        const int m = MIXED ? rowmap[wr * TM + i * 16 + l15] : brow + wr * TM + i * 16 + l15;
+        if ((MIXED ? m >= 0 : m < rend) && okn) {
+          float y[8];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            y[e] += b0[e];
-            y[4 + e] += b1[e];
+            y[e] = acc[i][j][e];
+            y[4 + e] = acc[i][j + 1][e];
           }
-        }
-        if (p.residual) {
-          float r[8];
-          unpack8(*(const uint4*)(p.residual + (long long)m * p.ldr + n), r);
+          if (p.bias) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] += r[e];
+            for (int e = 0; e < 4; ++e) {
+              y[e] += b0[e];
+              y[4 + e] += b1[e];
+            }
+          }
+          if constexpr (RES) {
+            float r[8];
+            unpack8(*(const uint4*)(p.residual + (long long)m * p.ldr + n), r);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] += r[e];
+          }
+          const uint4 o = pack8(y);
+          u32x4* const to = (u32x4*)(p.out + (long long)m * p.ldo + n);
+          if constexpr (RES) *to = (u32x4){o.x, o.y, o.z, o.w};
+          else __builtin_nontemporal_store((u32x4){o.x, o.y, o.z, o.w}, to);
         }
-        // past the L2, which holds the operands: with the attention that reads the result next, 96 x 96 to_q 26.3 -> 24.0 us, 48 x 48
-        // q|k|v 219 -> 214
-        const uint4 o = pack8(y);
-        __builtin_nontemporal_store((u32x4){o.x, o.y, o.z, o.w}, (u32x4*)(p.out + (long long)m * p.ldo + n));
       }
     }
-  }
+  };
+  if (p.residual) finish(std::true_type{});
+  else finish(std::false_type{});
 }
 
 // ------------------------------------------------------------------------------------------------------------ host

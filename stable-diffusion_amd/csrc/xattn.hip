@@ -275,8 +275,35 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void xattn_k
     l = lall;
     __syncthreads();
   }
-  if (rho >= p.rows) return;
   const float inv = l > 0.f ? 1.0f / l : 0.f;
+  if constexpr (WK == 1) {
+    if (p.splits == 1) {
+      // a lane has 8 bytes here and there of one row: turned in the wave's own piece of LDS, rows leave as whole lines (9216 rows to 77
+      // keys 12.2 -> 10.9 us, 576 rows to 231 24.7 -> 22.3).  Not past the L2: 9.9 and 21.2 alone, but the projection behind them reads
+      // the rows over and over (84 -> 89 us together)
+      constexpr int LD = DP + 8;  // the row, then where it goes
+      static_assert(4 * 32 * LD * 2 <= S::bytes, "the rows in the tiles' memory");
+      u16* const so = smem + wv * 32 * LD;
+      __syncthreads();
+#pragma unroll
+      for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *(uint2*)&so[r * LD + 32 * dt + 8 * g + 4 * hh] = make_uint2(pack2h(oacc[dt][4 * g] * inv, oacc[dt][4 * g + 1] * inv), pack2h(oacc[dt][4 * g + 2] * inv, oacc[dt][4 * g + 3] * inv));
+      if (hh == 0) *(long long*)&so[r * LD + DP] = rho < p.rows ? (long long)bz * p.so + (long long)qi * p.ldo + head * p.dim : -1;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's own writes
+      typedef u32x4 u32x4_a8 __attribute__((aligned(8)));
+#pragma unroll
+      for (int i = 0; i < CH / 2; ++i) {
+        const int piece = 64 * i + lane, row = piece / CH, ch = piece % CH;
+        const long long off = *(const long long*)&so[row * LD + DP];
+        const u32x4 v = *(const u32x4*)&so[row * LD + 8 * ch];
+        if (off >= 0 && 8 * ch < p.dim) *(u32x4_a8*)(p.o + off + 8 * ch) = v;
+      }
+      return;
+    }
+  }
+  if (rho >= p.rows) return;
   const long long prow = ((long long)bz * p.kvh + hk) * p.rows + rho;
   float* po = p.po + (prow * p.splits + sp) * p.dim;
   u16* O = p.o + (long long)bz * p.so + (long long)qi * p.ldo + head * p.dim;

@@ -201,6 +201,16 @@ def test_attention_writes_its_own_columns_only(nq, nkv):
     assert bool((buf[..., :8] == 7.0).all()) and bool((buf[..., 88:] == 7.0).all())
 
 
+@pytest.mark.parametrize("dim,off", [(64, 4), (40, 12), (256, 4), (32, 20), (96, 0), (160, 4)])
+def test_attention_rows_start_anywhere_on_8_bytes(dim, off):
+    q, k, v, kd, vd, _, _ = _attention_case(31, 2, 2, 2, 1, dim, 100, 77, lens=[77, 0])
+    buf = torch.full((2, 100, 2 * dim + 28), 3.0, dtype=H16, device=DEV)
+    _run_attention(q, kd, vd, 2, 1, dim, None, [77, 0], None, None, out=E.Act(buf, 2, 1, 100, 2 * dim + 28).cols(off, 2 * dim))
+    want, tol = _attention_oracle(q, k, v, 2, 1, dim, dim ** -0.5, None, [77, 0], None, None)
+    _close(buf[..., off:off + 2 * dim], want, tol, "attention, %d wide from column %d" % (dim, off))
+    assert bool((buf[..., :off] == 3.0).all()) and bool((buf[..., off + 2 * dim:] == 3.0).all())
+
+
 def test_attention_offsets_past_32_bits():
     """Rows 128 KB apart (the last one 5 GB behind the first) and contexts further still."""
     nkv, ld = 40000, 1 << 16
