@@ -15,7 +15,7 @@
 //   - many rows, whole tiles of one request (lora_gemm_kernel, MIXED = false): the adapters are more K.  Ranks up to 32: t is a
 //     by-product of the same K-loop (one launch).  Larger: behind the K-tiles of (x, w) come tiles of (t, b) through the same ring
 //     and MFMAs.  18432 x 640 -> 1920, 3 groups of rank 8: 66 us, 700 TFLOP/s (a library's product alone: 64); MFMAs are busy a third
-//     of the time, the 71 MB that leave at the blocks' ends and 10 K-steps a block cost the rest.  18432 x 320 -> 320: 14.4 us.
+//     of the time, the 71 MB that leave at the blocks' ends and 10 K-steps a block cost the rest.  18432 x 320 -> 320: 13.2 us.
 //     2304 x 1280 -> 1280, rank 64: 5.9 us for t, 19 us (460 TFLOP/s), bound by what the LDS delivers to 32 x 32 wave tiles and by
 //     2.8 blocks to a CU (larger tiles: fewer blocks than CUs; measured 20 - 21 us).
 //   - many rows of small requests (MIXED = true): the same with tiles over rows in the order of their adapters.  1155 rows, 5

@@ -19,7 +19,7 @@
 // for each MFMA's - 2 x 10 heads of 64, 2304 rows to 9216 keys 142 us, 766 TFLOP/s; 96 x 96 rows 310 us, 701; heads of 128 to 4096 keys
 // 126 us, 615; 160: 130 us, 742; 80: 78 us, 616; 256 (one wave to a SIMD): 155 us, 497.  The prompt's lengths the start of a block (Q, the
 // first tile, the store: memory latencies behind one another, two to four blocks to a CU to cover them) - 2 x 5 heads, 9216 rows to
-// 77 keys 12.1 us, 16 x 20 heads, 576 rows to 231 shared keys 24 us, 2304 rows to 154 keys in regions 15.0 us.  One row the reading
+// 77 keys 11.0 us, 16 x 20 heads, 576 rows to 231 shared keys 22.4 us, 2304 rows to 154 keys in regions 14.2 us.  One row the reading
 // of the keys - 320 rows to 9216 keys (755 MB) 138 + 5 us, 5.3 TB/s; 8 x 16 heads of 128 on 4, 4096 keys (38 MB where half exist) 13.6 + 4 us.
 #include "common.h"
 #include <atomic>
