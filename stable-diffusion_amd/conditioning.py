@@ -47,6 +47,7 @@ class EncoderStates(object):
         if index is None and n != 1 and n != b:
             raise L.SdmiError("EncoderStates: %d contexts for %d samples need an index" % (n, b))
         self.batch = b                      # None: one context for a batch of any size
+        self.pair = None                    # GuidancePair of the two sides that cat() put together
         self.index = _words(index, (b,), dev, "index")
         self.key_regions = _words(key_regions, (n, t), dev, "key_regions")
         self._levels = {}                   # (h, w) -> (b, h * w) sets of the positions of that level
@@ -86,18 +87,28 @@ class EncoderStates(object):
         s = lambda v: None if v is None else tuple(v.shape)
         return (s(self.tokens), str(self.tokens.device), self.batch, s(self.lens), s(self.index), s(self.key_regions), s(self.query_regions))
 
+    @property
+    def shared(self):
+        """Whether samples pick their contexts by an index, or all read one: the samples' adapters then do not say the contexts'."""
+        return self.index is not None or self.batch != self.tokens.shape[0]
+
     def copy_(self, other):
         """Takes over another batch's values in place."""
         if other.signature() != self.signature():
             raise L.SdmiError("EncoderStates.copy_: %s cannot take %s" % (self.signature(), other.signature()))
+        if self.pair is not None and other.pair is not None and (self.pair.counts, self.pair.shared) != (other.pair.counts, other.pair.shared):
+            raise L.SdmiError("EncoderStates.copy_: sides of %s contexts cannot take sides of %s" % (self.pair.counts, other.pair.counts))
         for name in ("tokens", "lens", "index", "key_regions", "query_regions"):
             if getattr(self, name) is not None:
                 getattr(self, name).copy_(getattr(other, name))
+        self.pair = other.pair
         self._fill_levels()
         return self
 
     def clone(self):
-        return EncoderStates(self.tokens, self.lens, self.index, self.key_regions, self.query_regions)
+        twin = EncoderStates(self.tokens, self.lens, self.index, self.key_regions, self.query_regions)
+        twin.pair = self.pair
+        return twin
 
     @staticmethod
     def cat(a, b, batch=None):
@@ -128,7 +139,31 @@ class EncoderStates(object):
             if a.query_regions is not None and b.query_regions is not None and a.query_regions.shape[1:] != b.query_regions.shape[1:]:
                 raise L.SdmiError("EncoderStates.cat: query_regions of %s and %s" % (tuple(a.query_regions.shape), tuple(b.query_regions.shape)))
             kr, qr = torch.cat([pad(keys(a)), pad(keys(b))]), torch.cat([queries(a, ba), queries(b, bb)])
-        return EncoderStates(torch.cat([pad(a.tokens), pad(b.tokens)]), lens_ab, index, kr, qr)
+        both = EncoderStates(torch.cat([pad(a.tokens), pad(b.tokens)]), lens_ab, index, kr, qr)
+        both.pair = GuidancePair(a, b)
+        return both
+
+
+class GuidancePair(object):
+    """The contexts of the two sides of a guidance batch [uncond | cond], EncoderStates or plain (b, T, C) tokens: how many, whether
+    samples share them, and which sample reads which.  The same for one object that holds both sides and for an object of each."""
+
+    def __init__(self, uncond, cond):
+        sides = (uncond, cond)
+        self.counts = tuple((s.tokens if isinstance(s, EncoderStates) else s).shape[0] for s in sides)
+        self.shared = tuple(isinstance(s, EncoderStates) and s.shared for s in sides)
+        self._index = tuple(s.index.clone() if shared and s.index is not None else None for s, shared in zip(sides, self.shared))
+
+    def alike(self):
+        """Whether every sample reads the same place among the contexts on both sides.  Waits for the GPU where both have an index."""
+        (na, nb), (sa, sb), (ia, ib) = self.counts, self.shared, self._index
+        if na != nb or sa != sb or (ia is None) != (ib is None):
+            return False
+        if ia is None:
+            return True
+        if ia.is_cuda and torch.cuda.is_current_stream_capturing():
+            return False                    # not to be asked there
+        return torch.equal(ia, ib)
 
 
 class LayerAdapters(object):
@@ -232,8 +267,12 @@ class AdapterSet(object):
         return buf
 
     def select(self, ids, context_ids=None):
-        """The adapters of the next batch, written where a step captured for a batch of this size reads them.  A ContextKV made
-        before has to be made or updated again, as Sampler.sample does."""
+        """The adapters of the next batch, written where a step captured for a batch of this size reads them: ids, one for each
+        sample; context_ids, one for each context of the states that come with it.  Of the two sides that a sampler takes
+        [uncond | cond], context_ids are the conditional one's, or the unconditional one's followed by the conditional one's.  A
+        side (or states) that they leave out goes by the samples' ids where every sample has a context of its own, and by the same
+        context_ids where both sides are laid out alike; anything else is refused.  A ContextKV made before has to be made or
+        updated again, as Sampler.sample does."""
         self.ids = self._keep("ids", ids)
         self.context_ids = None if context_ids is None else self._keep("contexts", context_ids)
         return self
@@ -250,10 +289,51 @@ class AdapterSet(object):
             raise L.SdmiError("AdapterSet: select(ids) first")
         return self._take(self.ids, n, "samples")
 
-    def ids_for_contexts(self, n, shared):
-        """The ids of n contexts; shared: samples pick theirs by an index (or all read one), so the samples' ids do not say."""
-        if self.context_ids is not None:
-            return self._take(self.context_ids, n, "contexts")
-        if shared:
-            raise L.SdmiError("AdapterSet: samples share contexts, whose to_k / to_v have adapters: say which (select(ids, context_ids))")
-        return self.ids_for(n)
+    def _one_id(self, n):
+        """One id was selected for all samples: it is any context's as well."""
+        return self.ids[:1].expand(n).contiguous() if self.ids is not None and self.ids.numel() == 2 else None
+
+    def ids_for_contexts(self, n, shared, pair=None, side=None):
+        """The ids of n contexts; shared: samples pick theirs by an index (or all read one), so the samples' ids do not say.
+        pair: the GuidancePair that the contexts belong to; side: 0 uncond, 1 cond, None both in a row."""
+        if pair is not None:
+            return self._ids_for_pair(n, pair, side)
+        if self.context_ids is None:
+            if not shared:
+                return self.ids_for(n)
+            one = self._one_id(n)
+            if one is None:
+                raise L.SdmiError("AdapterSet: samples share contexts, whose to_k / to_v have adapters: say which (select(ids, context_ids))")
+            return one
+        have = self.context_ids.numel() // 2
+        # contexts of the samples' own, twice as many as ids of either kind: a batch [uncond | cond]
+        if n == have or (not shared and n == 2 * have and self.ids is not None and self.ids.numel() == n):
+            return self.context_ids[:n]
+        raise L.SdmiError("AdapterSet: %d ids for %d contexts" % (have, n))
+
+    def _ids_for_pair(self, n, pair, side):
+        given, have = self.context_ids, 0 if self.context_ids is None else self.context_ids.numel() // 2
+        na, nb = pair.counts
+        if n != (na + nb if side is None else pair.counts[side]):
+            raise L.SdmiError("AdapterSet: %d contexts, where the sides of this batch have %d and %d" % (n, na, nb))
+        if given is not None and have not in (nb, na + nb):
+            raise L.SdmiError("AdapterSet: %d context_ids for %d unconditional and %d conditional contexts: give the conditional ones', or all of them" % (have, na, nb))
+
+        def of(s):
+            m = pair.counts[s]
+            if have == na + nb:
+                return given[:na] if s == 0 else given[na:have]
+            if given is not None and (s == 1 or pair.alike()):
+                return given[:m]
+            if not pair.shared[s]:
+                if self.ids is None:
+                    raise L.SdmiError("AdapterSet: select(ids) first")
+                if self.ids.numel() != 2 * m:
+                    raise L.SdmiError("AdapterSet: %d ids for %d samples" % (self.ids.numel() // 2, m))
+                return self.ids[:m]
+            one = self._one_id(m)
+            if one is None:
+                raise L.SdmiError("AdapterSet: samples share the %s contexts, whose to_k / to_v have adapters: say which (select(ids, context_ids), the "
+                                  "unconditional ones' first)" % ("unconditional", "conditional")[s])
+            return one
+        return torch.cat([of(0), of(1)]) if side is None else of(side)

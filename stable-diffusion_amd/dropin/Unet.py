@@ -95,13 +95,13 @@ class Unet(nn.Module):
         self.adapters = adapters.attach() if adapters is not None else None
 
     @torch.no_grad()
-    def precompute_context(self, context):
+    def precompute_context(self, context, pair=None, side=None):
         """Project the (2b, 77, 1024) text context through every cross-attention to_k / to_v once.  The result can be
         passed as `context=` to forward() for every DDIM step of the same prompt (step-invariant hoisting).  context: that
-        tensor, or conditioning.EncoderStates (forward() takes either as well)."""
+        tensor, or conditioning.EncoderStates (forward() takes either as well).  pair, side: see ContextKV."""
         if isinstance(context, list):
             context = context[0]
-        return ContextKV(list(self._cross_attn_modules()), context)
+        return ContextKV(list(self._cross_attn_modules()), context, pair, side)
 
     def _embeddings(self, timesteps):
         """t_emb MLP (Unet.py:112-114) + every ResBlock's emb_proj(SiLU(t_emb)) (layers/ResBlock.py:70), batched."""

@@ -26,42 +26,45 @@ class ContextKV(object):
     (they depend only on the prompt, not on the latent or the timestep: 32 Linears per UNet step in the reference,
     layers/SpatialTransformer.py:73-74).  `kv[id(attn_module)]` is that layer's (B, 77, 2*inner) view.
     states: the EncoderStates the tokens came from (lengths, contexts and regions for the attention), None for plain tokens.
-    Layers whose to_k / to_v have adapters are projected again with them, into the same columns."""
+    Layers whose to_k / to_v have adapters are projected again with them, into the same columns.
+    pair, side: where the contexts belong to a guidance batch (conditioning.GuidancePair), that batch and which of its sides they
+    are (0 uncond, 1 cond, None both): what the ids of the adapters go by."""
 
-    def __init__(self, attn_modules, context):
+    def __init__(self, attn_modules, context, pair=None, side=None):
         self._modules = list(attn_modules)
         self._ws = tuple(w for m in self._modules for w in (m.to_k.weight, m.to_v.weight))
         self._ntot = sum(w.shape[0] for w in self._ws)
         self._allkv = None
         self.states = context.clone() if isinstance(context, EncoderStates) else None
         self.kv = {}
-        self.update(context)
+        self.update(context, pair, side)
 
-    def update(self, context):
+    def update(self, context, pair=None, side=None):
         """Project a new prompt INTO THE SAME BUFFERS (same batch and token count): a HIP graph captured over a forward
         that read this object stays valid, which is how the sampler reuses one captured step across images."""
         if isinstance(context, EncoderStates) != (self.states is not None):
             raise E.L.SdmiError("ContextKV.update: plain tokens and EncoderStates do not take each other's place")
         if self.states is not None:
             context = self.states.copy_(context).tokens
+            if pair is None:
+                pair = self.states.pair
         ctx = context if isinstance(context, E.Act) else E.tokens_from_f32(context)
         if self._allkv is not None:
             assert (ctx.n, ctx.h * ctx.w) == self._shape, "ContextKV.update: batch / token count changed"
         self._shape = (ctx.n, ctx.h * ctx.w)
         self._allkv = E.gemm(ctx, E.packed_linear(self._ws), self._ntot, out=self._allkv)
-        off = 0
+        off, ids = 0, {}
         for m in self._modules:
             n2 = m.to_k.weight.shape[0] + m.to_v.weight.shape[0]
             if id(m) not in self.kv:
                 self.kv[id(m)] = self._allkv.cols(off, n2)
             off += n2
             if m.adapters is not None and m.adapters.pack("kv") is not None:
-                m.project_context(ctx, self.shared, out=self.kv[id(m)])
+                owner = m.adapters.owner
+                if owner not in ids:
+                    ids[owner] = owner.ids_for_contexts(ctx.n, self.states is not None and self.states.shared, pair, side)
+                m.project_context(ctx, ids[owner], out=self.kv[id(m)])
         return self
-
-    @property
-    def shared(self):
-        return self.states is not None and (self.states.index is not None or self.states.batch != self.states.tokens.shape[0])
 
     def serves(self, n):
         """Whether a batch of n samples can read this context."""
@@ -73,8 +76,6 @@ class _StatesIn(object):
 
     def __init__(self, states):
         self.states, self.act = states, E.tokens_from_f32(states.tokens)
-
-    shared = ContextKV.shared
 
 
 def _as_ctx(context):
@@ -152,13 +153,14 @@ class MemoryEfficientCrossAttention(nn.Module):
         x = E.layernorm(a, ln.weight, ln.bias, ln.eps) if ln is not None else a
         return E.lora_gemm(x, E.packed_linear(ws, scales=scales), n, pack, self.adapters.owner.ids_for(a.n))
 
-    def project_context(self, ctx, shared=False, out=None):
-        """to_k | to_v of the context's tokens, with the adapters this layer has for them."""
+    def project_context(self, ctx, ids=None, out=None):
+        """to_k | to_v of the context's tokens, with the adapters this layer has for them: ids, one for each context (default: the
+        samples')."""
         ws, pack = (self.to_k.weight, self.to_v.weight), self._pack("kv")
         n = ws[0].shape[0] + ws[1].shape[0]
         if pack is None:
             return E.gemm(ctx, E.packed_linear(ws), n, out=out)
-        return E.lora_gemm(ctx, E.packed_linear(ws), n, pack, self.adapters.owner.ids_for_contexts(ctx.n, shared), out=out)
+        return E.lora_gemm(ctx, E.packed_linear(ws), n, pack, self.adapters.owner.ids_for_contexts(ctx.n, False) if ids is None else ids, out=out)
 
     def run(self, a, context=None, residual=None, ln=None, rowstats=False):
         """ln: the LayerNorm module in front of this layer (BasicTransformerBlock.norm1/2): `a` is then the UN-normalised
@@ -179,10 +181,12 @@ class MemoryEfficientCrossAttention(nn.Module):
             if isinstance(context, ContextKV):
                 kv, states = context.kv[id(self)], context.states
             else:
-                shared = False
+                ids = None
                 if isinstance(context, _StatesIn):
-                    states, shared, context = context.states, context.shared, context.act
-                kv = self.project_context(context, shared)
+                    states, context = context.states, context.act
+                    if self._pack("kv") is not None:
+                        ids = self.adapters.owner.ids_for_contexts(context.n, states.shared, states.pair)
+                kv = self.project_context(context, ids)
             k, v = kv.cols(0, inner), kv.cols(inner, inner)
             # LayerNorm + to_q inside the attention kernel where the engine offers it (one launch less)
             if ln is not None and states is None and self._pack("q") is None:

@@ -97,25 +97,26 @@ class Sampler(object):
         The objects are owned by the sampler and refilled IN PLACE for every prompt of the same batch size: the captured
         UNet step reads their buffers, so they must not move between images.  Either side may be EncoderStates; batch: samples
         of a half, for states that say nothing of it."""
-        from .conditioning import EncoderStates
+        from .conditioning import EncoderStates, GuidancePair
         states = isinstance(cond, EncoderStates) or isinstance(uncond, EncoderStates)
         if states:
             cond, uncond = EncoderStates.of(cond), EncoderStates.of(uncond)
         sig = lambda v: v.signature() if states else (tuple(v.shape), str(v.device))
         key = (sig(uncond), sig(cond), self.dual_stream, self.cfg_group is not None, batch if states else None)
         own = (lambda v: v) if states else (lambda v: v.contiguous())
+        pair = GuidancePair(uncond, cond)                       # adapters of to_k / to_v: ids go by the side
         if self.cfg_group is not None:
-            halves = (own((uncond, cond)[self.cfg_role]),)      # this rank's half only
+            halves = ((own((uncond, cond)[self.cfg_role]), self.cfg_role),)      # this rank's half only
         elif self.dual_stream:
-            halves = (own(uncond), own(cond))
+            halves = ((own(uncond), 0), (own(cond), 1))
         else:
-            halves = (EncoderStates.cat(uncond, cond, batch) if states else torch.cat([uncond, cond]).contiguous(),)
+            halves = ((EncoderStates.cat(uncond, cond, batch) if states else torch.cat([uncond, cond]).contiguous(), None),)
         if getattr(self, "_cc_key", None) != key:
-            self._cc = tuple(self.unet.precompute_context(h) for h in halves)
+            self._cc = tuple(self.unet.precompute_context(h, pair, side) for h, side in halves)
             self._cc_key = key
         else:
-            for c, h in zip(self._cc, halves):
-                c.update(h)
+            for c, (h, side) in zip(self._cc, halves):
+                c.update(h, pair, side)
         return self._cc if (self.dual_stream and self.cfg_group is None) else self._cc[0]
 
     def _static_xc(self, shape, dev):

@@ -12,7 +12,7 @@ import torch
 import sd_oracle as O
 from conftest import rel_err
 from stable_diffusion_amd import engine as E, _lib as L
-from stable_diffusion_amd.conditioning import AdapterSet, EncoderStates
+from stable_diffusion_amd.conditioning import AdapterSet, EncoderStates, GuidancePair
 from stable_diffusion_amd.synth import fill_state_dict, make_inputs
 
 DEV = "cuda"
@@ -354,3 +354,133 @@ def test_a_set_belongs_to_its_model(monkeypatch):
         unet = Unet()
     with pytest.raises(L.SdmiError, match="another model"):
         unet.set_adapters(AdapterSet(_layer(), [{"transformer_blocks.0.attn1.to_q": (torch.zeros(4, 64), torch.zeros(64, 4))}]))
+
+# ------------------------------------------------------------------------------------------------------------ adapters of contexts, side by side
+def _set_on_host(monkeypatch, n=3):
+    """An AdapterSet with n adapters on a layer's to_k (attn2), on the host."""
+    monkeypatch.setattr(E, "_need_cuda", lambda t, what: None)
+    return AdapterSet(_layer(), [{"transformer_blocks.0.attn2.to_k": (torch.zeros(3, 1024), torch.zeros(64, 3))}] * n)
+
+
+def _side(n, index=None):
+    return EncoderStates(torch.zeros(n, 5, 8), index=index)
+
+
+def test_each_side_of_a_guidance_batch_has_its_own_adapters(monkeypatch):
+    """Four samples on two prompts beside ordinary negatives, and the other layouts: for each side as for both in one object."""
+    s, plain = _set_on_host(monkeypatch), torch.zeros(4, 7, 8)
+    cases = [  # uncond, cond, ids, context_ids, what the sides read (None: refused)
+        (plain, _side(2, [0, 0, 1, 1]), [0, 0, 1, 1], [0, 1], ([0, 0, 1, 1], [0, 1])),
+        (plain, _side(2, [0, 0, 1, 1]), [0, 0, 1, 1], [2, -1, 2, -1, 0, 1], ([2, -1, 2, -1], [0, 1])),
+        (plain, _side(2, [0, 0, 1, 1]), [0, 0, 1, 1], None, None),
+        (plain, _side(2, [0, 0, 1, 1]), [0, 0, 1, 1], [0, 1, 0], None),
+        (_side(1), _side(2, [0, 0, 1, 1]), [0, 0, 1, 1], [0, 1], None),                     # the shared negative's is not said
+        (_side(1), _side(2, [0, 0, 1, 1]), [0, 0, 1, 1], [-1, 0, 1], ([-1], [0, 1])),
+        (_side(2, [0, 0, 1, 1]), _side(4), [0, 0, 1, 1], [2, 1], None),                     # not twice the list
+        (_side(2, [0, 0, 1, 1]), _side(4), [0, 0, 1, 1], [2, 1, 0, 0, 1, 1], ([2, 1], [0, 0, 1, 1])),
+        (_side(2, [0, 0, 1, 1]), _side(2, [0, 0, 1, 1]), [0, 0, 1, 1], [0, 1], ([0, 1], [0, 1])),
+        (_side(2, [0, 1, 0, 1]), _side(2, [0, 0, 1, 1]), [0, 0, 1, 1], [0, 1], None),       # as many, read by others
+        (_side(3, [2, 0, 1]), torch.zeros(3, 5, 8), [0, 1, -1], [1, 2, 0], None),
+        (torch.zeros(3, 5, 8), _side(3, [2, 0, 1]), [0, 1, -1], [1, -1, 0], ([0, 1, -1], [1, -1, 0])),
+        (plain, plain, [0, 1, 2, -1], None, ([0, 1, 2, -1], [0, 1, 2, -1])),
+        (plain, plain, [0, 1, 2, -1], [1, 1, 0, 2], ([1, 1, 0, 2], [1, 1, 0, 2])),
+        (plain, plain, [0, 1], None, None),
+        (_side(1), _side(1), [1], None, ([1], [1])),                                        # one sample: its contexts are its own
+        (plain[:1], _side(3, [2]), [1], None, ([1], [1, 1, 1])),
+        (_side(1), _side(1), [1, 0], None, None),
+        (_side(1), _side(1), [1, 0], [2], ([2], [2])),
+    ]
+    for uncond, cond, ids, cids, want in cases:
+        s.select(ids, cids)
+        pair = GuidancePair(uncond, cond)
+        both = EncoderStates.cat(EncoderStates.of(uncond), EncoderStates.of(cond), batch=len(ids))
+        counts = pair.counts
+        ask = [lambda: s.ids_for_contexts(counts[0], pair.shared[0], pair, 0), lambda: s.ids_for_contexts(counts[1], pair.shared[1], pair, 1),
+               lambda: s.ids_for_contexts(sum(counts), both.shared, both.pair), lambda: s.ids_for_contexts(sum(counts), both.shared, both.clone().pair)]
+        if want is None:
+            refused = 0
+            for f in ask:
+                try:
+                    f()
+                except L.SdmiError:
+                    refused += 1
+            assert refused >= 3, (ids, cids)                                                # a side that the list names may have its ids
+        else:
+            assert [f().tolist() for f in ask] == [want[0], want[1], want[0] + want[1], want[0] + want[1]], (ids, cids)
+    with pytest.raises(L.SdmiError, match="sides of this batch"):
+        s.ids_for_contexts(3, False, pair, 0)
+
+
+def test_ids_of_contexts_by_themselves(monkeypatch):
+    s = _set_on_host(monkeypatch)
+    s.select([0, 1], [1, 2])
+    assert s.ids_for_contexts(2, True).tolist() == [1, 2] and s.ids_for_contexts(2, False).tolist() == [1, 2]
+    assert s.ids_for_contexts(4, False).tolist() == [1, 2, 1, 2]                            # [uncond | cond], a context for each sample
+    for n, shared in ((4, True), (3, True), (1, False)):
+        with pytest.raises(L.SdmiError, match="contexts"):
+            s.ids_for_contexts(n, shared)
+    s.select([0, 1, 2, 0], [1, 2])
+    with pytest.raises(L.SdmiError, match="contexts"):
+        s.ids_for_contexts(4, False)                                                        # not a batch of twice the samples
+    assert s.select([2]).ids_for_contexts(1, True).tolist() == [2] and s.ids_for_contexts(3, True).tolist() == [2, 2, 2]
+
+
+def test_states_that_cat_made_keep_their_sides(monkeypatch):
+    monkeypatch.setattr(E, "_need_cuda", lambda t, what: None)
+    make = lambda a, b: EncoderStates.cat(a, b, batch=4)
+    one, two = make(_side(2, [0, 0, 1, 1]), _side(4)), make(_side(2, [0, 1, 0, 1]), _side(4))
+    one.copy_(two)
+    assert one.pair is two.pair and one.index.tolist() == [0, 1, 0, 1, 2, 3, 4, 5]
+    with pytest.raises(L.SdmiError, match="sides"):
+        one.copy_(make(_side(4), _side(2, [0, 1, 0, 1])))
+    loose = EncoderStates(torch.zeros(6, 5, 8), index=[0] * 8)
+    assert loose.copy_(one).pair is one.pair                                                # as before, states of any origin
+
+
+@pytest.fixture(scope="module")
+def side_refs(net):
+    """eps of every sample with its own merged weights: cond, uncond with the sample's adapter, uncond of one shared negative."""
+    unet, sd = net
+    rs = np.random.RandomState(21)
+    x, tokens, t = _rand(rs, 4, 9, 16, 16), _rand(rs, 2, 60, 1024), torch.tensor([481] * 4)
+    plain, one = _rand(rs, 4, 77, 1024), _rand(rs, 1, 40, 1024)
+    ads, ids, index, lens = _unet_adapters(rs, sd, 0.3), [0, 0, 1, 1], [0, 0, 1, 1], [60, 33]
+    eps = lambda i, ic, ctx: O.unet_forward(_merged(sd, ads, ids[i], ic), x[i:i + 1], t[i:i + 1], ctx)
+    with torch.no_grad():
+        cond = [eps(i, index[i], tokens[index[i]:index[i] + 1, :lens[index[i]]]) for i in range(4)]
+        own = [eps(i, ids[i], plain[i:i + 1]) for i in range(4)]
+        shared = [eps(i, 1, one) for i in range(4)]
+    return dict(x=x, tokens=tokens, t=t, plain=plain, one=one, ads=ads, ids=ids, index=index, lens=lens, cond=cond, own=own, shared=shared)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("negatives", ["plain", "one"])
+@pytest.mark.parametrize("dual", [True, False])
+def test_sampler_gives_each_side_its_own_adapters(net, side_refs, dual, negatives):
+    """Two prompts for four samples beside four plain negatives, or beside one for all of them (its adapter said first)."""
+    from stable_diffusion_amd.sampler import Sampler
+    unet, _ = net
+    r = side_refs
+    dev = lambda v: v.to(DEV)
+    cond = EncoderStates(dev(r["tokens"]), r["lens"], r["index"])
+    uncond, cids, refs = (dev(r["plain"]), [0, 1], r["own"]) if negatives == "plain" else (EncoderStates(dev(r["one"])), [1, 0, 1], r["shared"])
+    try:
+        unet.set_adapters(AdapterSet(unet, r["ads"]).select(r["ids"], cids))
+        xc, t = dev(r["x"]).repeat(2, 1, 1, 1), dev(r["t"]).repeat(2)
+        got = []
+        for use_graph in (False, True):
+            s = Sampler(unet, None, dual_stream=dual)
+            eps = s._unet_step(xc, t, s.make_context(uncond, cond, 4), use_graph, same_halves=True).clone()
+            for i in range(4):
+                _gate(eps[i:i + 1], refs[i], 7e-3, 6e-3, "uncond, sample %d" % i)
+                _gate(eps[4 + i:5 + i], r["cond"][i], 7e-3, 6e-3, "cond, sample %d" % i)
+            got.append(eps)
+        assert torch.equal(got[0], got[1])
+        inp = make_inputs(4, 16, 2, seed=51)
+        args = (2, cond, uncond, dev(inp["c_concat"]), dev(inp["x_T"]), [dev(n) for n in inp["noises"]], 7.5)
+        s = Sampler(unet, None, dual_stream=dual)
+        eager = s.sample(*args, decode=False)[0]
+        for _ in range(2):
+            assert torch.equal(s.sample(*args, decode=False, use_graph=True)[0], eager)
+    finally:
+        unet.set_adapters(None)
