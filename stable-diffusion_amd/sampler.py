@@ -101,6 +101,9 @@ class Sampler(object):
         states = isinstance(cond, EncoderStates) or isinstance(uncond, EncoderStates)
         if states:
             cond, uncond = EncoderStates.of(cond), EncoderStates.of(uncond)
+            for side, what in ((uncond, "unconditional"), (cond, "conditional")):
+                if batch is not None and side.batch not in (None, batch):
+                    raise E.L.SdmiError("Sampler: the %s states are for %d samples, the batch has %d" % (what, side.batch, batch))
         sig = lambda v: v.signature() if states else (tuple(v.shape), str(v.device))
         key = (sig(uncond), sig(cond), self.dual_stream, self.cfg_group is not None, batch if states else None)
         own = (lambda v: v) if states else (lambda v: v.contiguous())

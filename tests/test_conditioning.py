@@ -484,3 +484,19 @@ def test_sampler_gives_each_side_its_own_adapters(net, side_refs, dual, negative
             assert torch.equal(s.sample(*args, decode=False, use_graph=True)[0], eager)
     finally:
         unet.set_adapters(None)
+
+
+@pytest.mark.parametrize("dual", [True, False])
+def test_sampler_refuses_states_of_another_number_of_samples(monkeypatch, dual):
+    """One and three samples in the sides of a batch of two: as many in all, but not each sample's own."""
+    from stable_diffusion_amd.sampler import Sampler
+    monkeypatch.setattr(E, "_need_cuda", lambda t, what: None)
+
+    class Net(object):
+        def precompute_context(self, context, pair=None, side=None):
+            return context
+    s = Sampler(Net(), None, dual_stream=dual)
+    for uncond, cond, what in ((_side(1, [0]), _side(2, [0, 1, 1]), "unconditional"), (_side(2), _side(3), "conditional")):
+        with pytest.raises(L.SdmiError, match="the %s states are for" % what):
+            s.make_context(uncond, cond, 2)
+    s.make_context(_side(1), _side(2), 2)
