@@ -10,6 +10,18 @@ from . import _lib as L
 from . import engine as E
 
 
+def _int32(v, dev, sets=False):
+    """Integers as int32 on `dev`, a copy.  Numbers past 32 bits stay past every count that they are compared with; of sets the bits
+    count, and a bit past the 32nd is refused."""
+    if v.dtype in (torch.int64, torch.uint32):
+        v = v.to(device=dev, dtype=torch.int64)
+        if not sets:
+            v = v.clamp(-2 ** 31, 2 ** 31 - 1)
+        elif v.numel() and not (v.is_cuda and torch.cuda.is_current_stream_capturing()) and bool(((v < -2 ** 31) | (v >= 2 ** 32)).any()):
+            raise L.SdmiError("EncoderStates: sets of regions are 32 bits")
+    return v.to(device=dev, dtype=torch.int32, copy=True).contiguous()
+
+
 def _words(v, shape, dev, what):
     """An integer tensor of this shape as its own contiguous int32 on `dev` (sets of 32 regions keep their bits)."""
     if v is None:
@@ -17,7 +29,7 @@ def _words(v, shape, dev, what):
     v = torch.as_tensor(v)
     if v.is_floating_point() or v.is_complex() or tuple(v.shape) != tuple(shape):
         raise L.SdmiError("EncoderStates: %s has to be integers of shape %s, got %s %s" % (what, tuple(shape), v.dtype, tuple(v.shape)))
-    return v.to(device=dev, dtype=torch.int32, copy=True).contiguous()
+    return _int32(v, dev, what.endswith("regions"))
 
 
 class EncoderStates(object):
@@ -256,9 +268,10 @@ class AdapterSet(object):
         return self
 
     def _keep(self, what, v):
-        v = torch.as_tensor(v).to(device=self.device, dtype=torch.int32).reshape(-1)
-        if v.numel() == 0:
-            raise L.SdmiError("AdapterSet.select: no ids")
+        v = torch.as_tensor(v).reshape(-1)
+        if v.numel() == 0 or v.is_floating_point() or v.is_complex():
+            raise L.SdmiError("AdapterSet.select: %d ids of %s: at least one integer" % (v.numel(), v.dtype))
+        v = _int32(v, self.device)
         buf = self._buffers.get((what, v.numel()))
         if buf is None:
             buf = self._buffers[(what, v.numel())] = torch.empty((2 * v.numel(),), dtype=torch.int32, device=self.device)

@@ -500,3 +500,22 @@ def test_sampler_refuses_states_of_another_number_of_samples(monkeypatch, dual):
         with pytest.raises(L.SdmiError, match="the %s states are for" % what):
             s.make_context(uncond, cond, 2)
     s.make_context(_side(1), _side(2), 2)
+
+
+def test_numbers_past_32_bits_are_not_taken_for_others(monkeypatch):
+    """A length, a context or an adapter of 2^32 is past the end, not 0; a region past the 32nd is refused."""
+    s, big = _set_on_host(monkeypatch), 1 << 32
+    e = EncoderStates(torch.zeros(2, 5, 8), lens=[big, -big - 1], index=[big, 1])
+    assert e.lens.tolist() == [2 ** 31 - 1, -2 ** 31] and e.index.tolist() == [2 ** 31 - 1, 1]
+    assert EncoderStates.cat(e, e).index.tolist() == [-1, 1, -1, 3]
+    assert s.select([big, big + 2, -big, 1]).ids_for(4).tolist() == [2 ** 31 - 1, 2 ** 31 - 1, -2 ** 31, 1]
+    for v in ([0.0, 1.0], [0.7], torch.zeros(2, dtype=torch.bfloat16)):
+        with pytest.raises(L.SdmiError, match="integer"):
+            s.select(v)
+        with pytest.raises(L.SdmiError, match="integer"):
+            s.select([0, 1], v)
+    sets = lambda k, q: EncoderStates(torch.zeros(1, 2, 8), key_regions=torch.tensor([k]), query_regions=torch.tensor([[[q]]]))
+    assert sets([big - 1, -2 ** 31], -1).key_regions.tolist() == [[-1, -2 ** 31]]
+    for k, q in (([big, 1], 1), ([1, 1], big), ([1, -2 ** 31 - 1], 1)):
+        with pytest.raises(L.SdmiError, match="32 bits"):
+            sets(k, q)
