@@ -287,7 +287,7 @@ int sdmi_attention_log2q(const void* q, int ldq, int64_t sq, const void* k, int 
  *      with regions, where (query_regions[b * sqr + i] & key_regions[context * skr + j]) != 0: sets of up to 32 regions that a
  *      position of the picture and a token of the prompt belong to.
  *        o[b][i] = sum_j softmax_j(scale q.k) v over the keys that i sees; a row that sees none is 0.
- *      Memory of keys at or past lens[context] is not read, and a key in no region may hold anything (NaN too); every other key
+ *      o overlaps no operand.  Memory of keys at or past lens[context] is not read, and a key in no region may hold anything (NaN too); every other key
  *      has to be finite.  lens outside [0, nkv] count as the nearer end; an index outside [0, contexts) sees nothing.
  *      heads a multiple of kv_heads, dim a multiple of 8 up to 256, any nq >= 1 and nkv >= 0, scale in (0, 1e15].  ws: scratch of
  *      sdmi_cross_attention_ws_bytes for few rows over long states, whose keys are cut into pieces that a second launch joins
@@ -310,7 +310,8 @@ int sdmi_cross_attention_packed(const sdmi_cross_attention_args* args);
 /* ---- low-rank adapters of many requests beside one shared projection (no counterpart in the reference, whose Linears at
  *      layers/SpatialTransformer.py:62-66 have one set of weights):
  *        out[m] = x[m] w^T + t[m] b[id]^T (+ bias) (+ residual[m]),  t[m] = scale[id] x[m] a[id]^T,  id = ids[m / rows_per_id]
- *      x [m][k], w [n][k], out / residual [m][n]: h16, as sdmi_gemm (out may be residual's memory).  lora_a h16
+ *      x [m][k], w [n][k], out / residual [m][n]: h16, as sdmi_gemm (out may be residual's
+ *      memory, column for column, and no other operand's).  lora_a h16
  *      [adapters][groups * rank][k], lora_b h16 [adapters][n][rank], lora_scale fp32 [adapters], ids int32
  *      [ceil(m / rows_per_id)]; an id outside [0, adapters) leaves its rows without an adapter.  groups > 1: w stacks that many
  *      projections along n; group g is columns [g n / groups, (g + 1) n / groups) and rows [g rank, (g + 1) rank) of lora_a.

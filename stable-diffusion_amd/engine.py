@@ -587,10 +587,16 @@ def _int32(t, shape, what):
 
 
 def _apart(what, out, *inputs):
-    """`out` was given: it must not share columns of a buffer with an operand that other blocks are still reading."""
+    """`out` was given: its columns must not share memory with an operand that other blocks are still reading.  Buffers may be
+    views of one storage, so what counts is where the rows lie."""
+    o0, ld = out.ptr, out.ld
+    o1 = o0 + 2 * ((out.n * out.hw - 1) * ld + out.c)
     for a in inputs:
-        if a.buf.data_ptr() == out.buf.data_ptr() and a.off < out.off + out.c and out.off < a.off + a.c:
-            raise L.SdmiError("%s: `out` lies in an operand's memory" % what)
+        a0 = a.ptr
+        if a0 < o1 and o0 < a0 + 2 * ((a.n * a.hw - 1) * a.ld + a.c):
+            d = (a0 - o0) // 2 % ld             # the operand's first column, counted from out's
+            if a.ld != ld or d < out.c or d + a.c > ld:
+                raise L.SdmiError("%s: `out` lies in an operand's memory" % what)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -678,6 +684,8 @@ def lora_gemm(a, wp, n_out, lora, ids, bias=None, residual=None, out=None):
         if (residual.n * residual.hw, residual.c) != (m, n_out):
             raise L.SdmiError("lora_gemm: residual holds %d rows x %d channels, the product has %d x %d" % (residual.n * residual.hw, residual.c, m, n_out))
         flags, rp, rld = L.F_RESIDUAL, residual.ptr, residual.ld
+        if out is not None and (rp, rld) != (res.ptr, res.ld):       # every element of the residual is read where it is written, or apart
+            _apart("lora_gemm", res, residual)
     if bias is not None:
         if bias.dtype != torch.float32 or bias.shape != (n_out,) or not bias.is_contiguous():
             raise L.SdmiError("lora_gemm: bias is contiguous fp32 (%d,), got %s %s" % (n_out, bias.dtype, tuple(bias.shape)))

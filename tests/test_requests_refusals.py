@@ -52,6 +52,36 @@ def test_no_cpu_fallback():
         E.lora_gemm(a, torch.zeros((64, 64), dtype=h), 64, pack, torch.zeros(2, dtype=torch.int32))
 
 
+def test_out_apart_from_operands():
+    """An `out` whose columns share memory with an operand is refused, however the two are cut from one storage; the residual may
+    be out itself.  (Host tensors: what passes here is refused as such, before any launch.)"""
+    import torch
+    from stable_diffusion_amd import engine as E
+    h = E.act_dtype()
+    big = torch.zeros((4, 8, 192), dtype=h)
+    act = lambda buf, off, c: E.Act(buf, buf.shape[0], 1, buf.shape[1], buf.shape[2]).cols(off, c)
+    pack = E.LoraPack(torch.zeros((1, 8, 64), dtype=h), torch.zeros((1, 64, 8), dtype=h), torch.ones(1))
+    w, ids, x = torch.zeros((64, 64), dtype=h), torch.zeros(2, dtype=torch.int32), act(torch.zeros((2, 8, 64), dtype=h), 0, 64)
+    lora = lambda a, **kw: E.lora_gemm(a, w, 64, pack, ids, **kw)
+    att = lambda q, k, o: E.cross_attention(q, k, k, 1, out=o)
+    low, mid, top = big[0:2], big[1:3], big[2:4]
+    flat = big.view(-1)[:2 * 8 * 64].view(2, 8, 64)
+    shared = [lambda: lora(x, residual=act(low, 0, 64), out=act(low, 8, 64)),       # a residual that other columns overwrite
+              lambda: lora(x, residual=act(low, 0, 64), out=act(mid, 0, 64)), lambda: lora(x, residual=act(low, 64, 64), out=act(mid, 32, 64)),
+              lambda: lora(act(low, 0, 64), out=act(mid, 0, 64)), lambda: lora(act(mid, 0, 64), out=act(low, 40, 64)), lambda: lora(act(flat, 0, 64), out=act(low, 128, 64)),
+              lambda: lora(x, residual=act(flat, 0, 64), out=act(low, 0, 64)),
+              lambda: att(act(mid, 0, 64), x, act(low, 0, 64)), lambda: att(x, act(low, 128, 64), act(mid, 120, 64))]
+    apart = [lambda: lora(x, residual=act(low, 8, 64), out=act(low, 8, 64)), lambda: lora(x, residual=act(low, 0, 64), out=act(low, 64, 64)),
+             lambda: lora(x, residual=act(low, 0, 64), out=act(top, 0, 64)), lambda: lora(act(low, 0, 64), out=act(mid, 64, 64)), lambda: lora(act(mid, 128, 64), out=act(low, 64, 64)),
+             lambda: att(act(low, 0, 64), act(mid, 64, 64), act(low, 128, 64)), lambda: att(act(low, 0, 64), act(low, 0, 64), act(top, 0, 64))]
+    for f in shared:
+        with pytest.raises(L.SdmiError, match="memory"):
+            f()
+    for f in apart:
+        with pytest.raises(L.SdmiError, match="cpu"):
+            f()
+
+
 def _packed(fmt, args):
     return fmt.pack(*(0 if v is None else v for v in args.values()))
 
