@@ -693,9 +693,11 @@ def lora_gemm(a, wp, n_out, lora, ids, bias=None, residual=None, out=None):
     ip = _int32(ids, (nid,), "lora_gemm: ids")
     if nid == 0 or m % nid:
         raise L.SdmiError("lora_gemm: %d ids do not divide %d rows" % (nid, m))
-    _own_device("lora_gemm", ab, wp, lora.a, lora.b, lora.scale, ids, bias, None if residual is None else residual.buf, res.buf)
+    rb, ob = None if residual is None else residual.buf, res.buf
+    if ob.dtype is not ab.dtype or (rb is not None and rb.dtype is not ab.dtype):
+        raise L.SdmiError("lora_gemm: tokens %s, residual %s, out %s: the kernels take one type" % (ab.dtype, None if rb is None else rb.dtype, ob.dtype))
+    _own_device("lora_gemm", ab, wp, lora.a, lora.b, lora.scale, ids, bias, rb, ob)
     need = _ws_need("sdmi_lora_gemm_ws_bytes", m, n_out, k, lora.rank, lora.groups, m // nid)
-    ob = res.buf
     ws = ab.new_empty(((need + 1) // 2,)) if need else None     # the call's own: two graphs never share it
     L.call("sdmi_lora_gemm_packed", L.LORA_GEMM_ARGS.pack(
         ap, ab.shape[-1], wp.data_ptr(), wp.stride(0), ob.data_ptr() + 2 * res.off, ob.shape[-1], m, n_out, k, 0 if bias is None else bias.data_ptr(), rp, rld,

@@ -82,6 +82,19 @@ def test_out_apart_from_operands():
             f()
 
 
+def test_lora_refuses_a_residual_or_out_of_another_type():
+    import torch
+    from stable_diffusion_amd import engine as E
+    h = E.act_dtype()
+    act = lambda t: E.Act(torch.zeros((2, 8, 64), dtype=t), 2, 1, 8, 64)
+    pack = E.LoraPack(torch.zeros((1, 8, 64), dtype=h), torch.zeros((1, 64, 8), dtype=h), torch.ones(1))
+    w, ids = torch.zeros((64, 64), dtype=h), torch.zeros(2, dtype=torch.int32)
+    for t in (torch.float32, torch.int16, torch.bfloat16 if h is torch.float16 else torch.float16):
+        for kw in (dict(residual=act(t)), dict(out=act(t))):
+            with pytest.raises(L.SdmiError, match="one type"):
+                E.lora_gemm(act(h), w, 64, pack, ids, **kw)
+
+
 def _packed(fmt, args):
     return fmt.pack(*(0 if v is None else v for v in args.values()))
 
