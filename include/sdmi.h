@@ -287,11 +287,12 @@ int sdmi_attention_log2q(const void* q, int ldq, int64_t sq, const void* k, int 
  *      with regions, where (query_regions[b * sqr + i] & key_regions[context * skr + j]) != 0: sets of up to 32 regions that a
  *      position of the picture and a token of the prompt belong to.
  *        o[b][i] = sum_j softmax_j(scale q.k) v over the keys that i sees; a row that sees none is 0.
- *      o overlaps no operand.  Memory of keys at or past lens[context] is not read, and a key in no region may hold anything (NaN too); every other key
- *      has to be finite.  lens outside [0, nkv] count as the nearer end; an index outside [0, contexts) sees nothing.
- *      heads a multiple of kv_heads, dim a multiple of 8 up to 256, any nq >= 1 and nkv >= 0, scale in (0, 1e15].  ws: scratch of
- *      sdmi_cross_attention_ws_bytes for few rows over long states, whose keys are cut into pieces that a second launch joins
- *      in a fixed order; with NULL or fewer bytes they are not cut.  Calls that may overlap in time need a workspace each. */
+ *      o overlaps no operand.  Memory of keys at or past lens[context] is not read, and a key in no region may hold anything (NaN too);
+ *      every other key has to be finite, and (the bf16 build) dot products, scaled ones too, within 1e38.  lens outside [0, nkv] count as
+ *      the nearer end; an index outside [0, contexts) sees nothing.  heads a multiple of kv_heads, dim a multiple of 8 up to 256, any
+ *      nq >= 1 and nkv >= 0, scale in (0, 1e15].  ws: scratch of sdmi_cross_attention_ws_bytes for few rows over long states, whose keys
+ *      are cut into pieces that a second launch joins in a fixed order; with NULL or fewer bytes they are not cut.  Calls that may
+ *      overlap in time need a workspace each. */
 int sdmi_cross_attention(const void* q, int ldq, int64_t sq, const void* k, int ldk, int64_t sk, const void* v, int ldv, int64_t sv,
                          void* o, int ldo, int64_t so, int batch, int contexts, int heads, int kv_heads, int dim, int nq, int nkv,
                          const int32_t* index, const int32_t* lens, const uint32_t* query_regions, int64_t sqr,

@@ -281,6 +281,75 @@ def test_attention_refuses_tensors_of_another_kind():
             E.cross_attention(q, k, k, 1, out=out)
 
 
+FAR = [  # nq, nkv, dim, regions: a wave with a share of the tile or all of it, one partial tile, keys in pieces
+    (1, 1, 64, 0), (200, 1, 64, 0), (200, 77, 64, 0), (5, 77, 64, 0), (130, 600, 64, 0), (1, 2000, 64, 0), (70, 130, 32, 0), (100, 200, 96, 0), (3, 900, 128, 0),
+    (90, 140, 160, 0), (66, 100, 256, 0), (200, 154, 64, 3), (9, 600, 64, 3)]
+
+
+@pytest.mark.parametrize("x,y,scale", [(60000.0, 60000.0, None), (30000.0, 50000.0, None), (3.0, 2.0, 1e9), (100.0, -90.0, 1e9), (1.5, 1.25, 1e15), (0.75, -0.5, 1e15)])
+@pytest.mark.parametrize("nq,nkv,dim,regions", FAR)
+def test_attention_scores_far_apart(nq, nkv, dim, regions, x, y, scale):
+    """Scores up to 2^60 in magnitude, each row's best one ahead of the next by 2^64 or more in weight: its value comes out, to the bit.
+    Every score is one product, exact in fp32."""
+    rs = np.random.RandomState(nq + nkv + dim)
+    q, k, v = torch.zeros(1, nq, dim), torch.zeros(1, nkv, dim), _h(rs, 1, nkv, dim)
+    q[0, torch.arange(nq), torch.arange(nq) % dim] = x
+    # of the keys that meet a query, one after the other a step of the 16-bit type nearer to y
+    rank = torch.from_numpy(np.argsort(rs.rand(dim, nkv), 1)).t()
+    k[0] = (y * (1 - torch.clamp(rank, max=12) * 2 * U)).to(H16).float()
+    k[0][rank > 12] = float(-y)
+    q, k = q.to(H16), k.to(H16)
+    qr = kr = None
+    seen = torch.ones(nq, nkv, dtype=torch.bool)
+    if regions:
+        qr, kr = torch.from_numpy(rs.randint(0, 8, (1, nq))).to(torch.int32), torch.from_numpy(rs.randint(1, 8, (1, nkv))).to(torch.int32)
+        seen = (qr[0][:, None] & kr[0][None]) != 0
+    s = (q[0].double() @ k[0].double().t()).masked_fill(~seen, -math.inf)
+    top = s.topk(min(2, nkv), 1).values
+    ahead = top[:, 0] - top[:, -1] if nkv > 1 else torch.full((nq,), math.inf, dtype=torch.float64)
+    got = _run_attention(q, k, v, 1, 1, dim, None, None, qr, kr, scale=scale)[0].cpu()
+    for i in range(nq):
+        if not seen[i].any():
+            assert not got[i].any(), i
+        elif float(ahead[i]) * (dim ** -0.5 if scale is None else scale) > 64:
+            assert torch.equal(got[i], v[0, int(s[i].argmax())]), (i, got[i][:4], v[0, int(s[i].argmax())][:4])
+        else:                                               # a tie: neither of the values may be lost
+            best = torch.nonzero(s[i] == top[i, 0]).flatten()
+            mean = v[0, best].double().mean(0)
+            assert bool(((got[i].double() - mean).abs() <= 2 * U * mean.abs() + U * v[0, best].double().abs().mean(0) + TINY).all()), i
+
+
+@pytest.mark.parametrize("e", [-8, -5, -4, -3, 0, 4, 8, 12, 24])
+@pytest.mark.parametrize("nq,nkv,dim", [(200, 90, 64), (4, 90, 64), (3, 1500, 64), (130, 700, 64), (100, 150, 128), (2, 1000, 256)])
+def test_attention_near_ties_of_large_scores(nq, nkv, dim, e):
+    """Scores of 2^20 + d, d = 0, 1/8, ... 8, times 2^e: exact in fp32, so the weights are 2^-((8 - d) 2^e) however large they are.
+    The scale's rounding and log2(e)'s move an exponent by 2^-22 of itself at most (20 times that where the weight still counts)."""
+    rs = np.random.RandomState(e + 50)
+    q, k, v = torch.zeros(1, nq, dim), torch.zeros(1, nkv, dim), _h(rs, 1, nkv, dim)
+    d = torch.from_numpy(rs.randint(0, 65, nkv)) / 8.0
+    q[..., 0], q[..., 1], k[..., 0], k[0, :, 1] = 1024.0, 1.0, 1024.0, d.float()
+    scale = float(np.float32(math.log(2.0) * 2.0 ** e))
+    got = _run_attention(q.to(H16), k.to(H16), v, 1, 1, dim, None, None, None, None, scale=scale)
+    p = torch.exp2((d - d.max()).double() * (scale / math.log(2.0)))
+    o, a = p @ v[0].double() / p.sum(), p @ v[0].double().abs() / p.sum()
+    r = 20 * 2.0 ** -22 + 16 * E32
+    tol = U * (a + o.abs()) + (2 * r + 2 * (nkv + 64) * E32) * (a + o.abs()) + nkv * TINY * float(v.double().abs().max())
+    _close(got, o.expand(1, nq, dim), tol.expand(1, nq, dim), "attention, near ties of 2^%d" % (20 + e))
+
+
+@pytest.mark.skipif(H16 is torch.float16, reason="dot products of fp16 cannot lie past 2^40")
+@pytest.mark.parametrize("nq,nkv", [(200, 77), (2, 50), (1, 1500), (130, 700)])
+@pytest.mark.parametrize("x,y", [(2.0 ** 60, -2.0 ** 60), (-2.0 ** 50, 2.0 ** 60), (2.0 ** 60, 2.0 ** 60), (2.0 ** 62, -2.0 ** 64)])
+def test_attention_of_bf16_rows_far_from_zero(nq, nkv, x, y):
+    """Every score of a row past 1e30 in magnitude (down to -1e38): the mean of the values."""
+    q, k, v = torch.zeros(1, nq, 64), torch.zeros(1, nkv, 64), _h(np.random.RandomState(1), 1, nkv, 64)
+    q[..., 0], k[..., 0] = x, y
+    got = _run_attention(q.to(H16), k.to(H16), v, 1, 1, 64, None, None, None, None)
+    mean, mag = v[0].double().mean(0), v[0].double().abs().mean(0)
+    tol = U * mean.abs() + 2 * (nkv + 64) * E32 * mag
+    _close(got, mean.expand(1, nq, 64), tol.expand(1, nq, 64), "attention, rows of scores %g" % (x * y))
+
+
 # ------------------------------------------------------------------------------------------------------------ adapters
 def _lora_oracle(x, w, a, b, scale, ids, per, groups, bias, residual):
     x, w, a, b = x.double(), w.double(), a.double(), b.double()
