@@ -705,7 +705,22 @@ def lora_gemm(a, wp, n_out, lora, ids, bias=None, residual=None, out=None):
         ws.data_ptr() if need else 0, need, _stream()))
     if RANGE_AUDIT:
         _audit("lora_gemm %dx%dx%d" % (m, n_out, k), res)
+        _audit_low_rank(a, lora, ids)
     return res
+
+
+def _audit_low_rank(a, lora, ids):
+    """The 16-bit factor t between the two low-rank products, which stays inside the kernels: the same call with nothing beside the
+    adapters and an identity in place of b has it for its result."""
+    global RANGE_AUDIT
+    n = lora.groups * lora.rank
+    eye = torch.eye(lora.rank, dtype=lora.b.dtype, device=lora.b.device).repeat(lora.groups, 1).expand(lora.adapters, n, lora.rank).contiguous()
+    RANGE_AUDIT = False
+    try:
+        t = lora_gemm(a, lora.a.new_zeros((n, a.c)), n, LoraPack(lora.a, eye, lora.scale), ids)
+    finally:
+        RANGE_AUDIT = True
+    _audit("lora_gemm's low-rank factor %dx%dx%d" % (a.n * a.hw, n, a.c), t)
 
 
 def linear_small_m(x, wp, bias, silu_in=False):

@@ -506,6 +506,30 @@ def test_lora_residual_in_place():
     _close(stream.buf[0], want, tol, "lora, residual in place")
 
 
+@pytest.mark.skipif(H16 is torch.bfloat16, reason="bf16 does not saturate")
+@pytest.mark.parametrize("per,ids,groups,rank", [(1, [0, 1, -1], 1, 8), (1, [i % 3 - 1 for i in range(40)], 2, 16), (80, [1, 0], 3, 8), (80, [1, 0], 1, 64), (1, [i % 3 - 1 for i in range(160)], 1, 24)])
+def test_range_audit_sees_a_clipped_low_rank_factor(per, ids, groups, rank):
+    """x a^T past the 16-bit range while the result, through a small b, is well inside: reported, with how many of it."""
+    m, k, n = per * len(ids), 128, 48 * groups
+    x, w, a, b, scale, _, _ = _lora_case(1, m, k, n, groups, rank, 2, False, False)
+    x, b, scale = x.abs() + 1.0, b * 2.0 ** -14, torch.tensor([1.0, 500.0])
+    a = a.abs()
+    a[1, 3] = 8.0                                               # adapter 1, rank 3: a sum past 1024, times 500
+    want = sum(per for j in ids if j == 1)
+    E.RANGE_LOG.clear()
+    E.RANGE_AUDIT = True
+    try:
+        y = _run_lora(x, w, a, b, scale, ids, None, None)
+        assert torch.isfinite(y).all()
+        rows = [e for e in E.RANGE_LOG if "low-rank" in e[0]]
+        assert len(rows) == len(E.RANGE_LOG) == (1 if want else 0), E.RANGE_LOG
+        assert all(e[1:] == (m, groups * rank, want) for e in rows), E.RANGE_LOG
+        assert E.RANGE_AUDIT
+    finally:
+        E.RANGE_AUDIT = False
+        E.RANGE_LOG.clear()
+
+
 # ------------------------------------------------------------------------------------------------------------ streams and graphs
 def _both(seed, nq, nkv):
     """A projection with adapters whose result attends to encoder states, as a block of the UNet does; returns a function that runs it."""
