@@ -433,9 +433,11 @@ static bool xattn_shape_ok(int batch, int heads, int kv_heads, int dim, int nq, 
   return batch > 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && dim >= 8 && dim <= 256 && dim % 8 == 0 && nq > 0 && nkv >= 0 &&
          nkv < (1 << 30) && (long long)nq * (heads / kv_heads) < (1ll << 30) && (long long)heads * dim < (1ll << 22);
 }
+// a launch has fewer than 2^32 threads, and products with these two stay within 64 bits
+static bool xattn_grid_ok(int batch, int kv_heads) { return (long long)batch * kv_heads < (1ll << 24); }
 
 extern "C" int64_t sdmi_cross_attention_ws_bytes(int batch, int heads, int kv_heads, int dim, int nq, int nkv) {
-  if (!xattn_shape_ok(batch, heads, kv_heads, dim, nq, nkv)) return 0;
+  if (!xattn_shape_ok(batch, heads, kv_heads, dim, nq, nkv) || !xattn_grid_ok(batch, kv_heads)) return 0;
   const XattnPlan pl = xattn_plan(batch, kv_heads, dim, nq * (heads / kv_heads), nkv);
   return pl.splits == 1 ? 0 : (int64_t)batch * heads * nq * pl.splits * ((int64_t)dim * 4 + 8);
 }
@@ -448,6 +450,7 @@ extern "C" int sdmi_cross_attention(const void* q, int ldq, int64_t sq, const vo
   SDMI_REQUIRE(xattn_shape_ok(batch, heads, kv_heads, dim, nq, nkv),
                "cross_attention: bad shape (batch %d, %d heads on %d key heads, head width %d: a multiple of 8 up to 256, %d queries, %d keys)", batch, heads,
                kv_heads, dim, nq, nkv);
+  SDMI_REQUIRE(xattn_grid_ok(batch, kv_heads), "cross_attention: grid too large");
   SDMI_REQUIRE(contexts > 0, "cross_attention: %d contexts", contexts);
   SDMI_REQUIRE(index || contexts == 1 || contexts == batch, "cross_attention: %d contexts for a batch of %d need an index", contexts, batch);
   SDMI_REQUIRE(ldq % 8 == 0 && ldk % 8 == 0 && ldv % 8 == 0 && ldo % 4 == 0, "cross_attention: row strides must be multiples of 8");
@@ -475,7 +478,6 @@ extern "C" int sdmi_cross_attention(const void* q, int ldq, int64_t sq, const vo
   p.po = (float*)ws;
   p.pml = pl.splits > 1 ? (float2*)((float*)ws + prows * pl.splits * dim) : nullptr;
   const long long blocks = (long long)batch * kv_heads * pl.rtiles * pl.splits;
-  // a launch has fewer than 2^32 threads
   SDMI_REQUIRE(blocks < (1ll << 24) && (pl.splits == 1 || (prows + 3) / 4 < (1ll << 24)), "cross_attention: grid too large");
   hipStream_t st = (hipStream_t)stream;
   int rc;

@@ -52,6 +52,16 @@ def test_no_cpu_fallback():
         E.lora_gemm(a, torch.zeros((64, 64), dtype=h), 64, pack, torch.zeros(2, dtype=torch.int32))
 
 
+def test_attention_refuses_grids_whose_size_passes_64_bits():
+    """2^64 blocks and more, whose number comes out as 0 or a few."""
+    wide = dict(heads=1 << 18, kv_heads=1 << 18, dim=8, ldq=1 << 21, ldk=1 << 21, ldv=1 << 21, ldo=1 << 21)
+    for change in (dict(wide, batch=1 << 30, nq=1 << 23), dict(wide, batch=(1 << 30) + 1, nq=1 << 23), dict(wide, batch=1 << 30, nq=1 << 24), dict(wide, batch=1 << 24, nq=1)):
+        args = {**ATT, "contexts": 1, **change}
+        with pytest.raises(L.SdmiError, match="grid"):
+            L.call("sdmi_cross_attention", *args.values())
+        assert L.load().sdmi_cross_attention_ws_bytes(args["batch"], args["heads"], args["kv_heads"], args["dim"], args["nq"], args["nkv"]) == 0
+
+
 def test_out_apart_from_operands():
     """An `out` whose columns share memory with an operand is refused, however the two are cut from one storage; the residual may
     be out itself.  (Host tensors: what passes here is refused as such, before any launch.)"""
