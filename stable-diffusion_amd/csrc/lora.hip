@@ -798,6 +798,7 @@ extern "C" int sdmi_lora_gemm(const void* x, int ldx, const void* w, int ldw, vo
                  ((flags & SDMI_F_RESIDUAL) ? (uintptr_t)residual : 0) | ((flags & SDMI_F_BIAS) ? (uintptr_t)bias : 0)) & 15) == 0 &&
                    (((uintptr_t)lora_scale | (uintptr_t)ids) & 3) == 0,
                "lora_gemm: pointer alignment");
+  SDMI_REQUIRE(m > 64 || (n + 15) / 16 < (1 << 23), "lora_gemm: grid too large");  // lora_rows_kernel: a launch has fewer than 2^32 threads
   const int64_t need = sdmi_lora_gemm_ws_bytes(m, n, k, rank, groups, rows_per_id);
   SDMI_REQUIRE(need == 0 || (ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= need), "lora_gemm: workspace of %lld bytes, %lld needed, 16-byte aligned",
                (long long)(ws ? ws_bytes : 0), (long long)need);

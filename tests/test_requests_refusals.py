@@ -62,6 +62,12 @@ def test_attention_refuses_grids_whose_size_passes_64_bits():
         assert L.load().sdmi_cross_attention_ws_bytes(args["batch"], args["heads"], args["kv_heads"], args["dim"], args["nq"], args["nkv"]) == 0
 
 
+@pytest.mark.parametrize("m", [1, 40])
+def test_lora_refuses_a_few_rows_by_too_many_columns(m):
+    with pytest.raises(L.SdmiError, match="grid"):
+        L.call("sdmi_lora_gemm", *{**LORA, "m": m, "n": (1 << 27) - 8, "ldo": 1 << 27}.values())
+
+
 def test_out_apart_from_operands():
     """An `out` whose columns share memory with an operand is refused, however the two are cut from one storage; the residual may
     be out itself.  (Host tensors: what passes here is refused as such, before any launch.)"""
