@@ -451,6 +451,71 @@ def test_lora_kinds(case):
     _close(got, want, tol, "lora %s" % ((per, len(ids)) + LORA_KINDS[case][2:],))
 
 
+def _lora_oracle_by_id(x, w, a, b, scale, ids, per, groups, bias, residual):
+    """_lora_oracle, all rows of an adapter at once."""
+    x, w, a, b = x.double(), w.double(), a.double(), b.double()
+    m, n, r, k = x.shape[0], w.shape[0], b.shape[2], x.shape[1]
+    out, mag, extra = x @ w.t(), x.abs() @ w.abs().t(), torch.zeros(m, n, dtype=torch.float64)
+    row_id = torch.tensor(ids).repeat_interleave(per)
+    for j in sorted({i for i in ids if 0 <= i < a.shape[0]}):
+        rows, sc = torch.nonzero(row_id == j).flatten(), float(scale[j])
+        t, ta = sc * (x[rows] @ a[j].t()), abs(sc) * (x[rows].abs() @ a[j].abs().t())
+        for g in range(groups):
+            c, gr = slice(g * n // groups, (g + 1) * n // groups), slice(g * r, (g + 1) * r)
+            out[rows, c] += t[:, gr] @ b[j, c].t()
+            mag[rows, c] += t[:, gr].abs() @ b[j, c].abs().t()
+            extra[rows, c] = (U * t[:, gr].abs() + TINY + 2 * (k + 4) * E32 * ta[:, gr]) @ b[j, c].abs().t()
+    if bias is not None:
+        out, mag = out + bias.double(), mag + bias.double().abs()
+    if residual is not None:
+        out, mag = out + residual.double(), mag + residual.double().abs()
+    return out, U * out.abs() + TINY + extra + (k + r + 8) * E32 * mag
+
+
+LORA_LONG = [  # every ring and panel refilled several times, the last step of K a partial one
+    # rows per id, ids, k, n, groups, rank, adapters, bias, residual, kernel
+    (4096, [1, 0], 392, 2048, 1, 16, 2, True, False, "lora_gemm_kernel<128, 128, false, 16>"),
+    (4096, [1, -1], 392, 2048, 1, 32, 2, False, True, "lora_gemm_kernel<128, 128, false, 32>"),
+    (2048, [1, 0], 456, 1032, 1, 8, 2, False, True, "lora_gemm_kernel<128, 64, false, 16>"),
+    (2048, [0, 1], 456, 1032, 1, 24, 2, True, False, "lora_gemm_kernel<128, 64, false, 32>"),
+    (600, [0, 1], 648, 136, 1, 16, 2, True, True, "lora_gemm_kernel<64, 64, false, 16>"),
+    (600, [1, 0], 520, 1080, 3, 32, 2, False, False, "lora_gemm_kernel<64, 64, false, 32>"),
+    (576, [0, 1], 648, 136, 1, 64, 2, True, False, "lora_shrink_kernel + lora_gemm_kernel<64, 64, false, 0>"),
+    (600, [1, -1, 0], 520, 264, 3, 72, 2, False, True, "lora_shrink_kernel + lora_gemm_kernel<64, 64, false, 0>"),
+    (2048, [1, 0], 456, 1032, 1, 200, 2, False, False, "lora_shrink_kernel + lora_gemm_kernel<128, 64, false, 0>"),
+    (1, [(i * i) % 6 - 1 for i in range(1155)], 648, 200, 1, 72, 5, True, True, "lora_shrink_kernel + lora_gemm_kernel<64, 64, true, 0>"),
+    (16, [(i * 7) % 9 - 1 for i in range(256)], 520, 1040, 2, 40, 8, False, False, "lora_shrink_kernel + lora_gemm_kernel<128, 64, true, 0>"),
+    (1, [(i * 3) % 5 - 1 for i in range(40)], 2056, 72, 1, 32, 4, True, False, "lora_shrink_kernel + lora_rows_kernel<4, false>"),
+    (2, [(i * 3) % 5 - 1 for i in range(15)], 3080, 72, 1, 40, 4, False, True, "lora_shrink_kernel + lora_rows_kernel<2, false>"),
+    (1, [(i * 3) % 5 - 1 for i in range(12)], 4104, 40, 1, 16, 4, True, True, "lora_shrink_kernel + lora_rows_kernel<1, false>"),
+    (1, [1, 0, -1], 5000, 72, 1, 16, 2, True, False, "lora_rows_kernel<1, true>"),
+    # the low-rank factor by blocks of 64, 32 and 16 rows
+    (4096, [1, 0], 1160, 64, 1, 64, 2, False, False, "lora_shrink_kernel + lora_gemm_kernel<64, 64, false, 0>"),
+    (1152, [0, 1], 2056, 72, 1, 64, 2, True, False, "lora_shrink_kernel + lora_gemm_kernel<64, 64, false, 0>"),
+    (1, [(i * i) % 6 - 1 for i in range(2100)], 1096, 72, 1, 56, 5, False, False, "lora_shrink_kernel + lora_gemm_kernel<64, 64, true, 0>"),
+    (1, [(i * 7) % 3 for i in range(500)], 2120, 72, 1, 24, 3, False, False, "lora_shrink_kernel + lora_gemm_kernel<64, 64, true, 0>"),
+    (1, [(i * 7) % 3 for i in range(70)], 4104, 72, 1, 8, 3, False, False, "lora_shrink_kernel + lora_gemm_kernel<64, 64, true, 0>"),
+]
+
+
+@pytest.mark.parametrize("case", range(len(LORA_LONG)))
+def test_lora_many_steps(case):
+    per, ids, k, n, groups, rank, adapters, bias, residual, kernel = LORA_LONG[case]
+    x, w, a, b, scale, bi, res = _lora_case(300 + case, per * len(ids), k, n, groups, rank, adapters, bias, residual)
+    got = _run_lora(x, w, a, b, scale, ids, bi, res)
+    ran = L.load().sdmi_last_kernel().decode()
+    assert ran == kernel
+    want, tol = _lora_oracle_by_id(x, w, a, b, scale, ids, per, groups, bi, res)
+    _close(got, want, tol, "lora %s" % ((per, len(ids)) + LORA_LONG[case][2:],))
+
+
+def test_the_two_forms_of_the_oracle_agree():
+    args = _lora_case(5, 60, 40, 48, 3, 8, 3, True, True)
+    a, b = (f(*args[:5], [0, -1, 2, 3, 1, 2], 10, 3, *args[5:]) for f in (_lora_oracle, _lora_oracle_by_id))
+    assert torch.allclose(a[0], b[0], rtol=1e-12, atol=1e-12)
+    assert (b[1] >= a[1] - 1e-12).all()                     # a negative scale's bound is its size
+
+
 @pytest.mark.parametrize("m", [3, 40, 200, 1000])
 def test_lora_one_id_for_any_number_of_rows(m):
     x, w, a, b, scale, _, _ = _lora_case(9, m, 64, 72, 1, 16, 3, False, False)
