@@ -182,14 +182,15 @@ class Sampler(object):
         return eps
 
     # one UNet evaluation on the static buffers, eager or replayed
-    def _unet_step(self, xc, t_buf, cc, use_graph, same_halves=False):
+    def _unet_step(self, xc, t_buf, cc, use_graph, same_halves=False, adapters=None):
         """same_halves: the caller guarantees xc[:b] == xc[b:] and equal timesteps (sample() builds them that way), which
-        lets the two CFG halves share the context-free head of the UNet."""
+        lets the two CFG halves share the context-free head of the UNet.  adapters: adapters_of(unet), where the caller has asked
+        already (sample() does once per image)."""
         if not use_graph:
             return self._unet_eval(xc, t_buf, cc, same_halves)
         # the graph is valid while the buffers it read are alive and in place: key on the objects that own them (the
         # sampler keeps xc, the TimeEmb row and the ContextKV alive; a caller's own buffers must outlive the graph)
-        adapters, akey = getattr(self, "_adapters", None) or self.adapters_of(self.unet)
+        adapters, akey = adapters or self.adapters_of(self.unet)
         key = (xc.data_ptr(), t_buf.table.data_ptr() if hasattr(t_buf, "table") else t_buf.data_ptr(), id(cc), tuple(xc.shape), same_halves,
                getattr(self, "_usig", None) or self.weights_signature(self.unet), akey)
         if self._gkey != key:
@@ -212,7 +213,7 @@ class Sampler(object):
         ts, a_t, a_prev, sig, s1m = ddim_schedule(num_ddim_timesteps, eta)
         total = ts.shape[0]
         self._usig = self.weights_signature(self.unet)      # once per image: keys the captured step and the cached tables
-        self._adapters = self.adapters_of(self.unet)
+        adapters = self.adapters_of(self.unet)
         b, _, h, w = x_T.shape
         dev = x_T.device
         xc = self._static_xc((2 * b, 4 + c_concat.shape[1], h, w), dev)
@@ -230,7 +231,7 @@ class Sampler(object):
         for i, step in enumerate(np.flip(ts)):
             index = total - i - 1
             emb_cur.table.copy_(emb_table[i])
-            eps = self._unet_step(xc, emb_cur, cc, use_graph, same_halves=True)   # xc halves are built identical above
+            eps = self._unet_step(xc, emb_cur, cc, use_graph, True, adapters)     # xc halves are built identical above
             if self.cfg_group is not None:
                 from .shard import exchange_cfg_halves
                 exchange_cfg_halves(eps, self.cfg_role, self.cfg_group)

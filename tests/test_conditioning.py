@@ -519,3 +519,23 @@ def test_numbers_past_32_bits_are_not_taken_for_others(monkeypatch):
     for k, q in (([big, 1], 1), ([1, 1], big), ([1, -2 ** 31 - 1], 1)):
         with pytest.raises(L.SdmiError, match="32 bits"):
             sets(k, q)
+
+
+@pytest.mark.gpu
+def test_a_step_behind_an_image_sees_the_adapters_of_now(net):
+    """A captured step asked for by itself, after an image with other adapters."""
+    from stable_diffusion_amd.sampler import Sampler
+    unet, sd = net
+    rs = np.random.RandomState(61)
+    dev = lambda v: v.to(DEV)
+    inp, first, second = make_inputs(2, 16, 2, seed=61), *(AdapterSet(unet, [a]).select([0, 0]) for a in _unet_adapters(rs, sd, 0.3))
+    s = Sampler(unet, None)
+    try:
+        unet.set_adapters(first)
+        s.sample(2, dev(inp["cond"]), dev(inp["uncond"]), dev(inp["c_concat"]), dev(inp["x_T"]), [dev(n) for n in inp["noises"]], 7.5, decode=False, use_graph=True)
+        unet.set_adapters(second)
+        cc = s.make_context(dev(inp["uncond"]), dev(inp["cond"]))
+        want = s._unet_step(s._xc, s._emb_cur, cc, False, same_halves=True).clone()
+        assert torch.equal(s._unet_step(s._xc, s._emb_cur, cc, True, same_halves=True), want)
+    finally:
+        unet.set_adapters(None)
