@@ -32,9 +32,10 @@ class TimeEmb(object):
 
 
 class Unet(nn.Module):
+    adapters = None             # conditioning.AdapterSet (set_adapters)
+
     def __init__(self):
         super().__init__()
-        self.adapters = None        # conditioning.AdapterSet (set_adapters)
         self.emb_channels = MODEL_CH
         temb = MODEL_CH * 4
         self.time_embed = nn.Sequential(nn.Linear(MODEL_CH, temb), nn.SiLU(), nn.Linear(temb, temb))

@@ -126,6 +126,8 @@ def _tokens_out(a, like):
 
 
 class MemoryEfficientCrossAttention(nn.Module):
+    adapters = None     # conditioning.LayerAdapters (AdapterSet.attach); of the class, so that modules saved whole without it load
+
     def __init__(self, query_dim, context_dim=None, heads=8, dim_head=64, dropout=0.):
         super().__init__()
         if dim_head != 64:
@@ -138,7 +140,6 @@ class MemoryEfficientCrossAttention(nn.Module):
         self.to_v = nn.Linear(context_dim, inner, bias=False)
         self.to_out = nn.Sequential(nn.Linear(inner, query_dim), nn.Dropout(dropout))
         self.attention_op = None
-        self.adapters = None        # conditioning.LayerAdapters (AdapterSet.attach)
 
     def _pack(self, kind):
         return None if self.adapters is None else self.adapters.pack(kind)

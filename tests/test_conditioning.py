@@ -539,3 +539,21 @@ def test_a_step_behind_an_image_sees_the_adapters_of_now(net):
         assert torch.equal(s._unet_step(s._xc, s._emb_cur, cc, True, same_halves=True), want)
     finally:
         unet.set_adapters(None)
+
+
+def test_modules_saved_whole_before_there_were_adapters_load():
+    """A module's attributes as torch.save(module) wrote them when layers had no adapters."""
+    import io
+    from Unet import Unet
+    m = _layer()
+    for mod in m.modules():
+        mod.__dict__.pop("adapters", None)
+    buf = io.BytesIO()
+    torch.save(m, buf)
+    buf.seek(0)
+    back = torch.load(buf, weights_only=False)
+    assert all(a._pack(kind) is None for a in (back.transformer_blocks[0].attn1, back.transformer_blocks[0].attn2) for kind in ("qkv", "q", "kv", "out"))
+    with torch.device("meta"):
+        unet = Unet()
+    unet.__dict__.pop("adapters", None)
+    assert unet.adapters is None
