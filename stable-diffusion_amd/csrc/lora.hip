@@ -11,15 +11,15 @@
 // or, where that is cheaper, by the kernel that uses it.  Device times below: MI355X, fp16, operands from HBM.
 //   - up to 64 rows (lora_rows_kernel; one token of each request): the product is a stream over w beside the b rows of each request.
 //     Bound by the chain of memory latencies behind one another (launch, ids, rows, join).  1 row, 1024 x 1024: 5.6 us with t in
-//     the block; 64 rows of 64 adapters of rank 32, 1024 -> 4096 (29 MB): 5.4 us for t and 10.7 for the product, 2.4 TB/s.
+//     the block; 64 rows of 64 adapters of rank 32, 1024 -> 4096: 5.3 us for t and 10.9 for the product, which reads 26 MB at 2.4 TB/s.
 //   - many rows, whole tiles of one request (lora_gemm_kernel, MIXED = false): the adapters are more K.  Ranks up to 32: t is a
 //     by-product of the same K-loop (one launch).  Larger: behind the K-tiles of (x, w) come tiles of (t, b) through the same ring
-//     and MFMAs.  18432 x 640 -> 1920, 3 groups of rank 8: 66 us, 700 TFLOP/s (a library's product alone: 64); MFMAs are busy a third
-//     of the time, the 71 MB that leave at the blocks' ends and 10 K-steps a block cost the rest.  18432 x 320 -> 320: 13.2 us.
-//     2304 x 1280 -> 1280, rank 64: 5.9 us for t, 19 us (460 TFLOP/s), bound by what the LDS delivers to 32 x 32 wave tiles and by
-//     2.8 blocks to a CU (larger tiles: fewer blocks than CUs; measured 20 - 21 us).
+//     and MFMAs.  18432 x 640 -> 1920, 3 groups of rank 8: 65 us, 710 TFLOP/s (a library's product alone: 64); MFMAs are busy a third
+//     of the time, the 71 MB that leave at the blocks' ends and 10 K-steps a block cost the rest.  18432 x 320 -> 320: 13.3 us.
+//     2304 x 1280 -> 1280, rank 64: 5.9 us for t, 18.7 us (424 TFLOP/s; a library's product alone 14.3): 32 x 32 wave tiles read a fragment
+//     for each MFMA, 2.8 blocks to a CU, waves wait a third of the time (larger tiles: fewer blocks than CUs; measured 20 - 21 us).
 //   - many rows of small requests (MIXED = true): the same with tiles over rows in the order of their adapters.  1155 rows, 5
-//     adapters of rank 128, 1024 -> 1024: 9.6 us for t and the order, 12.0 for the product.
+//     adapters of rank 128, 1024 -> 1024: 10.6 us for t and the order, 13.0 for the product.
 #include "common.h"
 #include <atomic>
 #include <type_traits>
@@ -763,7 +763,8 @@ template <int BM, int NSTAGE>
 static int lora_tiles_launch(const LoraParams& p, int kind, hipStream_t st) {
   if (kind == LORA_MIXED) return lora_launch<BM, 64, 2, 2, NSTAGE, true, 0>(p, st);
   if (kind == LORA_TILES) return lora_launch<BM, 64, 2, 2, NSTAGE, false, 0>(p, st);
-  // 128 x 128 tiles, which move a quarter less, once there are four to a CU: 18432 x 1920 66 us against 78, 18432 x 320 14.8 against 14.4
+  // 128 x 128 tiles, which move a quarter less, once there are four to a CU: 18432 x 640 -> 1920 68 us against 78, 9216 x 640 -> 1920 38 against
+  // 41; with fewer 18432 x 320 -> 320 12.4 against 12.1, 18432 x 320 -> 960 28.7 against 27.8 (but 18432 x 640 -> 896 32.7 against 38.7: K counts too)
   if (BM == 128 && (long long)(p.M / 128) * (p.N / 128) >= 1024)
     return p.rank <= 16 ? lora_launch<BM, BM, 2, 2, 2, false, 16>(p, st) : lora_launch<BM, BM, 2, 2, 2, false, 32>(p, st);
   return p.rank <= 16 ? lora_launch<BM, 64, 2, 2, 2, false, 16>(p, st) : lora_launch<BM, 64, 2, 2, 2, false, 32>(p, st);

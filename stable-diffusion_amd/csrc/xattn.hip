@@ -15,12 +15,15 @@
 // through ds_read_b64_tr_b16 in that order).  P is rounded to 16 bits for the matrix cores (half a step of its value);
 // S, m, l and O stay in fp32.
 //
-// What bounds it (MI355X, fp16, device times): long states the exponentials and the rescaled sums, two vector instructions' time
-// for each MFMA's - 2 x 10 heads of 64, 2304 rows to 9216 keys 142 us, 766 TFLOP/s; 96 x 96 rows 310 us, 701; heads of 128 to 4096 keys
-// 126 us, 615; 160: 130 us, 742; 80: 78 us, 616; 256 (one wave to a SIMD): 155 us, 497.  The prompt's lengths the start of a block (Q, the
-// first tile, the store: memory latencies behind one another, two to four blocks to a CU to cover them) - 2 x 5 heads, 9216 rows to
-// 77 keys 11.0 us, 16 x 20 heads, 576 rows to 231 shared keys 22.4 us, 2304 rows to 154 keys in regions 14.2 us.  One row the reading
-// of the keys - 320 rows to 9216 keys (755 MB) 138 + 5 us, 5.3 TB/s; 8 x 16 heads of 128 on 4, 4096 keys (38 MB where half exist) 13.6 + 4 us.
+// What bounds it (MI355X, fp16, device times).  Long states: 9.7 vector instructions beside each MFMA (the exponent's fma and exp2, the
+// maximum, the row sum, the packing), MFMAs busy a third of the time - 2 x 10 heads of 64, 2304 rows to 9216 keys 135 us, 803 TFLOP/s; 96 x 96
+// rows 301 us, 722; heads of 128 to 4096 keys 124 us, 622; 160: 130 us, 744; 80: 75 us, 645; 256 (one wave to a SIMD): 155 us, 498.  That is
+// this loop's form, not the problem's: attn64x2_kernel, for equal lengths and queries that carry log2(e), needs 6.8 and takes 134 and 226
+// us for the first two.  The prompt's lengths: the start of a block (Q, the first tile, the store: memory latencies behind one another, two
+// to four blocks to a CU to cover them) - 2 x 5 heads, 9216 rows to 77 keys 11.3 us, 2304 rows to 154 keys in regions 14.8 us; 16 x 20 heads,
+// 576 rows to 231 shared keys 22.5 us (4.5 blocks of 128 rows, 1.6 rounds of blocks, the last of four tiles on the masked path: 22 vector
+// instructions to an MFMA).  One row: the reading of the keys - 320 rows to 9216 keys (755 MB) 138 + 5 us, 5.3 TB/s; 8 x 16 heads of 128 on 4,
+// 4096 keys (38 MB where half exist) 13.1 + 4.0 us, half of each block's waves without rows.
 #include "common.h"
 #include <atomic>
 
@@ -384,16 +387,19 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(const XattnParams p, lo
 struct XattnPlan { int wk, rtiles, splits; };
 static XattnPlan xattn_plan(int batch, int kvh, int dim, int rows, int nkv) {
   XattnPlan pl;
-  // one wave sweeps all keys for its 32 rows, or two waves share them.  The second gives blocks of 64 rows: fewer of them idle where
-  // there are few, and finer pieces where contexts differ (2304 rows to 9216 keys, heads of 64: 144 us against 175; of 80, to 4096: 78
-  // against 92; of 128: 140 against 124; 2304 rows to 154 keys: 19.7 against 14.8, for the merge is paid per block)
+  // one wave sweeps all keys for its 32 rows, or two waves share them.  The second gives blocks of 64 rows, fewer of them idle where
+  // there are few and finer pieces where contexts differ, and pays a merge for each block.  Measured, one / two, us: heads of 64, 2304
+  // rows to 154 keys 8.7 / 10.1, to 512 13.9 / 13.9, to 2304 42 / 38, to 9216 148 / 133; of 32 and of 80 to 4096 60 / 47 and 84 / 75; of 128 and of 160
+  // 110 / 135 and 121 / 200; 128 heads of 64 to 512 keys, 1 row 11.7 / 10.9, 64 rows 15.6 / 15.1.  Where the rule loses: many blocks over few keys (9216
+  // rows to 512 keys 21.2 / 25.1, to 1024 35.4 / 38.9), few rows to a prompt's (1 row to 77: 5.1 / 5.7, heads of 128 6.4 / 7.5), heads of 256 over 512
+  // keys, which one wave cuts in two pieces (55.8 / 41.9)
   const bool few = rows <= 64;
   pl.wk = few || (dim <= 96 && nkv >= 512) ? 2 : 1;
   const int per = pl.wk == 2 ? 64 : 128;
   pl.rtiles = (rows + per - 1) / per;
   const long long blocks = (long long)batch * kvh * pl.rtiles;
   // few blocks over long states: cut the keys until the chip is full (512 blocks: two per CU), at least 256 keys to a piece.  With
-  // few rows the join is cheap and the quotient is rounded up (320 blocks of one row to 9216 keys: 161 us whole)
+  // few rows the join is cheap and the quotient is rounded up (320 blocks of one row to 9216 keys: 161 us whole, 138 + 5 in pieces)
   long long s = (few ? 511 + blocks : 512) / (blocks > 0 ? blocks : 1);
   if (s > nkv / 256) s = nkv / 256;
   if (s > 64) s = 64;
