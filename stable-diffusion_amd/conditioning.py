@@ -152,18 +152,19 @@ class EncoderStates(object):
                 raise L.SdmiError("EncoderStates.cat: query_regions of %s and %s" % (tuple(a.query_regions.shape), tuple(b.query_regions.shape)))
             kr, qr = torch.cat([pad(keys(a)), pad(keys(b))]), torch.cat([queries(a, ba), queries(b, bb)])
         both = EncoderStates(torch.cat([pad(a.tokens), pad(b.tokens)]), lens_ab, index, kr, qr)
-        both.pair = GuidancePair(a, b)
+        both.pair = GuidancePair(a, b, batch)
         return both
 
 
 class GuidancePair(object):
     """The contexts of the two sides of a guidance batch [uncond | cond], EncoderStates or plain (b, T, C) tokens: how many, whether
-    samples share them, and which sample reads which.  The same for one object that holds both sides and for an object of each."""
+    samples share them, and which sample reads which.  The same for one object that holds both sides and for an object of each.
+    batch: samples of a side, for states that say nothing of it."""
 
-    def __init__(self, uncond, cond):
+    def __init__(self, uncond, cond, batch=None):
         sides = (uncond, cond)
         self.counts = tuple((s.tokens if isinstance(s, EncoderStates) else s).shape[0] for s in sides)
-        self.shared = tuple(isinstance(s, EncoderStates) and s.shared for s in sides)
+        self.shared = tuple(isinstance(s, EncoderStates) and s.shared and not (s.batch is None and batch == 1) for s in sides)
         self._index = tuple(s.index.clone() if shared and s.index is not None else None for s, shared in zip(sides, self.shared))
 
     def alike(self):
@@ -341,9 +342,10 @@ class AdapterSet(object):
             if not pair.shared[s]:
                 if self.ids is None:
                     raise L.SdmiError("AdapterSet: select(ids) first")
-                if self.ids.numel() != 2 * m:
+                # an id for each sample of a side, or of the whole batch [uncond | cond]
+                if self.ids.numel() not in (2 * m, 4 * m):
                     raise L.SdmiError("AdapterSet: %d ids for %d samples" % (self.ids.numel() // 2, m))
-                return self.ids[:m]
+                return self.ids[s * m:(s + 1) * m]
             one = self._one_id(m)
             if one is None:
                 raise L.SdmiError("AdapterSet: samples share the %s contexts, whose to_k / to_v have adapters: say which (select(ids, context_ids), the "

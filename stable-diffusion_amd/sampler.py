@@ -107,7 +107,7 @@ class Sampler(object):
         sig = lambda v: v.signature() if states else (tuple(v.shape), str(v.device))
         key = (sig(uncond), sig(cond), self.dual_stream, self.cfg_group is not None, batch if states else None)
         own = (lambda v: v) if states else (lambda v: v.contiguous())
-        pair = GuidancePair(uncond, cond)                       # adapters of to_k / to_v: ids go by the side
+        pair = GuidancePair(uncond, cond, batch)                # adapters of to_k / to_v: ids go by the side
         if self.cfg_group is not None:
             halves = ((own((uncond, cond)[self.cfg_role]), self.cfg_role),)      # this rank's half only
         elif self.dual_stream:

@@ -557,3 +557,20 @@ def test_modules_saved_whole_before_there_were_adapters_load():
         unet = Unet()
     unet.__dict__.pop("adapters", None)
     assert unet.adapters is None
+
+
+def test_ids_for_the_samples_of_both_sides(monkeypatch):
+    """One id for each sample of [uncond | cond] (no adapter without the prompt, say): each side's contexts go by their own."""
+    s = _set_on_host(monkeypatch).select([-1, -1, 0, 1])
+    plain = torch.zeros(2, 7, 8)
+    assert s.ids_for(4).tolist() == [-1, -1, 0, 1]
+    for uncond, cond in ((plain, plain), (EncoderStates(plain), EncoderStates(plain))):
+        pair = GuidancePair(uncond, cond)
+        assert s.ids_for_contexts(4, False, pair).tolist() == [-1, -1, 0, 1]
+        assert [s.ids_for_contexts(2, False, pair, side).tolist() for side in (0, 1)] == [[-1, -1], [0, 1]]
+    # one sample: its one context of states that fit any batch is its own
+    both = EncoderStates.cat(_side(1), _side(1), batch=1)
+    for pair in (both.pair, GuidancePair(_side(1), _side(1), 1)):
+        assert s.select([-1, 2]).ids_for_contexts(2, both.shared, pair).tolist() == [-1, 2] and s.select([2]).ids_for_contexts(2, both.shared, pair).tolist() == [2, 2]
+    with pytest.raises(L.SdmiError, match="3 ids for 2 samples"):
+        s.select([0, 1, 2]).ids_for_contexts(2, False, GuidancePair(plain, plain), 0)
