@@ -71,7 +71,8 @@ class Sampler(object):
     def adapters_of(module):
         """What of its adapters a captured step has baked in: each layer's (kept alive beside the graph, so that their ids stay
         their own) and the lengths of the sets' ids, which say where those live."""
-        found = [m.adapters for m in module.modules() if hasattr(m, "to_q") and getattr(m, "adapters", None) is not None] if module is not None else []
+        modules = module.modules() if hasattr(module, "modules") else ()
+        found = [m.adapters for m in modules if hasattr(m, "to_q") and getattr(m, "adapters", None) is not None]
         return found, tuple((id(a), 0 if a.owner.ids is None else a.owner.ids.numel()) for a in found)
 
     def _time_tables(self, steps, bc, dev):
@@ -107,7 +108,8 @@ class Sampler(object):
         sig = lambda v: v.signature() if states else (tuple(v.shape), str(v.device))
         key = (sig(uncond), sig(cond), self.dual_stream, self.cfg_group is not None, batch if states else None)
         own = (lambda v: v) if states else (lambda v: v.contiguous())
-        pair = GuidancePair(uncond, cond, batch)                # adapters of to_k / to_v: ids go by the side
+        # adapters of to_k / to_v: ids go by the side
+        sided = {"pair": GuidancePair(uncond, cond, batch)} if self.adapters_of(self.unet)[0] else None
         if self.cfg_group is not None:
             halves = ((own((uncond, cond)[self.cfg_role]), self.cfg_role),)      # this rank's half only
         elif self.dual_stream:
@@ -115,11 +117,11 @@ class Sampler(object):
         else:
             halves = ((EncoderStates.cat(uncond, cond, batch) if states else torch.cat([uncond, cond]).contiguous(), None),)
         if getattr(self, "_cc_key", None) != key:
-            self._cc = tuple(self.unet.precompute_context(h, pair, side) for h, side in halves)
+            self._cc = tuple(self.unet.precompute_context(h, **(dict(sided, side=side) if sided else {})) for h, side in halves)
             self._cc_key = key
         else:
             for c, (h, side) in zip(self._cc, halves):
-                c.update(h, pair, side)
+                c.update(h, **(dict(sided, side=side) if sided else {}))
         return self._cc if (self.dual_stream and self.cfg_group is None) else self._cc[0]
 
     def _static_xc(self, shape, dev):

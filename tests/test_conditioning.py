@@ -574,3 +574,25 @@ def test_ids_for_the_samples_of_both_sides(monkeypatch):
         assert s.select([-1, 2]).ids_for_contexts(2, both.shared, pair).tolist() == [-1, 2] and s.select([2]).ids_for_contexts(2, both.shared, pair).tolist() == [2, 2]
     with pytest.raises(L.SdmiError, match="3 ids for 2 samples"):
         s.select([0, 1, 2]).ids_for_contexts(2, False, GuidancePair(plain, plain), 0)
+
+
+@pytest.mark.parametrize("dual", [True, False])
+def test_sampler_asks_a_model_without_adapters_as_before(dual):
+    """A model of a caller's own whose precompute_context takes the context alone, and whose contexts are updated by it alone."""
+    from stable_diffusion_amd.sampler import Sampler
+
+    class Context(object):
+        def __init__(self, v):
+            self.seen = [v]
+
+        def update(self, v):
+            self.seen.append(v)
+
+    class Net(object):
+        def precompute_context(self, context):
+            return Context(context)
+    s, a, b = Sampler(Net(), None, dual_stream=dual), torch.zeros(2, 7, 8), torch.ones(2, 7, 8)
+    for _ in range(2):
+        cc = s.make_context(a, b)
+    sides = [c.seen for c in cc] if dual else [cc.seen]
+    assert [len(v) for v in sides] == [2] * len(sides) and torch.equal(torch.cat([v[1] for v in sides]), torch.cat([a, b]))
