@@ -13,8 +13,10 @@ from . import engine as E
 def _int32(v, dev, sets=False):
     """Integers as int32 on `dev`, a copy.  Numbers past 32 bits stay past every count that they are compared with; of sets the bits
     count, and a bit past the 32nd is refused."""
-    if v.dtype in (torch.int64, torch.uint32):
+    if v.dtype in (torch.int64, torch.uint32, torch.uint64):
+        past = v.dtype is torch.uint64              # its upper half comes out negative
         v = v.to(device=dev, dtype=torch.int64)
+        v = v.where(v >= 0, 2 ** 63 - 1) if past else v
         if not sets:
             v = v.clamp(-2 ** 31, 2 ** 31 - 1)
         elif v.numel() and not (v.is_cuda and torch.cuda.is_current_stream_capturing()) and bool(((v < -2 ** 31) | (v >= 2 ** 32)).any()):

@@ -596,3 +596,11 @@ def test_sampler_asks_a_model_without_adapters_as_before(dual):
         cc = s.make_context(a, b)
     sides = [c.seen for c in cc] if dual else [cc.seen]
     assert [len(v) for v in sides] == [2] * len(sides) and torch.equal(torch.cat([v[1] for v in sides]), torch.cat([a, b]))
+
+
+def test_unsigned_numbers_past_63_bits_are_past_the_end_too(monkeypatch):
+    s = _set_on_host(monkeypatch)
+    v = np.array([2 ** 64 - 1, 1], dtype=np.uint64)
+    assert EncoderStates(torch.zeros(2, 5, 8), lens=v, index=v).lens.tolist() == [2 ** 31 - 1, 1] and s.select(v).ids_for(2).tolist() == [2 ** 31 - 1, 1]
+    with pytest.raises(L.SdmiError, match="32 bits"):
+        EncoderStates(torch.zeros(1, 2, 8), key_regions=v[None], query_regions=torch.ones(1, 1, 1, dtype=torch.int32))
