@@ -71,8 +71,17 @@ class Sampler(object):
     def adapters_of(module):
         """What of its adapters a captured step has baked in: each layer's (kept alive beside the graph, so that their ids stay
         their own) and the lengths of the sets' ids, which say where those live."""
-        modules = module.modules() if hasattr(module, "modules") else ()
-        found = [m.adapters for m in modules if hasattr(m, "to_q") and getattr(m, "adapters", None) is not None]
+        found = []
+
+        def walk(m):                        # asked twice an image: 0.2 ms for the 663 modules of the UNet (by modules() and hasattr 1.2)
+            children = getattr(m, "_modules", {})
+            if "to_q" in children and getattr(m, "adapters", None) is not None:
+                found.append(m.adapters)
+            for c in children.values():
+                if c is not None:
+                    walk(c)
+        if module is not None:
+            walk(module)
         return found, tuple((id(a), 0 if a.owner.ids is None else a.owner.ids.numel()) for a in found)
 
     def _time_tables(self, steps, bc, dev):
