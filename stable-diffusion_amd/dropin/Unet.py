@@ -163,7 +163,9 @@ class Unet(nn.Module):
         SpatialTransformer up to and including its self-attention.  The two halves of a classifier-free-guidance batch
         share latent, timestep and image conditioning (LatentDiffusionInpainting.py:179-193) and differ only in the
         prompt, so a sampler computes this once and continues it twice: `forward_from_prefix(p, ctx_uncond)` and
-        `forward_from_prefix(p.branch(), ctx_cond)`.  Same kernels on the same shapes: the bits of forward()."""
+        `forward_from_prefix(p.branch(), ctx_cond)`.  Same kernels on the same shapes: the bits of forward()
+        for the first.  A branch sums conv_in's GroupNorm statistics for the last output block anew where conv_in left them (from
+        48 x 48 latents on): equal to rounding there."""
         st = self._begin(x, timesteps)
         first = self.input_blocks[1]
         assert isinstance(first[0], ResBlock) and isinstance(first[1], SpatialTransformer), "unexpected first stage"
